@@ -43,9 +43,10 @@
 extern "C" {
 #endif
 
-#define PCAMD_ABI_VERSION 5 /* 2: pcamd_bmm_scaled_mixed; 3: pcamd_quant_block_ex, pcamd_quant_block_dual_ex;
+#define PCAMD_ABI_VERSION 6 /* 2: pcamd_bmm_scaled_mixed; 3: pcamd_quant_block_ex, pcamd_quant_block_dual_ex;
                               4: PCAMD_F64 scale arithmetic of pcamd_quant_tensor;
-                              5: pcamd_quant_channel_ws, pcamd_quant_tensor_ws */
+                              5: pcamd_quant_channel_ws, pcamd_quant_tensor_ws;
+                              6: pcamd_rms_norm_quant and the pcamd_latent_ functions */
 
 /* status codes */
 #define PCAMD_OK 0
@@ -305,6 +306,100 @@ int pcamd_repack_fp8(const void *x, int64_t batch, int64_t rows,
                      int64_t cols, int64_t sxb, int64_t sxr, int64_t sxc,
                      void *y, int64_t syb, int64_t syr, int64_t syc,
                      void *stream);
+
+/*
+ * Root-mean-square norm with the residual's addition, quantized in 1 x 128
+ * groups: r = x + residual in fp32 (residual may be NULL; otherwise
+ * residual_out, which may be residual or x, receives r in x's type),
+ * v = r * rsqrt(mean(r^2) + norm_eps) * weight over rows of n, and y, scale
+ * as pcamd_quant_block(block_m = 1, block_n = 128) gives for the fp32 v. x,
+ * residual, residual_out, y: [batch, m, n], contiguous along n, any row
+ * strides and alignment; weight: [n] (w_dtype: PCAMD_F32, PCAMD_BF16 or
+ * PCAMD_F16, like x_dtype); scale: [batch, m, ceil(n / 128)]. A NaN stays a
+ * NaN code and does not count in its group's maximum. Available from
+ * PCAMD_ABI_VERSION 6, as the functions below.
+ */
+int pcamd_rms_norm_quant(const void *x, int x_dtype, int64_t batch, int64_t m,
+                         int64_t n, int64_t sxb, int64_t sxm,
+                         const void *residual, int64_t srb, int64_t srm,
+                         const void *weight, int w_dtype, void *y, int y_dtype,
+                         int64_t syb, int64_t sym, float *scale, int64_t ssb,
+                         int64_t ssm, void *residual_out, int64_t sob,
+                         int64_t som, float norm_eps, float fp8_max, float eps,
+                         void *stream);
+
+/*
+ * Writes new tokens into the pages of a latent cache: latent[tokens,
+ * latent_dim], normed as above where weight is given, in the tokens' type
+ * (bf16 or fp16) or as e4m3fn codes with one fp32 scale per 128 columns, and
+ * rope[tokens, rope_dim] as it is. slots (slot_bytes 4 or 8: int32, int64)
+ * holds page * page_size + place per token; a token whose slot is negative or
+ * past pages * page_size is skipped. The cache arrays have a stride per page
+ * (clp, crp, csp) and per token (clt, crt, cst), in elements. latent_dim is a
+ * multiple of 128 up to 512, rope_dim one of 8 up to 512.
+ */
+int pcamd_latent_append(const void *latent, const void *rope, int dtype,
+                        int64_t tokens, int64_t latent_dim, int64_t rope_dim,
+                        int64_t slt, int64_t srt, const void *weight,
+                        int w_dtype, const void *slots, int slot_bytes,
+                        void *cache_latent, int cache_dtype, int64_t clp,
+                        int64_t clt, void *cache_rope, int64_t crp, int64_t crt,
+                        float *cache_scale, int64_t csp, int64_t cst,
+                        int64_t pages, int64_t page_size, float norm_eps,
+                        float eps, void *stream);
+
+/*
+ * Attention of absorbed queries over a latent cache: for new token i of S and
+ * head h, s[t] = softmax_scale * (q_latent . latent[t] + q_rope . rope[t]) over
+ * the tokens t < len - S + i + 1 of the sequence, out = sum_t softmax(s)[t]
+ * latent[t], lse (may be NULL) = log sum_t exp(s[t]); a row that sees no token
+ * gives zeros and -inf. q_latent [batch, S, heads, latent_dim], q_rope
+ * [batch, S, heads, rope_dim], out like q_latent (strides per batch, token and
+ * head); token t of sequence b is place t % page_size of page table[b, t /
+ * page_size]; lens[batch] counts a sequence's tokens. Lengths are cut to
+ * max_pages * page_size and page numbers to the pool. latent_dim and rope_dim
+ * are 512 and 64, or 256 and 32. The workspace (16-byte aligned, contents
+ * ignored and overwritten) has at least pcamd_latent_decode_workspace() bytes;
+ * a negative result of that call is a status.
+ */
+int64_t pcamd_latent_decode_workspace(int64_t batch, int64_t new_tokens,
+                                      int64_t heads, int64_t latent_dim,
+                                      int64_t page_size, int64_t max_pages);
+int pcamd_latent_decode(const void *q_latent, const void *q_rope, int dtype,
+                        int64_t batch, int64_t new_tokens, int64_t heads,
+                        int64_t latent_dim, int64_t rope_dim, int64_t qlb,
+                        int64_t qls, int64_t qlh, int64_t qrb, int64_t qrs,
+                        int64_t qrh, const void *cache_latent, int cache_dtype,
+                        int64_t clp, int64_t clt, const void *cache_rope,
+                        int64_t crp, int64_t crt, const float *cache_scale,
+                        int64_t csp, int64_t cst, int64_t pages,
+                        int64_t page_size, const int32_t *table,
+                        int64_t table_stride, int64_t max_pages,
+                        const int32_t *lens, void *out, int64_t ob, int64_t os,
+                        int64_t oh, float *lse, int64_t lb, int64_t ls,
+                        int64_t lh, float softmax_scale, void *workspace,
+                        int64_t workspace_bytes, void *stream);
+
+/*
+ * Attention of packed sequences with expanded keys: head h of key token t has
+ * the key [k_nope[t, h] | k_rope[t]] and the value v[t, h]; sequence i holds
+ * the queries cu_q[i] .. cu_q[i + 1] - 1 and the keys cu_k[i] .. cu_k[i + 1] -
+ * 1 (offsets beyond the tensors are cut to them). causal: query i of nq sees
+ * the first nk - nq + i + 1 keys of nk. out [total_q, heads, v_dim], lse
+ * [total_q, heads] (may be NULL); queries that see no key, and those behind
+ * the last sequence, give zeros and -inf. nope_dim, rope_dim and v_dim are
+ * 128, 64 and 128, or 64, 32 and 64.
+ */
+int pcamd_latent_prefill(const void *q, const void *k_nope, const void *k_rope,
+                         const void *v, int dtype, int64_t total_q,
+                         int64_t total_k, int64_t heads, int64_t nope_dim,
+                         int64_t rope_dim, int64_t v_dim, int64_t sqt,
+                         int64_t sqh, int64_t skt, int64_t skh, int64_t srt,
+                         int64_t svt, int64_t svh, const int32_t *cu_q,
+                         const int32_t *cu_k, int64_t sequences, void *out,
+                         int64_t sot, int64_t soh, float *lse, int64_t slt,
+                         int64_t slh, float softmax_scale, int causal,
+                         void *stream);
 
 #ifdef __cplusplus
 }

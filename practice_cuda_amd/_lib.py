@@ -50,6 +50,11 @@ EXPORTED_SYMBOLS = (
     "pcamd_bmm_scaled_mixed",
     "pcamd_bmm_quant_a",
     "pcamd_repack_fp8",
+    "pcamd_rms_norm_quant",
+    "pcamd_latent_append",
+    "pcamd_latent_decode_workspace",
+    "pcamd_latent_decode",
+    "pcamd_latent_prefill",
 )
 # test-only entry points (include/pcamd_fp8_selftest.h), exported by the same library
 TEST_SYMBOLS = ("pcamd_selftest_fp8_convert", "pcamd_selftest_copy16", "pcamd_selftest_narrow16")
@@ -109,6 +114,23 @@ def _declare(lib: ctypes.CDLL) -> None:
         + [_ptr] + [_i64] * 3 + [_ptr] + [_i64] * 3 + [_flt, _flt, _int, _ptr])
     lib.pcamd_repack_fp8.restype = _int
     lib.pcamd_repack_fp8.argtypes = [_ptr] + [_i64] * 6 + [_ptr] + [_i64] * 3 + [_ptr]
+    lib.pcamd_rms_norm_quant.restype = _int
+    lib.pcamd_rms_norm_quant.argtypes = (
+        [_ptr, _int] + [_i64] * 5 + [_ptr, _i64, _i64, _ptr, _int] + [_ptr, _int, _i64, _i64] + [_ptr, _i64, _i64] * 2
+        + [_flt, _flt, _flt, _ptr])
+    lib.pcamd_latent_append.restype = _int
+    lib.pcamd_latent_append.argtypes = (
+        [_ptr, _ptr, _int] + [_i64] * 5 + [_ptr, _int, _ptr, _int] + [_ptr, _int, _i64, _i64] + [_ptr, _i64, _i64] * 2
+        + [_i64, _i64, _flt, _flt, _ptr])
+    lib.pcamd_latent_decode_workspace.restype = _i64
+    lib.pcamd_latent_decode_workspace.argtypes = [_i64] * 6
+    lib.pcamd_latent_decode.restype = _int
+    lib.pcamd_latent_decode.argtypes = (
+        [_ptr, _ptr, _int] + [_i64] * 11 + [_ptr, _int, _i64, _i64] + [_ptr, _i64, _i64] * 2 + [_i64, _i64]
+        + [_ptr, _i64, _i64, _ptr] + [_ptr, _i64, _i64, _i64] * 2 + [_flt, _ptr, _i64, _ptr])
+    lib.pcamd_latent_prefill.restype = _int
+    lib.pcamd_latent_prefill.argtypes = (
+        [_ptr] * 4 + [_int] + [_i64] * 13 + [_ptr, _ptr, _i64] + [_ptr, _i64, _i64] * 2 + [_flt, _int, _ptr])
     lib.pcamd_selftest_fp8_convert.restype = _int
     lib.pcamd_selftest_fp8_convert.argtypes = [_int, _ptr, _ptr]
     lib.pcamd_selftest_copy16.restype = _int

@@ -20,7 +20,9 @@ LIB_NAME = "libpcamd_fp8.so"
 LIB_PATH = os.path.join(BUILD_DIR, LIB_NAME)
 SOURCES = ["abi.hip", "quant.hip", "bmm.hip", "bmm_fast.hip", "bmm_wide.hip", "bmm_wide_e5m2.hip",
            "bmm_wide_e5m2_e4m3.hip", "bmm_wide_e4m3_e5m2.hip", "bmm_stream.hip", "bmm_split.hip",
-           "bmm_fused_stream.hip", "repack.hip"]
+           "bmm_fused_stream.hip", "repack.hip", "rms_norm.hip", "latent_decode.hip",
+           "latent_decode_bf16_wide.hip", "latent_decode_bf16_narrow.hip", "latent_decode_f16_wide.hip",
+           "latent_decode_f16_narrow.hip", "latent_prefill.hip"]
 
 ARCH = os.environ.get("PCAMD_OFFLOAD_ARCH", "gfx950")
 

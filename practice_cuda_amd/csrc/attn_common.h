@@ -1,0 +1,148 @@
+// attn_common.h - matrix-instruction tiles shared by the latent attention
+// kernels.
+//
+// Scores are computed transposed, S^T = K Q^T (m = key token, n = query row),
+// and so is the output, O^T = V^T P^T (m = value column, n = query row). Both
+// put a query row on a lane: its maximum and sum are reductions over the
+// lane's own registers and one or two lane exchanges, its rescaling factor is
+// one register, and the registers that hold S^T hold the operand P^T of the
+// second product: the order of tokens within a contraction is free, so V^T is
+// read in the order in which S^T came out. P never leaves the registers.
+//
+// Tiles lie in LDS as rows of 16-byte chunks, chunk c of row t at c ^ f(t):
+// rows that are read together start in different banks.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+#include "fp8_common.h"
+
+namespace pcamd {
+namespace attn {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4* lds_s16x4_ptr;
+
+// Scores are kept times log2(e). The running maximum starts at a finite value
+// below every score that is told apart from -inf, so that a row that has seen
+// nothing (all scores -inf) gets weights exp2(-inf) = 0 and no NaN.
+constexpr float kNoMax = -3.0e38f;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+template <int DT>
+struct Elem;
+template <>
+struct Elem<kBF16> {
+  typedef bf16x8 vec8;
+  static PCAMD_DEV uint32_t narrow2(float a, float b) {
+    const bf16x2 h = {static_cast<__bf16>(a), static_cast<__bf16>(b)};
+    return __builtin_bit_cast(uint32_t, h);
+  }
+  // two fp32 values that the type holds exactly
+  static PCAMD_DEV uint32_t exact2(float a, float b) {
+    return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
+  }
+};
+template <>
+struct Elem<kF16> {
+  typedef f16x8 vec8;
+  static PCAMD_DEV uint32_t narrow2(float a, float b) {
+    const f16x2 h = {static_cast<_Float16>(a), static_cast<_Float16>(b)};
+    return __builtin_bit_cast(uint32_t, h);
+  }
+  static PCAMD_DEV uint32_t exact2(float a, float b) {
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b));
+  }
+};
+
+// MR query rows a wave: one 32x32x16 product, or one 16x16x32. Both take
+// 8 consecutive k per lane and operand; lane = (k group h = lane / MR, row
+// lane % MR). D: n = lane % MR; register quad q holds m = QSTEP q + 4 h + 0..3.
+template <int DT, int MR>
+struct Mfma;
+template <int DT>
+struct Mfma<DT, 32> {
+  typedef f32x16 acc;
+  static constexpr int K = 16, REGS = 16, QSTEP = 8;
+  static PCAMD_DEV acc mul(uint4 a, uint4 b, acc c) {
+    typedef typename Elem<DT>::vec8 v;
+    if constexpr (DT == kBF16)
+      return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v, a), __builtin_bit_cast(v, b), c, 0, 0, 0);
+    else
+      return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v, a), __builtin_bit_cast(v, b), c, 0, 0, 0);
+  }
+};
+template <int DT>
+struct Mfma<DT, 16> {
+  typedef f32x4 acc;
+  static constexpr int K = 32, REGS = 4, QSTEP = 16;
+  static PCAMD_DEV acc mul(uint4 a, uint4 b, acc c) {
+    typedef typename Elem<DT>::vec8 v;
+    if constexpr (DT == kBF16)
+      return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v, a), __builtin_bit_cast(v, b), c, 0, 0, 0);
+    else
+      return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v, a), __builtin_bit_cast(v, b), c, 0, 0, 0);
+  }
+};
+
+// f(t) for rows of CH chunks. ROWS: 16 consecutive rows are read at one chunk
+// (the S^T operand); they have to differ in their place within 256 bytes.
+// Rows of a multiple of 256 bytes: also the four rows t & ~3 .. +3 of a
+// transposing read, 64 bytes each, which bits 2-3 of f tell apart.
+template <int CH>
+PCAMD_DEV int swz(int t) {
+  if constexpr (CH % 16 == 0) return ((t & 3) << 2) | ((t >> 2) & 3);
+  else if constexpr (CH % 8 == 0) return (t >> 1) & 7;
+  else return (t >> 2) & 3;
+}
+// f(t) for values alone (transposing reads only): 128-byte rows
+template <int CH>
+PCAMD_DEV int swz_v(int t) {
+  if constexpr (CH % 16 == 0) return swz<CH>(t);
+  else return ((t >> 1) & 1) << 2;
+}
+
+// Four rows' 16-bit elements of one column, transposed within groups of 16
+// lanes: lane i addresses 8 bytes of row i / 4 at columns 4 (i % 4), and
+// receives column i of the four rows.
+PCAMD_DEV uint2 read_tr4(const uint8_t* p) {
+  return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(p)));
+}
+
+// max / sum over the lane groups that share a row
+template <int MR>
+PCAMD_DEV float row_max(float v) {
+  if constexpr (MR == 16) v = fmaxf(v, __shfl_xor(v, 16, 64));
+  return fmaxf(v, __shfl_xor(v, 32, 64));
+}
+template <int MR>
+PCAMD_DEV float row_sum(float v) {
+  if constexpr (MR == 16) v += __shfl_xor(v, 16, 64);
+  return v + __shfl_xor(v, 32, 64);
+}
+
+// four fp8 codes as two dwords of 16-bit elements (exact)
+template <int DT>
+PCAMD_DEV uint2 widen4(uint32_t c) {
+  const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(c), false);
+  const auto hi = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(c), true);
+  return make_uint2(Elem<DT>::exact2(lo[0], lo[1]), Elem<DT>::exact2(hi[0], hi[1]));
+}
+
+template <int DT>
+PCAMD_DEV void store_elem(void* base, int64_t at, float v) {
+  if constexpr (DT == kBF16) static_cast<__bf16*>(base)[at] = static_cast<__bf16>(v);
+  else static_cast<_Float16*>(base)[at] = static_cast<_Float16>(v);
+}
+
+}  // namespace attn
+}  // namespace pcamd

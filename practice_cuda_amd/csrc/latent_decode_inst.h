@@ -1,0 +1,38 @@
+// latent_decode_inst.h - the decode kernels of one element type and geometry.
+#pragma once
+
+#include <atomic>
+
+#include "abi_util.h"
+#include "latent_decode.h"
+
+namespace pcamd {
+namespace decode {
+
+template <int DT, bool FP8, int DL, int DR, int MR, int WR>
+int launch_shape(const Args& a, hipStream_t st) {
+  static std::atomic<uint64_t> done{0};
+  typedef Kernel<DT, FP8, DL, DR, MR, WR> K;
+  const auto kern = decode_kernel<DT, FP8, DL, DR, MR, WR>;
+  const int rc = ensure_dynamic_lds(reinterpret_cast<const void*>(kern), K::LDS, st, done);
+  if (rc != PCAMD_OK) return rc;
+  kern<<<a.groups, NT, K::LDS, st>>>(a);
+  return check_launch("decode_kernel");
+}
+
+template <int DT, int DL, int DR>
+int launch(const Args& a, Shape shape, bool fp8, hipStream_t st) {
+  int rc;
+  if (shape.mr == 32) rc = fp8 ? launch_shape<DT, true, DL, DR, 32, 4>(a, st) : launch_shape<DT, false, DL, DR, 32, 4>(a, st);
+  else if (shape.wr == 4) rc = fp8 ? launch_shape<DT, true, DL, DR, 16, 4>(a, st) : launch_shape<DT, false, DL, DR, 16, 4>(a, st);
+  else if (shape.wr == 2) rc = fp8 ? launch_shape<DT, true, DL, DR, 16, 2>(a, st) : launch_shape<DT, false, DL, DR, 16, 2>(a, st);
+  else rc = fp8 ? launch_shape<DT, true, DL, DR, 16, 1>(a, st) : launch_shape<DT, false, DL, DR, 16, 1>(a, st);
+  if (rc != PCAMD_OK || !a.parts) return rc;
+  const int64_t rows = a.batch * a.rows;
+  const uint32_t grid = static_cast<uint32_t>(rows < (1 << 20) ? rows : (1 << 20));
+  combine_kernel<DT, DL><<<grid, NT, 0, st>>>(a, shape.tile_rows(), shape.step());
+  return check_launch("combine_kernel");
+}
+
+}  // namespace decode
+}  // namespace pcamd

@@ -1,0 +1,156 @@
+"""rms_norm_quant against its formula in 64 bits.
+
+Tolerances: the kernel's y carries fp32 rounding errors (a row's sum of squares
+is summed pairwise: a relative error well under 1e-6), so a scale is within
+1e-5 of the exact one; a code is the value nearest to y / scale, so its value
+is within half a spacing (2^-4 of y for e4m3fn, 2^-3 for e5m2, half the
+smallest subnormal times the scale below that), the same 1e-5 included."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+import practice_cuda_amd as pca
+
+pytestmark = pytest.mark.gpu
+
+HALF = {torch.float8_e4m3fn: (2.0 ** -4, 2.0 ** -10), torch.float8_e5m2: (2.0 ** -3, 2.0 ** -17)}
+
+
+def formula(x, weight, residual, norm_eps):
+    t = x.double() + (0 if residual is None else residual.double())
+    y = t * torch.rsqrt(t.square().mean(-1, keepdim=True) + norm_eps) * weight.double()
+    return t, y
+
+
+def check(x, weight, residual=None, norm_eps=1e-6, fp8=torch.float8_e4m3fn, eps=1e-12, **kw):
+    t, y = formula(x, weight, residual, norm_eps)
+    q, total = pca.rms_norm_quant(x, weight, residual=residual, norm_eps=norm_eps, fp8_dtype=fp8, eps=eps, **kw)
+    if residual is None:
+        assert total is None
+    else:
+        assert torch.equal(total.double(), t.float().to(x.dtype).double())
+    n = x.shape[-1]
+    fill = -n % 128
+    groups = torch.nn.functional.pad(y, (0, fill)).unflatten(-1, (-1, 128))
+    want = groups.abs().amax(-1).clamp(min=eps) / torch.finfo(fp8).max
+    assert q.dequant_scale.shape == want.shape and q.dequant_scale.dtype == torch.float32
+    torch.testing.assert_close(q.dequant_scale.double(), want, rtol=1e-5, atol=0)
+    assert q.tensor.shape == x.shape and q.tensor.dtype == fp8
+    got = q.dequantize(torch.float64)
+    rel, sub = HALF[fp8]
+    spread = want.repeat_interleave(128, -1)[..., :n]
+    bound = (y.abs() * rel).maximum(spread * sub) * (1 + 1e-4) + 1e-5 * y.abs()
+    assert ((got - y).abs() <= bound).all()
+    return q, total
+
+
+def tensors(dev, shape, dtype, residual, seed=0, wdtype=None):
+    g = torch.Generator(device=dev).manual_seed(seed)
+    x = torch.randn(shape, generator=g, device=dev).to(dtype)
+    w = (1 + 0.1 * torch.randn(shape[-1], generator=g, device=dev)).to(wdtype or dtype)
+    r = (2 * torch.randn(shape, generator=g, device=dev)).to(dtype) if residual else None
+    return x, w, r
+
+
+@pytest.mark.parametrize("n", [1, 7, 8, 127, 128, 129, 512, 513, 1031, 2048, 2056, 4097, 7168, 8200, 16384, 16390,
+                               65536, 65541])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_row_lengths(dev, n, dtype):
+    x, w, r = tensors(dev, (5, n), dtype, True, seed=n)
+    check(x, w, r)
+    check(x, w)
+
+
+@pytest.mark.parametrize("rows", [1, 2, 3, 4, 5, 63, 1000])
+@pytest.mark.parametrize("n", [384, 7168])
+def test_rows(dev, rows, n):
+    x, w, r = tensors(dev, (rows, n), torch.bfloat16, True, seed=rows)
+    check(x, w, r)
+
+
+def test_batches_strides_and_alignment(dev):
+    g = torch.Generator(device=dev).manual_seed(3)
+    buf = torch.randn((4, 9, 1301), generator=g, device=dev).bfloat16()
+    for at, n in ((0, 1300), (1, 1024), (3, 777), (5, 128)):
+        x, r = buf[:3, 1:8, at:at + n], buf[1:, 2:, at:at + n]
+        w = torch.randn(1301, generator=g, device=dev).bfloat16()[at:at + n]
+        check(x, w, r)
+        check(x.transpose(0, 1), w, r.transpose(0, 1))
+
+
+@pytest.mark.parametrize("fp8", [torch.float8_e4m3fn, torch.float8_e5m2])
+@pytest.mark.parametrize("wdtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_types(dev, fp8, wdtype):
+    x, w, r = tensors(dev, (17, 640), torch.bfloat16, True, wdtype=wdtype)
+    check(x, w, r, fp8=fp8, norm_eps=1e-3, eps=1e-3)
+
+
+def test_residual_in_place(dev):
+    x, w, r = tensors(dev, (33, 1024), torch.bfloat16, True)
+    want = (x.float() + r.float()).bfloat16()
+    codes, _ = pca.rms_norm_quant(x, w, residual=r)
+    before = r.clone()
+    q, total = pca.rms_norm_quant(x, w, residual=r, residual_out=r)
+    assert total is r and torch.equal(r, want)
+    assert torch.equal(q.tensor.view(torch.uint8), codes.tensor.view(torch.uint8))
+    q, total = pca.rms_norm_quant(x, w, residual=before, residual_out=x)
+    assert total is x and torch.equal(x, want)
+
+
+def test_zeros_infinities_and_nan(dev):
+    x, w, _ = tensors(dev, (6, 300), torch.bfloat16, False)
+    x[0] = 0
+    x[1, 5] = float("nan")
+    x[2, 200] = float("inf")
+    q, _ = pca.rms_norm_quant(x, w)
+    v = q.tensor.float()
+    assert (v[0] == 0).all() and torch.isfinite(q.dequant_scale[0]).all()
+    assert torch.isnan(v[1]).all()  # the row's mean is one
+    assert torch.isnan(v[2, 200]) and (v[2, :128] == 0).all()  # an infinite mean leaves nothing else
+    check(x[3:], w)
+    w[4] = float("nan")  # a single column
+    q, _ = pca.rms_norm_quant(x[3:], w)
+    bad = torch.isnan(q.tensor.float())
+    assert bad[:, 4].all() and bad.sum() == 3 and torch.isfinite(q.dequant_scale).all()
+
+
+def test_empty(dev):
+    w = torch.ones(256, device=dev)
+    q, _ = pca.rms_norm_quant(torch.empty((0, 256), device=dev), w)
+    assert q.tensor.shape == (0, 256) and q.dequant_scale.shape == (0, 2)
+    q, total = pca.rms_norm_quant(torch.empty((3, 0), device=dev), w[:0], residual=torch.empty((3, 0), device=dev))
+    assert q.tensor.shape == (3, 0) and total.shape == (3, 0)
+
+
+def test_feeds_the_block_product(dev):
+    x, w, r = tensors(dev, (64, 512), torch.bfloat16, True)
+    q, _ = pca.rms_norm_quant(x[None], w, residual=r[None])
+    b = torch.randn((1, 256, 512), device=dev).bfloat16()
+    qb = pca.per_block_quant(b, block_m=128, block_n=128)
+    b_t = pca.QuantResult(qb.tensor.transpose(1, 2), qb.dequant_scale.transpose(1, 2).contiguous(), qb.impl, "block",
+                          {**qb.meta})
+    out = pca.per_block_bmm(q, b_t)
+    want = q.dequantize(torch.float64)[0] @ qb.dequantize(torch.float64)[0].t().contiguous()
+    assert (out[0].double() - want).abs().max() <= 1e-2 * want.abs().max()
+
+
+def test_streams_and_graph(dev):
+    x, w, r = tensors(dev, (64, 1024), torch.bfloat16, True)
+    want, total = pca.rms_norm_quant(x, w, residual=r)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got, _ = pca.rms_norm_quant(x, w, residual=r)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(got.tensor.view(torch.uint8), want.tensor.view(torch.uint8))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got, sums = pca.rms_norm_quant(x, w, residual=r)
+    for k in range(3):
+        x.copy_(torch.randn_like(x))
+        graph.replay()
+        want, total = pca.rms_norm_quant(x, w, residual=r)
+        torch.cuda.synchronize()
+        assert torch.equal(got.tensor.view(torch.uint8), want.tensor.view(torch.uint8))
+        assert torch.equal(got.dequant_scale, want.dequant_scale) and torch.equal(sums, total)
