@@ -47,10 +47,6 @@ struct Elem<kBF16> {
     const bf16x2 h = {static_cast<__bf16>(a), static_cast<__bf16>(b)};
     return __builtin_bit_cast(uint32_t, h);
   }
-  // two fp32 values that the type holds exactly
-  static PCAMD_DEV uint32_t exact2(float a, float b) {
-    return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
-  }
 };
 template <>
 struct Elem<kF16> {
@@ -58,9 +54,6 @@ struct Elem<kF16> {
   static PCAMD_DEV uint32_t narrow2(float a, float b) {
     const f16x2 h = {static_cast<_Float16>(a), static_cast<_Float16>(b)};
     return __builtin_bit_cast(uint32_t, h);
-  }
-  static PCAMD_DEV uint32_t exact2(float a, float b) {
-    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b));
   }
 };
 
@@ -130,12 +123,24 @@ PCAMD_DEV float row_sum(float v) {
   return v + __shfl_xor(v, 32, 64);
 }
 
-// four fp8 codes as two dwords of 16-bit elements (exact)
-template <int DT>
-PCAMD_DEV uint2 widen4(uint32_t c) {
-  const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(c), false);
-  const auto hi = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(c), true);
-  return make_uint2(Elem<DT>::exact2(lo[0], lo[1]), Elem<DT>::exact2(hi[0], hi[1]));
+// Eight rows' bytes of one column: lane i of 16 addresses 8 bytes of row i / 2
+// at columns 8 (i % 2), and receives column i of the eight rows.
+PCAMD_DEV uint2 read_tr8(const uint8_t* p) {
+  typedef int i32x2 __attribute__((ext_vector_type(2)));
+  typedef __attribute__((address_space(3))) i32x2* lds_ptr;
+  return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_ptr)(p)));
+}
+
+// two of four fp8 codes as 16-bit elements (exact: a scale of one)
+template <int DT, bool HI>
+PCAMD_DEV uint32_t widen2(uint32_t c) {
+  if constexpr (DT == kBF16) return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c, 1.0f, HI));
+  else return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(c, 1.0f, HI));
+}
+
+PCAMD_DEV uint32_t lds_addr(const void* p) {
+  return __builtin_amdgcn_readfirstlane(
+      static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const uint8_t*)p)));
 }
 
 template <int DT>

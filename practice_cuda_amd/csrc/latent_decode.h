@@ -30,6 +30,14 @@ using namespace attn;
 constexpr int NT = 256;
 constexpr int TOK = 32;  // tokens of a wave's step
 
+// How far (log2) a score may pass the reference point of its row's weights
+// before the reference moves and the wave's sums are rescaled. Weights and sums
+// are floating point: bf16 and fp32 hold 2^40 as exactly as 1, so the first
+// tile's maximum nearly always stays the reference. fp16 ends at 2^16, and has
+// no room left where an fp8 cache's scales multiply the weights.
+template <int DT, bool FP8>
+constexpr float kSlack = DT == kF16 ? (FP8 ? 0.0f : 8.0f) : 40.0f;
+
 // [first, last) unit of workgroup w, and the workgroup that unit u belongs to
 PCAMD_DEV int64_t first_unit(int64_t w, int64_t units, int64_t groups) { return w * units / groups; }
 PCAMD_DEV int64_t group_of(int64_t u, int64_t units, int64_t groups) { return ((u + 1) * groups - 1) / units; }
@@ -67,7 +75,6 @@ struct Kernel {
   static constexpr int WT = 4 / WR;
   static constexpr int STEP = TOK * WT;
   static constexpr int ROWS = MR * WR;
-  static constexpr int CL = DL / 8, CR = DR / 8;  // chunks of a latent and a rotary row
   static constexpr int GROUPS = DL / 128;
   typedef Mfma<DT, MR> M;
   typedef typename M::acc acc;
@@ -77,49 +84,104 @@ struct Kernel {
   static constexpr int OB = DL / MR;               // blocks of value columns
   static constexpr int PK = TOK / M::K;            // contraction steps of the second product
   static constexpr int LANES_K = 64 / MR;
-  // LDS: latent tile, rotary tile, scales; the epilogue reuses all of it
-  static constexpr int LAT = STEP * DL * 2, ROPE = STEP * DR * 2, SCALES = FP8 ? STEP * GROUPS * 4 : 0;
-  static constexpr int DC = MR == 32 && DL > 256 ? 256 : DL;  // columns of an epilogue pass
+  // A tile of 32 tokens as it lies in LDS: latent rows (in the cache's type),
+  // rotary rows, and with fp8 the scales [group][token].
+  static constexpr int LROW = DL * (FP8 ? 1 : 2), RROW = DR * 2;
+  static constexpr int CL = LROW / 16, CR = RROW / 16;  // 16-byte chunks of a row
+  static constexpr int ROPE = TOK * LROW, SCALES = ROPE + TOK * RROW;
+  static constexpr int TILE = SCALES + (FP8 ? TOK * GROUPS * 4 : 0);
+  // Tiles per token group: all that fit, up to four
+  static constexpr int FIT = 150000 / (WT * TILE);
+  static constexpr int NB = FIT > 4 ? 4 : FIT;
+  static_assert(NB >= (WR > 1 ? 2 : 1), "a shared ring needs two tiles");
+  static constexpr int PAGES = 256;  // page numbers kept in LDS
+  static constexpr int RING = WT * NB * TILE;
+  // epilogue, in the ring's place: DC columns of every row at a time
+  static constexpr int DC = MR == 32 && DL > 256 ? 256 : DL;
   static constexpr int PITCH = DC + 4;
   static constexpr int EPI = 4 * MR * PITCH * 4 + 4 * MR * 8;
-  static constexpr int LDS = LAT + ROPE + SCALES > EPI ? LAT + ROPE + SCALES : EPI;
+  static constexpr int BODY = RING > EPI ? RING : EPI;
+  static constexpr int LDS = BODY + PAGES * 4;
 
-  static PCAMD_DEV void stage(const Args& a, uint8_t* lds, const int32_t* table, int t0, int len) {
-    for (int j = threadIdx.x; j < STEP * CL / (FP8 ? 2 : 1); j += NT) {
-      constexpr int PER = CL / (FP8 ? 2 : 1);
-      const int row = j / PER, c = j % PER, tok = t0 + row;
-      uint4 v = make_uint4(0, 0, 0, 0);
-      const uint8_t* src = nullptr;
-      if (tok < len) {
-        const int64_t page = a.page_of(table, tok);
-        const int64_t at = page * a.slp + a.offset_of(tok) * a.slt;
-        src = static_cast<const uint8_t*>(a.latent) + at * (FP8 ? 1 : 2) + c * 16;
-        v = *reinterpret_cast<const uint4*>(src);
-      }
-      if constexpr (FP8) {
-        const uint2 w0 = widen4<DT>(v.x), w1 = widen4<DT>(v.y), w2 = widen4<DT>(v.z), w3 = widen4<DT>(v.w);
-        uint8_t* d = lds + row * (DL * 2);
-        *reinterpret_cast<uint4*>(d + (((2 * c) ^ swz<CL>(row)) << 4)) = make_uint4(w0.x, w0.y, w1.x, w1.y);
-        *reinterpret_cast<uint4*>(d + (((2 * c + 1) ^ swz<CL>(row)) << 4)) = make_uint4(w2.x, w2.y, w3.x, w3.y);
+  // ---- global -> LDS copies. The WR waves of a token group share a tile's
+  // rows; every wave issues the same number of copies for each tile, so the
+  // count of copies in flight says which tiles have arrived.
+  static constexpr int RW = TOK / WR;                                // a wave's rows of a tile
+  static constexpr int L_COPIES = RW * CL / 64;                      // 64 chunks a copy
+  static constexpr int R_COPIES = (RW * CR + 63) / 64;
+  static constexpr int S_LANES = FP8 ? TOK * GROUPS / WR : 0;        // scales of a wave
+  static constexpr int S_COPIES = (S_LANES + 63) / 64;
+  static constexpr int COPIES = L_COPIES + R_COPIES + S_COPIES;
+  static_assert(L_COPIES * 64 == RW * CL, "whole copies of latent rows");
+
+  // lane i's 16 (4) bytes at p land at lds + 16 i (4 i). Inline asm: the
+  // compiler would wait for every copy in flight before any read of LDS.
+  static PCAMD_DEV void copy16(const void* p, uint32_t lds) {
+    asm volatile("global_load_lds_dwordx4 %0, off" ::"v"(p), "{m0}"(lds) : "memory");
+  }
+  static PCAMD_DEV void copy16(uint32_t off, const void* base, uint32_t lds) {
+    asm volatile("global_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "{m0}"(lds) : "memory");
+  }
+  static PCAMD_DEV void copy4(const void* p, uint32_t lds) {
+    asm volatile("global_load_lds_dword %0, off" ::"v"(p), "{m0}"(lds) : "memory");
+  }
+  template <int N>
+  static PCAMD_DEV void wait_copies() {
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+  }
+
+  struct Source {
+    const int32_t* pages;  // in LDS: the table from page number `first` on
+    int first, len;
+  };
+  // page and place of a token, cut to the sequence's last one: what lies
+  // behind it is not read, and a copy of a row that is seen adds nothing once
+  // its weight is zero
+  static PCAMD_DEV void locate(const Args& a, const Source& src, int t, int64_t& page, int64_t& place) {
+    t = t < src.len ? t : src.len - 1;
+    const int n = a.page_index(t);
+    const uint32_t p = static_cast<uint32_t>(src.pages[n - src.first]);
+    page = p < static_cast<uint64_t>(a.pages) ? p : a.pages - 1;
+    place = t - n * a.page;
+  }
+
+  static PCAMD_DEV void issue(const Args& a, const Source& src, uint32_t tile, int t0, int wr, int lane) {
+    const int row0 = wr * RW;
+    int64_t page, place;
+    locate(a, src, t0 + lane % TOK, page, place);
+    const uint64_t mine = static_cast<uint64_t>(page * a.slp + place * a.slt) * (FP8 ? 1 : 2);
+    const uint32_t lo = static_cast<uint32_t>(mine), hi = static_cast<uint32_t>(mine >> 32);
+    const uint8_t* latent = static_cast<const uint8_t*>(a.latent);
+#pragma unroll
+    for (int i = 0; i < L_COPIES; ++i) {
+      const int r = row0 + i * 64 / CL + (CL < 64 ? lane / CL : 0);  // this lane's row
+      const int c = (lane % CL) ^ swz<16>(r);                        // and chunk
+      const uint32_t to = tile + row0 * LROW + i * 1024;
+      if constexpr (CL == 64) {
+        const uint64_t at = static_cast<uint64_t>(__builtin_amdgcn_readlane(hi, row0 + i)) << 32 |
+                            static_cast<uint32_t>(__builtin_amdgcn_readlane(lo, row0 + i));
+        copy16(16 * c, latent + at, to);
       } else {
-        *reinterpret_cast<uint4*>(lds + row * (DL * 2) + ((c ^ swz<CL>(row)) << 4)) = v;
+        const uint64_t at = static_cast<uint64_t>(static_cast<uint32_t>(__shfl(static_cast<int>(hi), r, 64))) << 32 |
+                            static_cast<uint32_t>(__shfl(static_cast<int>(lo), r, 64));
+        copy16(latent + at + 16 * c, to);
       }
     }
-    for (int j = threadIdx.x; j < STEP * CR; j += NT) {
-      const int row = j / CR, c = j % CR, tok = t0 + row;
-      uint4 v = make_uint4(0, 0, 0, 0);
-      if (tok < len) {
-        const int64_t at = a.page_of(table, tok) * a.srp + a.offset_of(tok) * a.srt;
-        v = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.rope) + at + 8 * c);
+#pragma unroll
+    for (int i = 0; i < R_COPIES; ++i) {
+      const int j = i * 64 + lane, r = row0 + j / CR;
+      if (RW * CR % 64 == 0 || j < RW * CR) {
+        locate(a, src, t0 + r, page, place);
+        const uint16_t* p = static_cast<const uint16_t*>(a.rope) + page * a.srp + place * a.srt;
+        copy16(p + 8 * ((j % CR) ^ swz<CR>(r)), tile + ROPE + row0 * RROW + i * 1024);
       }
-      *reinterpret_cast<uint4*>(lds + LAT + row * (DR * 2) + ((c ^ swz<CR>(row)) << 4)) = v;
     }
-    if constexpr (FP8) {
-      for (int j = threadIdx.x; j < STEP * GROUPS; j += NT) {
-        const int row = j / GROUPS, g = j % GROUPS, tok = t0 + row;
-        float v = 0.0f;
-        if (tok < len) v = a.scale[a.page_of(table, tok) * a.ssp + a.offset_of(tok) * a.sst + g];
-        reinterpret_cast<float*>(lds + LAT + ROPE)[g * STEP + row] = v;
+#pragma unroll
+    for (int i = 0; i < S_COPIES; ++i) {
+      const int j = wr * S_LANES + i * 64 + lane;  // [group][token]
+      if (S_LANES % 64 == 0 || i * 64 + lane < S_LANES) {
+        locate(a, src, t0 + j % TOK, page, place);
+        copy4(a.scale + page * a.ssp + place * a.sst + j / TOK, tile + SCALES + (wr * S_LANES + i * 64) * 4);
       }
     }
   }
@@ -185,95 +247,155 @@ struct Kernel {
     }
   }
 
+  // 8 fp8 codes as 16-bit elements (exact)
+  static PCAMD_DEV uint4 widen8(uint2 c) {
+    return make_uint4(widen2<DT, false>(c.x), widen2<DT, true>(c.x), widen2<DT, false>(c.y), widen2<DT, true>(c.y));
+  }
+
+  struct Lane {
+    int h, ln;
+    // offsets within a tile, without the parts that are the same for all lanes
+    int k[8], kr[4], v[16];
+    PCAMD_DEV explicit Lane(int lane) : h(lane / MR), ln(lane % MR) {
+      const int i16 = lane % 16, g16 = lane / 16;
+#pragma unroll
+      for (int i = 0; i < 16 / LANES_K; ++i) k[i] = ln * LROW + (((i * LANES_K + h) ^ swz<16>(ln)) << 4);
+#pragma unroll
+      for (int i = 0; i < CR / LANES_K; ++i) kr[i] = ROPE + ln * RROW + (((i * LANES_K + h) ^ swz<CR>(ln)) << 4);
+      if constexpr (FP8) {
+        const int q = i16 >> 3, t = q * M::QSTEP + 4 * h + ((i16 >> 1) & 3);
+#pragma unroll
+        for (int i = 0; i < (MR == 32 ? 8 : 16); ++i) {
+          const int c = MR == 32 ? 2 * i + (g16 & 1) : i;
+          v[i] = t * LROW + ((c ^ swz<16>(t)) << 4) + 8 * (i16 & 1);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < (MR == 32 ? 4 : 8); ++i)
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            const int t = q * M::QSTEP + 4 * h + (i16 >> 2);
+            const int c = (MR == 32 ? 4 * i + 2 * (g16 & 1) : 2 * i) + ((i16 >> 1) & 1);
+            v[2 * i + q] = t * LROW + ((c ^ swz<16>(t)) << 4) + 8 * (i16 & 1);
+          }
+      }
+    }
+    // V^T operand: value columns j * MR .., contraction step kk
+    PCAMD_DEV uint4 value(const uint8_t* tile, int j, int kk) const {
+      if constexpr (FP8) {
+        constexpr int P = MR == 32 ? 8 : 16;
+        return widen8(read_tr8(tile + v[j % P] + kk * 16 * LROW + j / P * 256));
+      } else {
+        constexpr int P = MR == 32 ? 4 : 8;
+        const int at = kk * 16 * LROW + j / P * 256;
+        const uint2 x = read_tr4(tile + v[2 * (j % P)] + at), y = read_tr4(tile + v[2 * (j % P) + 1] + at);
+        return make_uint4(x.x, x.y, y.x, y.y);
+      }
+    }
+  };
+
   static PCAMD_DEV void segment(const Args& a, uint8_t* lds, int64_t b, int rt, int s0, int n, int steps, int len,
                                 int64_t slot, int wr, int wt, int h, int ln) {
     const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64;
     const int row = rt * ROWS + wr * MR + ln;  // this lane's row
     const bool live = row < a.rows;
     const int tok_new = live ? row / a.heads : 0, head = live ? row % a.heads : 0;
-    // queries, in registers for the whole segment
+    // Queries, in registers for the whole segment, in the order in which the
+    // keys are read: 16 bytes of a key row a lane (with fp8 two steps' worth).
     uint4 ql[KL], qr[KR];
     {
       const uint16_t* p = static_cast<const uint16_t*>(a.q_latent) + b * a.qlb + tok_new * a.qls + head * a.qlh;
       const uint16_t* r = static_cast<const uint16_t*>(a.q_rope) + b * a.qrb + tok_new * a.qrs + head * a.qrh;
 #pragma unroll
-      for (int k = 0; k < KL; ++k)
-        ql[k] = live ? *reinterpret_cast<const uint4*>(p + k * M::K + 8 * h) : make_uint4(0, 0, 0, 0);
+      for (int k = 0; k < KL; ++k) {
+        const int at = FP8 ? (k / 2 * LANES_K + h) * 16 + k % 2 * 8 : (k * LANES_K + h) * 8;
+        ql[k] = live ? *reinterpret_cast<const uint4*>(p + at) : make_uint4(0, 0, 0, 0);
+      }
 #pragma unroll
       for (int k = 0; k < KR; ++k)
         qr[k] = live ? *reinterpret_cast<const uint4*>(r + k * M::K + 8 * h) : make_uint4(0, 0, 0, 0);
+      // arrived before the loop: a wait inside it would wait for the copies too
+#pragma unroll
+      for (int k = 0; k < KL; ++k) asm volatile("" : "+v"(ql[k].x), "+v"(ql[k].y), "+v"(ql[k].z), "+v"(ql[k].w));
+#pragma unroll
+      for (int k = 0; k < KR; ++k) asm volatile("" : "+v"(qr[k].x), "+v"(qr[k].y), "+v"(qr[k].z), "+v"(qr[k].w));
     }
-    const int limit = live ? len - a.new_tokens + 1 + tok_new : 0;  // tokens this row sees
+    const int limit = live ? len - a.new_tokens + 1 + tok_new : len;  // tokens this row sees
+    const int all_see = len - a.new_tokens + 1;                       // tokens that every row sees
+    const Lane L(lane);
     acc o[OB];
 #pragma unroll
     for (int i = 0; i < OB; ++i) o[i] = acc{};
     float m = kNoMax, l = 0.0f;
-    const int32_t* table = a.table + b * a.table_stride;
-    const float* scales = reinterpret_cast<const float*>(lds + LAT + ROPE);
 
-    for (int i = 0; i < n; ++i) {
-      const int t0 = (s0 + i) * STEP;
-      __syncthreads();
-      stage(a, lds, table, t0, len);
-      __syncthreads();
-      const int tb = t0 + wt * TOK;
-      if (tb >= len) continue;
-      const int lr = wt * TOK;  // first row of this wave's tokens in the tile
-
-      // ---- S^T
+    // ---- one tile of 32 tokens from tb on
+    auto compute = [&](const uint8_t* tile, int tb) {
+      const float* scales = reinterpret_cast<const float*>(tile + SCALES) + 4 * h;
       float s[QUADS * 4];
-      auto operand = [&](int sub, int chunk_pitch, int chunk, const uint8_t* tile, auto f) {
-        const int t = lr + sub * MR + ln;
-        return *reinterpret_cast<const uint4*>(tile + t * (chunk_pitch * 16) + ((chunk ^ f(t)) << 4));
-      };
 #pragma unroll
       for (int sub = 0; sub < SUB; ++sub) {
         acc c = {};
 #pragma unroll
         for (int k = 0; k < KR; ++k)
-          c = M::mul(operand(sub, CR, k * LANES_K + h, lds + LAT, [](int t) { return swz<CR>(t); }), qr[k], c);
+          c = M::mul(*reinterpret_cast<const uint4*>(tile + L.kr[k] + sub * MR * RROW), qr[k], c);
         if constexpr (FP8) {
 #pragma unroll
           for (int g = 0; g < GROUPS; ++g) {
             acc d = {};
 #pragma unroll
-            for (int k = g * (KL / GROUPS); k < (g + 1) * (KL / GROUPS); ++k)
-              d = M::mul(operand(sub, CL, k * LANES_K + h, lds, [](int t) { return swz<CL>(t); }), ql[k], d);
+            for (int k = g * (KL / GROUPS) / 2; k < (g + 1) * (KL / GROUPS) / 2; ++k) {
+              constexpr int P = 16 / LANES_K;
+              const uint4 x = *reinterpret_cast<const uint4*>(tile + L.k[k % P] + sub * MR * LROW + k / P * 256);
+              d = M::mul(widen8(make_uint2(x.x, x.y)), ql[2 * k], d);
+              d = M::mul(widen8(make_uint2(x.z, x.w)), ql[2 * k + 1], d);
+            }
 #pragma unroll
-            for (int r = 0; r < M::REGS; ++r) {
-              const int quad = sub * (M::REGS / 4) + r / 4;
-              c[r] += scales[g * STEP + lr + quad * M::QSTEP + 4 * h + r % 4] * d[r];
+            for (int q = 0; q < M::REGS / 4; ++q) {
+              const float4 f = *reinterpret_cast<const float4*>(scales + g * TOK + (sub * (M::REGS / 4) + q) * M::QSTEP);
+              c[4 * q] += f.x * d[4 * q];
+              c[4 * q + 1] += f.y * d[4 * q + 1];
+              c[4 * q + 2] += f.z * d[4 * q + 2];
+              c[4 * q + 3] += f.w * d[4 * q + 3];
             }
           }
         } else {
 #pragma unroll
-          for (int k = 0; k < KL; ++k)
-            c = M::mul(operand(sub, CL, k * LANES_K + h, lds, [](int t) { return swz<CL>(t); }), ql[k], c);
+          for (int k = 0; k < KL; ++k) {
+            constexpr int P = 16 / LANES_K;
+            c = M::mul(*reinterpret_cast<const uint4*>(tile + L.k[k % P] + sub * MR * LROW + k / P * 256), ql[k], c);
+          }
         }
 #pragma unroll
-        for (int r = 0; r < M::REGS; ++r) s[sub * M::REGS + r] = c[r];
+        for (int r = 0; r < M::REGS; ++r) s[sub * M::REGS + r] = c[r] * a.scale_log2;
       }
 
       // ---- softmax, one row a lane
-      float top = kNoMax;
+      if (tb + TOK > all_see) {
+#pragma unroll
+        for (int r = 0; r < QUADS * 4; ++r)
+          s[r] = tb + (r / 4) * M::QSTEP + 4 * h + r % 4 < limit ? s[r] : -INFINITY;
+      }
+      float top = s[0];
+#pragma unroll
+      for (int r = 1; r < QUADS * 4; ++r) top = fmaxf(top, s[r]);
+      top = row_max<MR>(top);
+      if (__any(top > m + kSlack<DT, FP8>)) {
+        const float to = fmaxf(m, top), alpha = __builtin_amdgcn_exp2f(m - to);
+        m = to;
+        l *= alpha;
+#pragma unroll
+        for (int j = 0; j < OB; ++j) {
+          // block by block through the vector registers, back to where the products keep it
+          asm volatile("" : "+a"(o[j]));
+          o[j] *= alpha;
+          asm volatile("" : "+a"(o[j]));
+        }
+      }
 #pragma unroll
       for (int r = 0; r < QUADS * 4; ++r) {
-        const int t = tb + (r / 4) * M::QSTEP + 4 * h + r % 4;
-        s[r] = t < limit ? s[r] * a.scale_log2 : -INFINITY;
-        top = fmaxf(top, s[r]);
+        s[r] = __builtin_amdgcn_exp2f(s[r] - m);
+        l += s[r];
       }
-      top = fmaxf(row_max<MR>(top), m);
-      const float alpha = exp2f(m - top);
-      m = top;
-      float part = 0.0f;
-#pragma unroll
-      for (int r = 0; r < QUADS * 4; ++r) {
-        s[r] = exp2f(s[r] - m);
-        part += s[r];
-      }
-      l = l * alpha + part;
-#pragma unroll
-      for (int j = 0; j < OB; ++j) o[j] *= alpha;
 
       // ---- O^T += V^T P^T
 #pragma unroll
@@ -283,34 +405,76 @@ struct Kernel {
         for (int kk = 0; kk < PK; ++kk) {
           uint32_t w[4];
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const int r = kk * 8 + 2 * q;
-            float x0 = s[r], x1 = s[r + 1];
+          for (int q = 0; q < 2; ++q) {
+            const int r = kk * 8 + 4 * q;
+            float x0 = s[r], x1 = s[r + 1], x2 = s[r + 2], x3 = s[r + 3];
             if constexpr (FP8) {
-              const float* f = scales + g * STEP + lr + (r / 4) * M::QSTEP + 4 * h + r % 4;
-              x0 *= f[0] * kScaleUp<DT>;
-              x1 *= f[1] * kScaleUp<DT>;
+              const float4 f = *reinterpret_cast<const float4*>(scales + g * TOK + (r / 4) * M::QSTEP);
+              x0 *= f.x * kScaleUp<DT>;
+              x1 *= f.y * kScaleUp<DT>;
+              x2 *= f.z * kScaleUp<DT>;
+              x3 *= f.w * kScaleUp<DT>;
             }
-            w[q] = Elem<DT>::narrow2(x0, x1);
+            w[2 * q] = Elem<DT>::narrow2(x0, x1);
+            w[2 * q + 1] = Elem<DT>::narrow2(x2, x3);
           }
           p[kk] = make_uint4(w[0], w[1], w[2], w[3]);
         }
 #pragma unroll
-        for (int j = g * (FP8 ? OB / GROUPS : OB); j < (g + 1) * (FP8 ? OB / GROUPS : OB); ++j) {
+        for (int j = g * (FP8 ? OB / GROUPS : OB); j < (g + 1) * (FP8 ? OB / GROUPS : OB); ++j)
 #pragma unroll
-          for (int kk = 0; kk < PK; ++kk) {
-            const int i16 = lane % 16, g16 = lane / 16;
-            const int col = j * MR + (MR == 32 ? 16 * (g16 & 1) : 0) + 4 * (i16 & 3);
-            uint2 v[2];
-#pragma unroll
-            for (int q = 0; q < 2; ++q) {
-              const int t = lr + (2 * kk + q) * M::QSTEP + 4 * h + i16 / 4;
-              v[q] = read_tr4(lds + t * (DL * 2) + (((col >> 3) ^ swz<CL>(t)) << 4) + ((col & 4) << 1));
-            }
-            o[j] = M::mul(make_uint4(v[0].x, v[0].y, v[1].x, v[1].y), p[kk], o[j]);
-          }
+          for (int kk = 0; kk < PK; ++kk) o[j] = M::mul(L.value(tile, j, kk), p[kk], o[j]);
+      }
+    };
+
+    // ---- the loop over tiles, window by window of the page table
+    const int32_t* table = a.table + b * a.table_stride;
+    int32_t* pages = reinterpret_cast<int32_t*>(lds + BODY);
+    const uint32_t ring = lds_addr(lds) + wt * NB * TILE;
+    const uint8_t* tiles = lds + wt * NB * TILE;
+    int done = len > 0 ? 0 : n;
+    while (done < n) {
+      const int first_t = (s0 + done) * STEP;
+      Source src{pages, a.page_index(first_t), len};
+      // steps whose tokens all lie within the window's pages (one at least:
+      // a step is at most 128 tokens, the window 256 pages)
+      const int64_t covered = (static_cast<int64_t>(src.first) + PAGES) * a.page;
+      int upto = covered >= len ? n : static_cast<int>(covered / STEP) - s0;
+      if (upto > n) upto = n;
+      __syncthreads();
+      {
+        const int last = a.page_index(len - 1), at = src.first + tid;
+        pages[tid] = table[at < last ? at : last];
+      }
+      __syncthreads();
+      const int count = upto - done;
+      auto start = [&](int i) {  // i: step of this window
+        issue(a, src, ring + i % NB * TILE, (s0 + done + i) * STEP + wt * TOK, wr, lane);
+      };
+      auto wait = [&](int later) {  // copies of `later` further steps may be in flight
+        if (NB > 2 && later >= 2) wait_copies<2 * COPIES <= 63 ? 2 * COPIES : 63>();
+        else if (later == 1) wait_copies<COPIES>();
+        else wait_copies<0>();
+      };
+      constexpr int AHEAD = WR > 1 ? NB - 1 : NB;
+      static_assert(AHEAD <= 3 || WR == 1, "wait() counts up to two further steps");
+      for (int i = 0; i < AHEAD && i < count; ++i) start(i);
+      for (int i = 0; i < count; ++i) {
+        const int later = count - 1 - i < AHEAD - 1 ? count - 1 - i : AHEAD - 1;
+        wait(later);
+        if constexpr (WR > 1) {
+          // the tile is there for all waves, and all have left the one before it
+          asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+          if (i + AHEAD < count) start(i + AHEAD);
+        }
+        const int tb = (s0 + done + i) * STEP + wt * TOK;
+        if (WT == 1 || tb < len) compute(tiles + i % NB * TILE, tb);
+        if constexpr (WR == 1) {
+          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+          if (i + AHEAD < count) start(i + AHEAD);
         }
       }
+      done = upto;
     }
     l = row_sum<MR>(l);
 

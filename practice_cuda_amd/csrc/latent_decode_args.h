@@ -23,15 +23,8 @@ struct Args {
   int groups, min_units;
   int64_t* plan; float* parts; float2* part_ml;
 
-  // the page that holds token t; an entry outside the pool reads some page of it, never past it
-  __device__ __forceinline__ int64_t page_of(const int32_t* row, int t) const {
-    const uint32_t p = static_cast<uint32_t>(row[page_shift >= 0 ? t >> page_shift : t / page]);
-    const int64_t last = pages - 1;
-    return p < pages ? p : last;
-  }
-  __device__ __forceinline__ int64_t offset_of(int t) const {
-    return page_shift >= 0 ? t & (page - 1) : t % page;
-  }
+  // place in the page table of the page that holds token t
+  __device__ __forceinline__ int page_index(int t) const { return page_shift >= 0 ? t >> page_shift : t / page; }
 };
 
 // Rows of a tile and tokens of a step for `rows` rows a sequence: up to 16 (32,
