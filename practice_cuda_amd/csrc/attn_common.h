@@ -87,6 +87,45 @@ struct Mfma<DT, 16> {
   }
 };
 
+// The same product where its sum stays in ordinary vector registers: with 256
+// accumulation registers taken by the output, the compiler would move 16 of
+// them out and back for every tile of scores. The compiler does not see these
+// as matrix instructions, so the waits that it would insert stand here: two
+// wait states ahead of each for operands that an ordinary instruction wrote
+// last, and 12 (settle: 16) between the last of a sum and its first ordinary
+// read. Where other products of this kind follow at once, two of them take
+// longer than that: mul_holding() makes reads of `held` wait for its own issue.
+template <int DT, int MR>
+struct ScoreMfma : Mfma<DT, MR> {
+  typedef typename Mfma<DT, MR>::acc acc;
+  static PCAMD_DEV acc first(uint4 a, uint4 b) { return Mfma<DT, MR>::mul(a, b, acc{}); }
+  static PCAMD_DEV acc mul_holding(uint4 a, uint4 b, acc c, acc&) { return Mfma<DT, MR>::mul(a, b, c); }
+  static PCAMD_DEV void settle(acc&) {}
+};
+template <int DT>
+struct ScoreMfma<DT, 32> {
+  typedef f32x16 acc;
+  typedef typename Elem<DT>::vec8 v;
+#define PCAMD_SCORE_MFMA(C, ...)                                                             \
+  if constexpr (DT == kBF16) asm("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %[a], %[b], " C : __VA_ARGS__); \
+  else asm("s_nop 1\n\tv_mfma_f32_32x32x16_f16 %0, %[a], %[b], " C : __VA_ARGS__)
+  static PCAMD_DEV acc first(uint4 a, uint4 b) {
+    acc c;
+    PCAMD_SCORE_MFMA("0", "=&v"(c) : [a] "v"(__builtin_bit_cast(v, a)), [b] "v"(__builtin_bit_cast(v, b)));
+    return c;
+  }
+  static PCAMD_DEV acc mul(uint4 a, uint4 b, acc c) {
+    PCAMD_SCORE_MFMA("%0", "+v"(c) : [a] "v"(__builtin_bit_cast(v, a)), [b] "v"(__builtin_bit_cast(v, b)));
+    return c;
+  }
+  static PCAMD_DEV acc mul_holding(uint4 a, uint4 b, acc c, acc& held) {
+    PCAMD_SCORE_MFMA("%0", "+v"(c), "+v"(held) : [a] "v"(__builtin_bit_cast(v, a)), [b] "v"(__builtin_bit_cast(v, b)));
+    return c;
+  }
+#undef PCAMD_SCORE_MFMA
+  static PCAMD_DEV void settle(acc& c) { asm volatile("s_nop 15" : "+v"(c)); }
+};
+
 // f(t) for rows of CH chunks. ROWS: 16 consecutive rows are read at one chunk
 // (the S^T operand); they have to differ in their place within 256 bytes.
 // Rows of a multiple of 256 bytes: also the four rows t & ~3 .. +3 of a

@@ -38,6 +38,12 @@ constexpr int TOK = 32;  // tokens of a wave's step
 template <int DT, bool FP8>
 constexpr float kSlack = DT == kF16 ? (FP8 ? 0.0f : 8.0f) : 40.0f;
 
+// Registers that hold operands read ahead of their products, in operands
+template <bool FP8>
+constexpr int kAheadKeys = FP8 ? 4 : 6;
+template <bool FP8>
+constexpr int kAheadValues = 6;
+
 // [first, last) unit of workgroup w, and the workgroup that unit u belongs to
 PCAMD_DEV int64_t first_unit(int64_t w, int64_t units, int64_t groups) { return w * units / groups; }
 PCAMD_DEV int64_t group_of(int64_t u, int64_t units, int64_t groups) { return ((u + 1) * groups - 1) / units; }
@@ -77,6 +83,7 @@ struct Kernel {
   static constexpr int ROWS = MR * WR;
   static constexpr int GROUPS = DL / 128;
   typedef Mfma<DT, MR> M;
+  typedef ScoreMfma<DT, MR> S;
   typedef typename M::acc acc;
   static constexpr int QUADS = TOK / M::QSTEP;     // register quads of a wave's S^T
   static constexpr int SUB = QUADS * 4 / M::REGS;  // S^T products side by side
@@ -101,7 +108,8 @@ struct Kernel {
   static constexpr int PITCH = DC + 4;
   static constexpr int EPI = 4 * MR * PITCH * 4 + 4 * MR * 8;
   static constexpr int BODY = RING > EPI ? RING : EPI;
-  static constexpr int LDS = BODY + PAGES * 4;
+  static constexpr int LDS = BODY + PAGES * 4 + 64;  // and a few words of the division of the work
+  static_assert(TILE % 256 == 0, "see Lane");
 
   // ---- global -> LDS copies. The WR waves of a token group share a tile's
   // rows; every wave issues the same number of copies for each tile, so the
@@ -187,8 +195,8 @@ struct Kernel {
   }
 
   static PCAMD_DEV void run(const Args& a, uint8_t* lds) {
-    __shared__ int64_t wave_total[NT / 64];
-    __shared__ int64_t found[2];
+    int64_t* wave_total = reinterpret_cast<int64_t*>(lds + BODY + PAGES * 4);
+    int64_t* found = wave_total + NT / 64;
     const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64;
     const int wr = wave % WR, wt = wave / WR;
     const int h = lane / MR, ln = lane % MR;
@@ -252,43 +260,45 @@ struct Kernel {
     return make_uint4(widen2<DT, false>(c.x), widen2<DT, true>(c.x), widen2<DT, false>(c.y), widen2<DT, true>(c.y));
   }
 
+  // Where this lane reads in a tile. A row's chunks lie at c ^ f(row), and
+  // tiles start at multiples of 256 bytes, so the place of another chunk
+  // differs by an exclusive or with a constant (within 256 bytes, or a rotary
+  // row) and an added one: three registers serve all reads.
   struct Lane {
     int h, ln;
-    // offsets within a tile, without the parts that are the same for all lanes
-    int k[8], kr[4], v[16];
+    uint32_t k, kr, v;
     PCAMD_DEV explicit Lane(int lane) : h(lane / MR), ln(lane % MR) {
       const int i16 = lane % 16, g16 = lane / 16;
-#pragma unroll
-      for (int i = 0; i < 16 / LANES_K; ++i) k[i] = ln * LROW + (((i * LANES_K + h) ^ swz<16>(ln)) << 4);
-#pragma unroll
-      for (int i = 0; i < CR / LANES_K; ++i) kr[i] = ROPE + ln * RROW + (((i * LANES_K + h) ^ swz<CR>(ln)) << 4);
+      k = ln * LROW + ((h ^ swz<16>(ln)) << 4);
+      kr = ROPE + ln * RROW + ((h ^ swz<CR>(ln)) << 4);
       if constexpr (FP8) {
-        const int q = i16 >> 3, t = q * M::QSTEP + 4 * h + ((i16 >> 1) & 3);
-#pragma unroll
-        for (int i = 0; i < (MR == 32 ? 8 : 16); ++i) {
-          const int c = MR == 32 ? 2 * i + (g16 & 1) : i;
-          v[i] = t * LROW + ((c ^ swz<16>(t)) << 4) + 8 * (i16 & 1);
-        }
+        const int t = (i16 >> 3) * M::QSTEP + 4 * h + ((i16 >> 1) & 3);
+        v = t * LROW + (((MR == 32 ? g16 & 1 : 0) ^ swz<16>(t)) << 4) + 8 * (i16 & 1);
       } else {
-#pragma unroll
-        for (int i = 0; i < (MR == 32 ? 4 : 8); ++i)
-#pragma unroll
-          for (int q = 0; q < 2; ++q) {
-            const int t = q * M::QSTEP + 4 * h + (i16 >> 2);
-            const int c = (MR == 32 ? 4 * i + 2 * (g16 & 1) : 2 * i) + ((i16 >> 1) & 1);
-            v[2 * i + q] = t * LROW + ((c ^ swz<16>(t)) << 4) + 8 * (i16 & 1);
-          }
+        const int t = 4 * h + (i16 >> 2);
+        v = t * LROW + (((MR == 32 ? 2 * (g16 & 1) : 0) + ((i16 >> 1) & 1) ^ swz<16>(t)) << 4) + 8 * (i16 & 1);
       }
     }
-    // V^T operand: value columns j * MR .., contraction step kk
-    PCAMD_DEV uint4 value(const uint8_t* tile, int j, int kk) const {
+    // 16 bytes of a token's latent (rotary) row, as step i reads them; token MR * sub + ln
+    PCAMD_DEV uint4 key(const uint8_t* lds, uint32_t tile, int sub, int i) const {
+      constexpr int P = 16 / LANES_K;
+      return *reinterpret_cast<const uint4*>(lds + ((tile + k) ^ (i % P * LANES_K << 4)) + sub * MR * LROW + i / P * 256);
+    }
+    PCAMD_DEV uint4 rope(const uint8_t* lds, uint32_t tile, int sub, int i) const {
+      return *reinterpret_cast<const uint4*>(lds + ((tile + kr) ^ (i * LANES_K << 4)) + sub * MR * RROW);
+    }
+    // value columns j * MR .. of contraction step kk: raw codes, or the operand itself
+    PCAMD_DEV uint4 value(const uint8_t* lds, uint32_t tile, int j, int kk) const {
       if constexpr (FP8) {
-        constexpr int P = MR == 32 ? 8 : 16;
-        return widen8(read_tr8(tile + v[j % P] + kk * 16 * LROW + j / P * 256));
+        constexpr int P = MR == 32 ? 8 : 16, C = MR / 16;
+        const uint2 x = read_tr8(lds + ((tile + v) ^ (j % P * C << 4)) + kk * 16 * LROW + j / P * 256);
+        return make_uint4(x.x, x.y, 0, 0);
       } else {
-        constexpr int P = MR == 32 ? 4 : 8;
-        const int at = kk * 16 * LROW + j / P * 256;
-        const uint2 x = read_tr4(tile + v[2 * (j % P)] + at), y = read_tr4(tile + v[2 * (j % P) + 1] + at);
+        constexpr int P = MR == 32 ? 4 : 8, C = MR / 8;
+        const uint32_t c = j % P * C;
+        // the second four tokens are QSTEP rows on, whose f differs in bit 1 (MR 32) or not at all
+        const uint2 x = read_tr4(lds + ((tile + v) ^ (c << 4)) + kk * 16 * LROW + j / P * 256);
+        const uint2 y = read_tr4(lds + ((tile + v) ^ ((MR == 32 ? c ^ 2 : c) << 4)) + (kk * 16 + M::QSTEP) * LROW + j / P * 256);
         return make_uint4(x.x, x.y, y.x, y.y);
       }
     }
@@ -329,47 +339,91 @@ struct Kernel {
     float m = kNoMax, l = 0.0f;
 
     // ---- one tile of 32 tokens from tb on
-    auto compute = [&](const uint8_t* tile, int tb) {
-      const float* scales = reinterpret_cast<const float*>(tile + SCALES) + 4 * h;
-      float s[QUADS * 4];
-#pragma unroll
-      for (int sub = 0; sub < SUB; ++sub) {
-        acc c = {};
-#pragma unroll
-        for (int k = 0; k < KR; ++k)
-          c = M::mul(*reinterpret_cast<const uint4*>(tile + L.kr[k] + sub * MR * RROW), qr[k], c);
+    // Reads of LDS run a few steps ahead of the products that take them
+    // (kAhead registers' worth), and sched_barrier keeps them there: left
+    // alone, the scheduler saves registers by waiting for every read.
+    auto compute = [&](uint32_t tile, int tb) {
+      const float* scales = reinterpret_cast<const float*>(lds + tile + SCALES) + 4 * h;
+
+      // ---- S^T: products n = 0 .. NA - 1, rotary steps first
+      constexpr int PER_LOAD = FP8 ? 2 : 1;
+      constexpr int LOADS = KR + KL / PER_LOAD, PER = KR + KL;
+      constexpr int NA = SUB * PER, TA = SUB * LOADS;
+      constexpr int DA = kAheadKeys<FP8> < TA ? kAheadKeys<FP8> : TA;
+      uint4 raw[DA];
+      auto load_key = [&](int i) {
+        const int sub = i / LOADS, r = i % LOADS;
+        return r < KR ? L.rope(lds, tile, sub, r) : L.key(lds, tile, sub, r - KR);
+      };
+      auto load_of = [](int n) { return n / PER * LOADS + (n % PER < KR ? n % PER : KR + (n % PER - KR) / PER_LOAD); };
+      auto operand = [&](int n) {
+        const uint4 x = raw[load_of(n) % DA];
         if constexpr (FP8) {
+          if (n % PER >= KR) return (n % PER - KR) % 2 ? widen8(make_uint2(x.z, x.w)) : widen8(make_uint2(x.x, x.y));
+        }
+        return x;
+      };
 #pragma unroll
-          for (int g = 0; g < GROUPS; ++g) {
-            acc d = {};
+      for (int i = 0; i < DA; ++i) raw[i] = load_key(i);
+      __builtin_amdgcn_sched_barrier(0);
+      acc c[SUB], d[2];
+      uint4 next = operand(0);
 #pragma unroll
-            for (int k = g * (KL / GROUPS) / 2; k < (g + 1) * (KL / GROUPS) / 2; ++k) {
-              constexpr int P = 16 / LANES_K;
-              const uint4 x = *reinterpret_cast<const uint4*>(tile + L.k[k % P] + sub * MR * LROW + k / P * 256);
-              d = M::mul(widen8(make_uint2(x.x, x.y)), ql[2 * k], d);
-              d = M::mul(widen8(make_uint2(x.z, x.w)), ql[2 * k + 1], d);
-            }
-#pragma unroll
-            for (int q = 0; q < M::REGS / 4; ++q) {
-              const float4 f = *reinterpret_cast<const float4*>(scales + g * TOK + (sub * (M::REGS / 4) + q) * M::QSTEP);
-              c[4 * q] += f.x * d[4 * q];
-              c[4 * q + 1] += f.y * d[4 * q + 1];
-              c[4 * q + 2] += f.z * d[4 * q + 2];
-              c[4 * q + 3] += f.w * d[4 * q + 3];
-            }
-          }
+      for (int n = 0; n < NA; ++n) {
+        const int sub = n / PER, r = n % PER;
+        const uint4 x = next;
+        if (n + 1 < NA) {
+          if (load_of(n + 1) != load_of(n) && load_of(n) + DA < TA) raw[load_of(n) % DA] = load_key(load_of(n) + DA);
+          next = operand(n + 1);
+        }
+        if (r < KR) {
+          c[sub] = r == 0 ? S::first(x, qr[0]) : S::mul(x, qr[r], c[sub]);
+        } else if constexpr (!FP8) {
+          c[sub] = S::mul(x, ql[r - KR], c[sub]);
         } else {
+          // a group's partial scores in d, scaled into c while the next group's are summed
+          constexpr int G = KL / GROUPS;
+          const int k = r - KR, g = k / G;
+          if (k % G == 0) d[g & 1] = S::first(x, ql[k]);
+          else if (k % G == 1 && g > 0) d[g & 1] = S::mul_holding(x, ql[k], d[g & 1], d[(g - 1) & 1]);
+          else d[g & 1] = S::mul(x, ql[k], d[g & 1]);
+          auto scale_in = [&](int group, int reg) {
+            const int q = sub * (M::REGS / 4) + reg / 4;
+            const float2 f = *reinterpret_cast<const float2*>(scales + group * TOK + q * M::QSTEP + reg % 4);
+            c[sub][reg] += f.x * d[group & 1][reg];
+            c[sub][reg + 1] += f.y * d[group & 1][reg + 1];
+          };
+          if (g > 0) {
+            // from the group's third product on the last of the group before has been written
 #pragma unroll
-          for (int k = 0; k < KL; ++k) {
-            constexpr int P = 16 / LANES_K;
-            c = M::mul(*reinterpret_cast<const uint4*>(tile + L.k[k % P] + sub * MR * LROW + k / P * 256), ql[k], c);
+            for (int reg = 0; reg < M::REGS; reg += 2)
+              if (2 + reg / 2 * (G - 2) / (M::REGS / 2) == k % G) scale_in(g - 1, reg);
+          }
+          if (r == PER - 1) {
+            S::settle(d[g & 1]);
+#pragma unroll
+            for (int reg = 0; reg < M::REGS; reg += 2) scale_in(g, reg);
           }
         }
-#pragma unroll
-        for (int r = 0; r < M::REGS; ++r) s[sub * M::REGS + r] = c[r] * a.scale_log2;
+        __builtin_amdgcn_sched_barrier(0);
       }
 
+      // ---- the first values are on their way during the softmax
+      constexpr int NP = OB * PK;  // products of the second kind: block n / PK, step n % PK
+      constexpr int DV = kAheadValues<FP8> < NP ? kAheadValues<FP8> : NP;
+      uint4 val[DV];
+#pragma unroll
+      for (int n = 0; n < DV; ++n) val[n] = L.value(lds, tile, n / PK, n % PK);
+      if constexpr (!FP8) {
+#pragma unroll
+        for (int sub = 0; sub < SUB; ++sub) S::settle(c[sub]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+
       // ---- softmax, one row a lane
+      float s[QUADS * 4];
+#pragma unroll
+      for (int r = 0; r < QUADS * 4; ++r) s[r] = c[r / M::REGS][r % M::REGS] * a.scale_log2;
       if (tb + TOK > all_see) {
 #pragma unroll
         for (int r = 0; r < QUADS * 4; ++r)
@@ -398,40 +452,49 @@ struct Kernel {
       }
 
       // ---- O^T += V^T P^T
-#pragma unroll
-      for (int g = 0; g < (FP8 ? GROUPS : 1); ++g) {
-        uint4 p[PK];
-#pragma unroll
-        for (int kk = 0; kk < PK; ++kk) {
-          uint32_t w[4];
-#pragma unroll
-          for (int q = 0; q < 2; ++q) {
-            const int r = kk * 8 + 4 * q;
-            float x0 = s[r], x1 = s[r + 1], x2 = s[r + 2], x3 = s[r + 3];
-            if constexpr (FP8) {
-              const float4 f = *reinterpret_cast<const float4*>(scales + g * TOK + (r / 4) * M::QSTEP);
-              x0 *= f.x * kScaleUp<DT>;
-              x1 *= f.y * kScaleUp<DT>;
-              x2 *= f.z * kScaleUp<DT>;
-              x3 *= f.w * kScaleUp<DT>;
-            }
-            w[2 * q] = Elem<DT>::narrow2(x0, x1);
-            w[2 * q + 1] = Elem<DT>::narrow2(x2, x3);
-          }
-          p[kk] = make_uint4(w[0], w[1], w[2], w[3]);
+      uint32_t p[2][PK * 4];  // P^T of a group of value columns, and of the next
+      auto weights = [&](int g, int i) {  // dword i: registers 2 i and 2 i + 1
+        float x0 = s[2 * i], x1 = s[2 * i + 1];
+        if constexpr (FP8) {
+          const float2 f = *reinterpret_cast<const float2*>(scales + g * TOK + (2 * i / 4) * M::QSTEP + 2 * i % 4);
+          x0 *= f.x * kScaleUp<DT>;
+          x1 *= f.y * kScaleUp<DT>;
         }
+        p[g & 1][i] = Elem<DT>::narrow2(x0, x1);
+      };
 #pragma unroll
-        for (int j = g * (FP8 ? OB / GROUPS : OB); j < (g + 1) * (FP8 ? OB / GROUPS : OB); ++j)
+      for (int i = 0; i < PK * 4; ++i) weights(0, i);
+      auto value_operand = [&](int n) {
+        const uint4 x = val[n % DV];
+        if constexpr (FP8) return widen8(make_uint2(x.x, x.y));
+        else return x;
+      };
+      next = value_operand(0);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-          for (int kk = 0; kk < PK; ++kk) o[j] = M::mul(L.value(tile, j, kk), p[kk], o[j]);
+      for (int n = 0; n < NP; ++n) {
+        constexpr int PER_GROUP = NP / (FP8 ? GROUPS : 1);
+        const int j = n / PK, kk = n % PK, g = n / PER_GROUP;
+        const uint4 x = next;
+        if (n + DV < NP) val[n % DV] = L.value(lds, tile, (n + DV) / PK, (n + DV) % PK);
+        if (n + 1 < NP) next = value_operand(n + 1);
+        const uint32_t* w = p[g & 1] + 4 * kk;
+        o[j] = M::mul(x, make_uint4(w[0], w[1], w[2], w[3]), o[j]);
+        if constexpr (FP8) {
+          if (g + 1 < GROUPS) {
+#pragma unroll
+            for (int i = 0; i < PK * 4; ++i)
+              if (i * PER_GROUP / (PK * 4) == n % PER_GROUP) weights(g + 1, i);
+          }
+        }
+        __builtin_amdgcn_sched_barrier(0);
       }
     };
 
     // ---- the loop over tiles, window by window of the page table
     const int32_t* table = a.table + b * a.table_stride;
     int32_t* pages = reinterpret_cast<int32_t*>(lds + BODY);
-    const uint32_t ring = lds_addr(lds) + wt * NB * TILE;
-    const uint8_t* tiles = lds + wt * NB * TILE;
+    const uint32_t ring = wt * NB * TILE;  // the dynamic LDS starts at address 0 (see decode_kernel)
     int done = len > 0 ? 0 : n;
     while (done < n) {
       const int first_t = (s0 + done) * STEP;
@@ -468,7 +531,7 @@ struct Kernel {
           if (i + AHEAD < count) start(i + AHEAD);
         }
         const int tb = (s0 + done + i) * STEP + wt * TOK;
-        if (WT == 1 || tb < len) compute(tiles + i % NB * TILE, tb);
+        if (WT == 1 || tb < len) compute(ring + i % NB * TILE, tb);
         if constexpr (WR == 1) {
           asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
           if (i + AHEAD < count) start(i + AHEAD);
@@ -536,6 +599,7 @@ struct Kernel {
 
 template <int DT, bool FP8, int DL, int DR, int MR, int WR>
 __global__ __launch_bounds__(NT, 1) void decode_kernel(Args a) {
+  // all of the kernel's LDS, so that it starts at address 0: copies and tile addresses count on it
   extern __shared__ __align__(16) uint8_t lds[];
   Kernel<DT, FP8, DL, DR, MR, WR>::run(a, lds);
 }
