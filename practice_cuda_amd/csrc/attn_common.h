@@ -150,16 +150,24 @@ PCAMD_DEV uint2 read_tr4(const uint8_t* p) {
   return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(p)));
 }
 
-// max / sum over the lane groups that share a row
+// max / sum over the lane groups that share a row: swapping rows of 16 (32)
+// lanes between two copies leaves one group's values in each
+template <int MR, typename F>
+PCAMD_DEV float row_reduce(float v, F f) {
+  if constexpr (MR == 16) {
+    const auto x = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = f(__uint_as_float(x[0]), __uint_as_float(x[1]));
+  }
+  const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return f(__uint_as_float(x[0]), __uint_as_float(x[1]));
+}
 template <int MR>
 PCAMD_DEV float row_max(float v) {
-  if constexpr (MR == 16) v = fmaxf(v, __shfl_xor(v, 16, 64));
-  return fmaxf(v, __shfl_xor(v, 32, 64));
+  return row_reduce<MR>(v, [](float a, float b) { return fmaxf(a, b); });
 }
 template <int MR>
 PCAMD_DEV float row_sum(float v) {
-  if constexpr (MR == 16) v += __shfl_xor(v, 16, 64);
-  return v + __shfl_xor(v, 32, 64);
+  return row_reduce<MR>(v, [](float a, float b) { return a + b; });
 }
 
 // Eight rows' bytes of one column: lane i of 16 addresses 8 bytes of row i / 2
@@ -180,12 +188,6 @@ PCAMD_DEV uint32_t widen2(uint32_t c) {
 PCAMD_DEV uint32_t lds_addr(const void* p) {
   return __builtin_amdgcn_readfirstlane(
       static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const uint8_t*)p)));
-}
-
-template <int DT>
-PCAMD_DEV void store_elem(void* base, int64_t at, float v) {
-  if constexpr (DT == kBF16) static_cast<__bf16*>(base)[at] = static_cast<__bf16>(v);
-  else static_cast<_Float16*>(base)[at] = static_cast<_Float16>(v);
 }
 
 }  // namespace attn

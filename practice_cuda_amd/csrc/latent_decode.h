@@ -12,11 +12,6 @@
 // codes enter the products as they are (16 bits hold them exactly); the scales
 // multiply fp32 values: the four groups' partial scores, and the weights p
 // ahead of their rounding to 16 bits, once for each group of value columns.
-//
-// The work is one list of steps of 32 * WT tokens: for each sequence, for each
-// tile of rows, the steps over its tokens. Workgroup w of G takes the w-th of
-// G equal pieces, whatever the lengths are; pieces of one (sequence, row tile)
-// are joined by combine_kernel through their maxima and sums.
 #pragma once
 
 #include "attn_common.h"
@@ -41,31 +36,40 @@ constexpr float kSlack = DT == kF16 ? (FP8 ? 0.0f : 8.0f) : 40.0f;
 // Registers that hold operands read ahead of their products, in operands
 template <bool FP8>
 constexpr int kAheadKeys = FP8 ? 4 : 6;
-template <bool FP8>
 constexpr int kAheadValues = 6;
 
-// [first, last) unit of workgroup w, and the workgroup that unit u belongs to
-PCAMD_DEV int64_t first_unit(int64_t w, int64_t units, int64_t groups) { return w * units / groups; }
-PCAMD_DEV int64_t group_of(int64_t u, int64_t units, int64_t groups) { return ((u + 1) * groups - 1) / units; }
+// ---------------------------------------------------------------------------
+// The division of the work. One list of units: for each sequence, for each tile
+// of its rows, kFixed units for what a piece costs whatever its length (its
+// queries, its output) and one for each step over the tokens. Workgroup w takes
+// the w-th of `groups` equal pieces of the list, whatever the lengths are; what
+// more than one of them has worked on, combine_kernel joins.
+// ---------------------------------------------------------------------------
+struct Division {
+  int units, groups, q, r;
+  PCAMD_DEV Division(int n, int g) : units(n), groups(g), q(n / g), r(n - n / g * g) {}
+  PCAMD_DEV int first(int w) const { return w * q + (w < r ? w : r); }
+  PCAMD_DEV int group_of(int u) const { return u < r * (q + 1) ? u / (q + 1) : r + (u - r * (q + 1)) / q; }
+};
 
-PCAMD_DEV int length_of(const Args& a, int64_t b) {
+PCAMD_DEV int length_of(const Args& a, int b) {
   const int n = a.lens[b];
   return n < 0 ? 0 : n > a.capacity ? a.capacity : n;
 }
 PCAMD_DEV int steps_of(int len, int step) { return len > step ? (len + step - 1) / step : 1; }
 
 // sum of v over the workgroup's threads before this one, and over all of them
-PCAMD_DEV int64_t block_scan(int64_t v, int64_t* wave_total, int64_t& total) {
+PCAMD_DEV int block_scan(int v, int* wave_total, int& total) {
   const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-  int64_t inc = v;
+  int inc = v;
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) {
-    const int64_t o = __shfl_up(inc, d, 64);
+    const int o = __shfl_up(inc, d, 64);
     if (lane >= d) inc += o;
   }
   if (lane == 63) wave_total[wave] = inc;
   __syncthreads();
-  int64_t before = 0;
+  int before = 0;
   total = 0;
 #pragma unroll
   for (int w = 0; w < NT / 64; ++w) {
@@ -91,44 +95,61 @@ struct Kernel {
   static constexpr int OB = DL / MR;               // blocks of value columns
   static constexpr int PK = TOK / M::K;            // contraction steps of the second product
   static constexpr int LANES_K = 64 / MR;
-  // A tile of 32 tokens as it lies in LDS: latent rows (in the cache's type),
-  // rotary rows, and with fp8 the scales [group][token].
-  static constexpr int LROW = DL * (FP8 ? 1 : 2), RROW = DR * 2;
-  static constexpr int CL = LROW / 16, CR = RROW / 16;  // 16-byte chunks of a row
-  static constexpr int ROPE = TOK * LROW, SCALES = ROPE + TOK * RROW;
+  // A tile of 32 tokens as it lies in LDS: the latent rows in blocks of 128
+  // bytes, [block][token][128 bytes], then the rotary rows as one more block
+  // (half filled where they are 64 bytes), and with fp8 the scales
+  // [group][token].
+  static constexpr int LROW = DL * (FP8 ? 1 : 2), BLOCKS = LROW / 128, BLOCK = TOK * 128;
+  static constexpr int CR = DR / 8;  // 16-byte chunks of a rotary row
+  static constexpr int ROPE = BLOCKS * BLOCK, SCALES = ROPE + BLOCK;
   static constexpr int TILE = SCALES + (FP8 ? TOK * GROUPS * 4 : 0);
   // Tiles per token group: all that fit, up to four
   static constexpr int FIT = 150000 / (WT * TILE);
   static constexpr int NB = FIT > 4 ? 4 : FIT;
   static_assert(NB >= (WR > 1 ? 2 : 1), "a shared ring needs two tiles");
+  static constexpr int AHEAD = WR > 1 ? NB - 1 : NB;  // tiles on their way or in use
+  // The 128-row kernel of a 16-bit cache overlaps one tile's softmax with the
+  // next one's scores; it has the registers for it.
+  static constexpr bool PIPE = MR == 32 && !FP8;
+  static_assert(!PIPE || NB == 4, "the overlapped loop holds two tiles while two more are on their way");
   static constexpr int PAGES = 256;  // page numbers kept in LDS
   static constexpr int RING = WT * NB * TILE;
   // epilogue, in the ring's place: DC columns of every row at a time
   static constexpr int DC = MR == 32 && DL > 256 ? 256 : DL;
   static constexpr int PITCH = DC + 4;
-  static constexpr int EPI = 4 * MR * PITCH * 4 + 4 * MR * 8;
+  static constexpr int EPI = 4 * MR * PITCH * 4 + 4 * MR * 8 + ROWS * 8;
   static constexpr int BODY = RING > EPI ? RING : EPI;
   static constexpr int LDS = BODY + PAGES * 4 + 64;  // and a few words of the division of the work
-  static_assert(TILE % 256 == 0, "see Lane");
 
-  // ---- global -> LDS copies. The WR waves of a token group share a tile's
-  // rows; every wave issues the same number of copies for each tile, so the
-  // count of copies in flight says which tiles have arrived.
-  static constexpr int RW = TOK / WR;                                // a wave's rows of a tile
-  static constexpr int L_COPIES = RW * CL / 64;                      // 64 chunks a copy
-  static constexpr int R_COPIES = (RW * CR + 63) / 64;
-  static constexpr int S_LANES = FP8 ? TOK * GROUPS / WR : 0;        // scales of a wave
-  static constexpr int S_COPIES = (S_LANES + 63) / 64;
-  static constexpr int COPIES = L_COPIES + R_COPIES + S_COPIES;
-  static_assert(L_COPIES * 64 == RW * CL, "whole copies of latent rows");
-
-  // lane i's 16 (4) bytes at p land at lds + 16 i (4 i). Inline asm: the
-  // compiler would wait for every copy in flight before any read of LDS.
-  static PCAMD_DEV void copy16(const void* p, uint32_t lds) {
-    asm volatile("global_load_lds_dwordx4 %0, off" ::"v"(p), "{m0}"(lds) : "memory");
+  // Chunk c of row t lies at c ^ f(t). Rows are 128 bytes apart, so t & 1 is a
+  // half of the 256 bytes that 16 lanes may read without conflict, and the rest
+  // of t has to spread 16 consecutive rows' equal chunks (keys) over all eight
+  // places, and what a transposing read takes at once over disjoint ones:
+  //   16-bit values: rows 4 h .. + 3 (MR 32: 64 bytes each; MR 16, two h: 32
+  //   bytes each) - the reversed bits of t / 2;
+  //   8-bit values: rows 4 h .. + 3 and QSTEP further on, 32 (16) bytes each.
+  static PCAMD_DEV int swizzle(int t) {
+    const int u = t >> 1;
+    if constexpr (FP8) return ((u & 1) << 2) | ((((u >> 2) ^ (u >> 3)) & 1) << 1) | ((u >> 1) & 1);
+    else return ((u & 1) << 2) | (u & 2) | ((u >> 2) & 1);
   }
-  static PCAMD_DEV void copy16(uint32_t off, const void* base, uint32_t lds) {
-    asm volatile("global_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "{m0}"(lds) : "memory");
+
+  // ---- global -> LDS copies: 8 rows x 128 bytes each. The WR waves of a token
+  // group share a tile's rows, and every wave issues the same number of copies
+  // for every tile (past the last one too, of rows it has already), so a count
+  // of copies in flight says which tiles have arrived.
+  static constexpr int RW = TOK / WR, RR = RW / 8;             // a wave's rows of a tile, in eights
+  static constexpr int S_LANES = FP8 ? TOK * GROUPS / WR : 0;  // scales of a wave
+  static constexpr int S_COPIES = (S_LANES + 63) / 64;
+  static constexpr int COPIES = RR * (BLOCKS + 1) + S_COPIES;
+  static_assert((AHEAD - 1) * COPIES < 64, "the counter of copies in flight ends at 63");
+
+  // lane i's 16 (4) bytes at p + OFF land at lds + 16 i (4 i). Inline asm: the
+  // compiler would wait for every copy in flight before any read of LDS. The
+  // instruction adds its offset to both addresses.
+  template <int OFF>
+  static PCAMD_DEV void copy16(const void* p, uint32_t lds) {
+    asm volatile("global_load_lds_dwordx4 %0, off offset:%2" ::"v"(p), "{m0}"(lds - OFF), "n"(OFF) : "memory");
   }
   static PCAMD_DEV void copy4(const void* p, uint32_t lds) {
     asm volatile("global_load_lds_dword %0, off" ::"v"(p), "{m0}"(lds) : "memory");
@@ -140,178 +161,218 @@ struct Kernel {
 
   struct Source {
     const int32_t* pages;  // in LDS: the table from page number `first` on
-    int first, len;
+    int first, last;       // last: the last token that they and the sequence hold
   };
-  // page and place of a token, cut to the sequence's last one: what lies
-  // behind it is not read, and a copy of a row that is seen adds nothing once
-  // its weight is zero
-  static PCAMD_DEV void locate(const Args& a, const Source& src, int t, int64_t& page, int64_t& place) {
-    t = t < src.len ? t : src.len - 1;
+  // Page and place of a token, cut to the last one: what lies behind it is not
+  // read, and a row that is there twice adds nothing, its second weight is zero.
+  static PCAMD_DEV void locate(const Args& a, const Source& src, int t, uint32_t& page, uint32_t& place) {
+    t = t < src.last ? t : src.last;
     const int n = a.page_index(t);
-    const uint32_t p = static_cast<uint32_t>(src.pages[n - src.first]);
-    page = p < static_cast<uint64_t>(a.pages) ? p : a.pages - 1;
+    page = static_cast<uint32_t>(src.pages[n - src.first]);
+    page = page < a.pages ? page : a.pages - 1;
     place = t - n * a.page;
   }
 
-  static PCAMD_DEV void issue(const Args& a, const Source& src, uint32_t tile, int t0, int wr, int lane) {
-    const int row0 = wr * RW;
-    int64_t page, place;
-    locate(a, src, t0 + lane % TOK, page, place);
-    const uint64_t mine = static_cast<uint64_t>(page * a.slp + place * a.slt) * (FP8 ? 1 : 2);
-    const uint32_t lo = static_cast<uint32_t>(mine), hi = static_cast<uint32_t>(mine >> 32);
-    const uint8_t* latent = static_cast<const uint8_t*>(a.latent);
+  // the addresses of a tile's copies, and the copies
+  struct Copies {
+    const uint8_t* latent[RR];
+    const uint8_t* rope[RR];
+    const float* scale[S_COPIES > 0 ? S_COPIES : 1];
+
+    PCAMD_DEV void prepare(const Args& a, const Source& src, int t0, int wr, int lane) {
 #pragma unroll
-    for (int i = 0; i < L_COPIES; ++i) {
-      const int r = row0 + i * 64 / CL + (CL < 64 ? lane / CL : 0);  // this lane's row
-      const int c = (lane % CL) ^ swz<16>(r);                        // and chunk
-      const uint32_t to = tile + row0 * LROW + i * 1024;
-      if constexpr (CL == 64) {
-        const uint64_t at = static_cast<uint64_t>(__builtin_amdgcn_readlane(hi, row0 + i)) << 32 |
-                            static_cast<uint32_t>(__builtin_amdgcn_readlane(lo, row0 + i));
-        copy16(16 * c, latent + at, to);
-      } else {
-        const uint64_t at = static_cast<uint64_t>(static_cast<uint32_t>(__shfl(static_cast<int>(hi), r, 64))) << 32 |
-                            static_cast<uint32_t>(__shfl(static_cast<int>(lo), r, 64));
-        copy16(latent + at + 16 * c, to);
+      for (int i = 0; i < RR; ++i) {
+        const int row = wr * RW + 8 * i + lane / 8, c = (lane % 8) ^ swizzle(row);
+        uint32_t page, place;
+        locate(a, src, t0 + row, page, place);
+        latent[i] = static_cast<const uint8_t*>(a.latent) +
+                    (uint64_t{page} * a.slp + uint64_t{place} * a.slt) * (FP8 ? 1 : 2) + 16 * c;
+        rope[i] = c < CR ? static_cast<const uint8_t*>(a.rope) + (uint64_t{page} * a.srp + uint64_t{place} * a.srt) * 2 + 16 * c
+                         : nullptr;
       }
-    }
 #pragma unroll
-    for (int i = 0; i < R_COPIES; ++i) {
-      const int j = i * 64 + lane, r = row0 + j / CR;
-      if (RW * CR % 64 == 0 || j < RW * CR) {
-        locate(a, src, t0 + r, page, place);
-        const uint16_t* p = static_cast<const uint16_t*>(a.rope) + page * a.srp + place * a.srt;
-        copy16(p + 8 * ((j % CR) ^ swz<CR>(r)), tile + ROPE + row0 * RROW + i * 1024);
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < S_COPIES; ++i) {
-      const int j = wr * S_LANES + i * 64 + lane;  // [group][token]
-      if (S_LANES % 64 == 0 || i * 64 + lane < S_LANES) {
+      for (int i = 0; i < S_COPIES; ++i) {
+        const int j = wr * S_LANES + i * 64 + lane;  // [group][token]
+        uint32_t page, place;
         locate(a, src, t0 + j % TOK, page, place);
-        copy4(a.scale + page * a.ssp + place * a.sst + j / TOK, tile + SCALES + (wr * S_LANES + i * 64) * 4);
+        scale[i] = a.scale + uint64_t{page} * a.ssp + uint64_t{place} * a.sst + j / TOK;
       }
     }
-  }
-
-  static PCAMD_DEV void run(const Args& a, uint8_t* lds) {
-    int64_t* wave_total = reinterpret_cast<int64_t*>(lds + BODY + PAGES * 4);
-    int64_t* found = wave_total + NT / 64;
-    const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64;
-    const int wr = wave % WR, wt = wave / WR;
-    const int h = lane / MR, ln = lane % MR;
-
-    // ---- this workgroup's piece of the list
-    int64_t sum = 0, units;
-    for (int64_t b = tid; b < a.batch; b += NT) sum += steps_of(length_of(a, b), STEP);
-    block_scan(sum, wave_total, units);
-    units *= a.row_tiles;
-    int64_t groups = (units + a.min_units - 1) / a.min_units;
-    if (groups > a.groups) groups = a.groups;
-    if (blockIdx.x == 0 && tid == 0 && a.parts) {
-      a.plan[0] = units;
-      a.plan[1] = groups;
-    }
-    const bool writes_plan = blockIdx.x == 0 && a.parts;
-    const int64_t w = blockIdx.x;
-    if (w >= groups) return;
-    int64_t u = first_unit(w, units, groups);
-    const int64_t end = first_unit(w + 1, units, groups);
-    const int64_t begin = u;
-    int64_t base = 0;
-    if (tid == 0) found[0] = -1;
-    __syncthreads();
-    for (int64_t b0 = 0; b0 < a.batch; b0 += NT) {
-      const int64_t b = b0 + tid;
-      const int64_t mine = b < a.batch ? int64_t{steps_of(length_of(a, b), STEP)} * a.row_tiles : 0;
-      int64_t total;
-      const int64_t before = base + block_scan(mine, wave_total, total);
-      if (b < a.batch) {
-        if (writes_plan) a.plan[2 + b] = before;
-        if (u >= before && u < before + mine) {
-          found[0] = b;
-          found[1] = u - before;
-        }
-      }
-      base += total;
-      __syncthreads();
-      if (found[0] >= 0 && !writes_plan) break;
-    }
-    int64_t b = found[0], in_seq = found[1];
-
-    while (u < end) {
-      const int len = length_of(a, b);
-      const int steps = steps_of(len, STEP);
-      const int rt = static_cast<int>(in_seq / steps), s0 = static_cast<int>(in_seq % steps);
-      const int64_t left = end - u;
-      const int n = left < steps - s0 ? static_cast<int>(left) : steps - s0;
-      segment(a, lds, b, rt, s0, n, steps, len, u == begin ? 2 * w : 2 * w + 1, wr, wt, h, ln);
-      u += n;
-      in_seq += n;
-      if (in_seq >= int64_t{steps} * a.row_tiles) {
-        ++b;
-        in_seq = 0;
+    // copy k of COPIES into the tile at LDS address `tile`
+    template <int K>
+    PCAMD_DEV void emit(uint32_t tile, int wr, int lane) const {
+      if constexpr (K < RR * BLOCKS) {
+        constexpr int i = K / BLOCKS, b = K % BLOCKS;
+        copy16<b * 128>(latent[i], tile + b * BLOCK + (wr * RW + 8 * i) * 128);
+      } else if constexpr (K < RR * (BLOCKS + 1)) {
+        constexpr int i = K - RR * BLOCKS;
+        if (CR == 8 || rope[i]) copy16<0>(rope[i], tile + ROPE + (wr * RW + 8 * i) * 128);
+      } else {
+        constexpr int i = K - RR * (BLOCKS + 1);
+        if (S_LANES % 64 == 0 || i * 64 + lane < S_LANES) copy4(scale[i], tile + SCALES + (wr * S_LANES + i * 64) * 4);
       }
     }
-  }
+    template <int K = 0>
+    PCAMD_DEV void emit_all(uint32_t tile, int wr, int lane) const {
+      if constexpr (K < COPIES) {
+        emit<K>(tile, wr, lane);
+        emit_all<K + 1>(tile, wr, lane);
+      }
+    }
+    // the copies that step n of `steps` gives time for: from step 4 on, evenly
+    template <int K = 0>
+    PCAMD_DEV void emit_at(int n, int steps, uint32_t tile, int wr, int lane) const {
+      if constexpr (K < COPIES) {
+        if (4 + K * (steps - 5) / COPIES == n) emit<K>(tile, wr, lane);
+        emit_at<K + 1>(n, steps, tile, wr, lane);
+      }
+    }
+  };
 
   // 8 fp8 codes as 16-bit elements (exact)
   static PCAMD_DEV uint4 widen8(uint2 c) {
     return make_uint4(widen2<DT, false>(c.x), widen2<DT, true>(c.x), widen2<DT, false>(c.y), widen2<DT, true>(c.y));
   }
 
-  // Where this lane reads in a tile. A row's chunks lie at c ^ f(row), and
-  // tiles start at multiples of 256 bytes, so the place of another chunk
-  // differs by an exclusive or with a constant (within 256 bytes, or a rotary
-  // row) and an added one: three registers serve all reads.
+  // Where this lane reads in a tile. Chunks of a row lie at c ^ f(row), so
+  // another chunk's place differs by an exclusive or with a constant (bits 4-6
+  // of the address), another block's by a constant to add.
   struct Lane {
     int h, ln;
-    uint32_t k, kr, v;
+    uint32_t k, v;
     PCAMD_DEV explicit Lane(int lane) : h(lane / MR), ln(lane % MR) {
       const int i16 = lane % 16, g16 = lane / 16;
-      k = ln * LROW + ((h ^ swz<16>(ln)) << 4);
-      kr = ROPE + ln * RROW + ((h ^ swz<CR>(ln)) << 4);
-      if constexpr (FP8) {
-        const int t = (i16 >> 3) * M::QSTEP + 4 * h + ((i16 >> 1) & 3);
-        v = t * LROW + (((MR == 32 ? g16 & 1 : 0) ^ swz<16>(t)) << 4) + 8 * (i16 & 1);
-      } else {
-        const int t = 4 * h + (i16 >> 2);
-        v = t * LROW + (((MR == 32 ? 2 * (g16 & 1) : 0) + ((i16 >> 1) & 1) ^ swz<16>(t)) << 4) + 8 * (i16 & 1);
-      }
+      k = ln * 128 + ((h ^ swizzle(ln)) << 4);
+      // the transposing read's row, and its chunk's part that is the lane's
+      const int t = FP8 ? (i16 >> 3) * M::QSTEP + 4 * h + ((i16 >> 1) & 3) : 4 * h + (i16 >> 2);
+      const int c = FP8 ? (MR == 32 ? g16 & 1 : 0) : (MR == 32 ? 2 * (g16 & 1) : 0) + ((i16 >> 1) & 1);
+      v = t * 128 + ((c ^ swizzle(t)) << 4) + 8 * (i16 & 1);
     }
     // 16 bytes of a token's latent (rotary) row, as step i reads them; token MR * sub + ln
     PCAMD_DEV uint4 key(const uint8_t* lds, uint32_t tile, int sub, int i) const {
-      constexpr int P = 16 / LANES_K;
-      return *reinterpret_cast<const uint4*>(lds + ((tile + k) ^ (i % P * LANES_K << 4)) + sub * MR * LROW + i / P * 256);
+      constexpr int P = 8 / LANES_K;
+      // 16 rows on, f is the same (16-bit rows) or differs in bit 1
+      const int x = (i % P * LANES_K ^ (FP8 && sub ? 2 : 0)) << 4;
+      return *reinterpret_cast<const uint4*>(lds + ((tile + k) ^ x) + i / P * BLOCK + sub * MR * 128);
     }
     PCAMD_DEV uint4 rope(const uint8_t* lds, uint32_t tile, int sub, int i) const {
-      return *reinterpret_cast<const uint4*>(lds + ((tile + kr) ^ (i * LANES_K << 4)) + sub * MR * RROW);
+      const int x = (i * LANES_K ^ (FP8 && sub ? 2 : 0)) << 4;
+      return *reinterpret_cast<const uint4*>(lds + ((tile + k) ^ x) + ROPE + sub * MR * 128);
     }
     // value columns j * MR .. of contraction step kk: raw codes, or the operand itself
     PCAMD_DEV uint4 value(const uint8_t* lds, uint32_t tile, int j, int kk) const {
       if constexpr (FP8) {
-        constexpr int P = MR == 32 ? 8 : 16, C = MR / 16;
-        const uint2 x = read_tr8(lds + ((tile + v) ^ (j % P * C << 4)) + kk * 16 * LROW + j / P * 256);
-        return make_uint4(x.x, x.y, 0, 0);
+        const int c = j * (MR / 16), x = (c % 8 ^ (kk ? 2 : 0)) << 4;
+        const uint2 y = read_tr8(lds + ((tile + v) ^ x) + c / 8 * BLOCK + kk * 16 * 128);
+        return make_uint4(y.x, y.y, 0, 0);
       } else {
-        constexpr int P = MR == 32 ? 4 : 8, C = MR / 8;
-        const uint32_t c = j % P * C;
-        // the second four tokens are QSTEP rows on, whose f differs in bit 1 (MR 32) or not at all
-        const uint2 x = read_tr4(lds + ((tile + v) ^ (c << 4)) + kk * 16 * LROW + j / P * 256);
-        const uint2 y = read_tr4(lds + ((tile + v) ^ ((MR == 32 ? c ^ 2 : c) << 4)) + (kk * 16 + M::QSTEP) * LROW + j / P * 256);
-        return make_uint4(x.x, x.y, y.x, y.y);
+        const int c = j * (MR / 8), x = c % 8 << 4, at = c / 8 * BLOCK + kk * 16 * 128;
+        // the second four tokens are QSTEP rows on: 8 rows change bit 0 of f, 16 do not
+        const uint2 y = read_tr4(lds + ((tile + v) ^ x) + at);
+        const uint2 z = read_tr4(lds + ((tile + v) ^ (MR == 32 ? x ^ 16 : x)) + at + M::QSTEP * 128);
+        return make_uint4(y.x, y.y, z.x, z.y);
       }
     }
   };
 
-  static PCAMD_DEV void segment(const Args& a, uint8_t* lds, int64_t b, int rt, int s0, int n, int steps, int len,
-                                int64_t slot, int wr, int wt, int h, int ln) {
+  static PCAMD_DEV void run(const Args& a, uint8_t* lds) {
+    int* wave_total = reinterpret_cast<int*>(lds + BODY + PAGES * 4);
+    int* found = wave_total + NT / 64;
+    const int tid = threadIdx.x;
+    constexpr int FIXED = kFixed<MR>;
+
+    // ---- this workgroup's piece of the list
+    int sum = 0, steps_all;
+    for (int b = tid; b < a.batch; b += NT) sum += steps_of(length_of(a, b), STEP);
+    int before = block_scan(sum, wave_total, steps_all);
+    const int tiles = a.batch * a.row_tiles;
+    const int wanted = (steps_all * a.row_tiles + a.min_steps - 1) / a.min_steps;
+    int groups = wanted > tiles ? wanted : tiles;
+    if (groups > a.groups) groups = a.groups;
+    const Division div(a.row_tiles * (steps_all + a.batch * FIXED), groups);
+    const int w = blockIdx.x;
+    if (w >= groups) {
+      if (a.parts && tid == 0) a.joins[w] = make_int4(0, 0, -1, 0);
+      return;
+    }
+    const int begin = div.first(w), end = div.first(w + 1);
+    int base = 0;
+    for (int b0 = 0; b0 < a.batch; b0 += NT) {
+      const int b = b0 + tid;
+      const int mine = b < a.batch ? (steps_of(length_of(a, b), STEP) + FIXED) * a.row_tiles : 0;
+      int total;
+      if (a.batch <= NT) before = (before + tid * FIXED) * a.row_tiles;  // the first scan's answer, where it had one sequence a thread
+      else before = base + block_scan(mine, wave_total, total);
+      if (mine && begin >= before && begin < before + mine) {
+        found[0] = b;
+        found[1] = begin - before;
+        found[2] = 1;
+      }
+      if (a.batch > NT) {
+        base += total;
+        if (base > begin) break;
+      }
+    }
+    __syncthreads();
+    int b = found[0], in_seq = found[1];
+    if (a.parts && tid == 0) {
+      // Where pieces meet: the first workgroup that starts inside a (sequence,
+      // row tile) notes which it is and which workgroup holds the last piece;
+      // the one before it holds the first.
+      const int tile = steps_of(length_of(a, b), STEP) + FIXED;
+      const int in_tile = in_seq % tile, real = begin - in_tile + FIXED;  // its first step's unit
+      a.joins[w] = begin > real && div.first(w - 1) <= real
+                       ? make_int4(b, in_seq / tile, 1, div.group_of(real + tile - FIXED - 1))
+                       : make_int4(0, 0, -1, 0);
+    }
+
+    for (int u = begin; u < end;) {
+      const int len = length_of(a, b);
+      const int steps = steps_of(len, STEP), tile = steps + FIXED;
+      const int rt = in_seq / tile, at = in_seq - rt * tile;
+      const int n = end - u < tile - at ? end - u : tile - at;
+      const int s0 = at > FIXED ? at - FIXED : 0, s1 = at + n - FIXED;
+      if (s1 > s0) segment(a, lds, b, rt, s0, s1 - s0, steps, len, s0 > 0 ? 2 * w : 2 * w + 1);
+      u += n;
+      in_seq += n;
+      if (in_seq >= tile * a.row_tiles) {
+        ++b;
+        in_seq = 0;
+      }
+    }
+  }
+
+  // Steps s0 .. s0 + n - 1 of a row tile's `steps`.
+  static PCAMD_DEV void segment(const Args& a, uint8_t* lds, int b, int rt, int s0, int n, int steps, int len,
+                                int slot) {
     const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64;
+    const int wr = wave % WR, wt = wave / WR;
+    const Lane L(lane);
+    const int h = L.h, ln = L.ln;
     const int row = rt * ROWS + wr * MR + ln;  // this lane's row
     const bool live = row < a.rows;
     const int tok_new = live ? row / a.heads : 0, head = live ? row % a.heads : 0;
-    // Queries, in registers for the whole segment, in the order in which the
-    // keys are read: 16 bytes of a key row a lane (with fp8 two steps' worth).
+
+    // ---- the page numbers, then the queries, then the first tiles: their
+    // latencies overlap. Queries stay in registers for the whole segment, in the
+    // order in which the keys are read: 16 bytes of a key row a lane (with fp8
+    // two products' worth).
+    const int32_t* table = a.table + static_cast<int64_t>(b) * a.table_stride;
+    int32_t* pages = reinterpret_cast<int32_t*>(lds + BODY);
+    Source src{pages, 0, 0};
+    int done = len > 0 ? 0 : n, upto = n;  // steps behind and, with the pages at hand, ahead of the loop
+    auto window = [&]() {                  // this thread's entry of the page numbers from step `done` on
+      src.first = a.page_index((s0 + done) * STEP);
+      // A step is at most 128 tokens and a window 256 pages, so it covers one at least.
+      const int64_t covered = (static_cast<int64_t>(src.first) + PAGES) * a.page;
+      src.last = (covered < len ? static_cast<int>(covered) : len) - 1;
+      upto = covered >= len ? n : static_cast<int>(covered / STEP) - s0;
+      if (upto > n) upto = n;
+      const int last = a.page_index(len - 1), at = src.first + tid;
+      return table[at < last ? at : last];
+    };
+    int entry = 0;
+    if (len > 0) entry = window();
     uint4 ql[KL], qr[KR];
     {
       const uint16_t* p = static_cast<const uint16_t*>(a.q_latent) + b * a.qlb + tok_new * a.qls + head * a.qlh;
@@ -324,57 +385,72 @@ struct Kernel {
 #pragma unroll
       for (int k = 0; k < KR; ++k)
         qr[k] = live ? *reinterpret_cast<const uint4*>(r + k * M::K + 8 * h) : make_uint4(0, 0, 0, 0);
-      // arrived before the loop: a wait inside it would wait for the copies too
-#pragma unroll
-      for (int k = 0; k < KL; ++k) asm volatile("" : "+v"(ql[k].x), "+v"(ql[k].y), "+v"(ql[k].z), "+v"(ql[k].w));
-#pragma unroll
-      for (int k = 0; k < KR; ++k) asm volatile("" : "+v"(qr[k].x), "+v"(qr[k].y), "+v"(qr[k].z), "+v"(qr[k].w));
     }
     const int limit = live ? len - a.new_tokens + 1 + tok_new : len;  // tokens this row sees
     const int all_see = len - a.new_tokens + 1;                       // tokens that every row sees
-    const Lane L(lane);
+    const uint32_t ring = wt * NB * TILE;  // the dynamic LDS starts at address 0 (see decode_kernel)
+    auto tile_of = [&](int i) { return ring + static_cast<uint32_t>(i % NB) * TILE; };
+    auto first_token = [&](int i) { return (s0 + done + i) * STEP + wt * TOK; };  // of this wave in step i of the window
+    auto start = [&]() {
+      pages[tid] = entry;
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) {
+        Copies c;
+        c.prepare(a, src, first_token(i), wr, lane);
+        c.emit_all(tile_of(i), wr, lane);
+      }
+    };
+    if (len > 0) start();
+    // here, ahead of the loop: a wait for a query inside it would wait for the copies too
+#pragma unroll
+    for (int k = 0; k < KL; ++k) asm volatile("" : "+v"(ql[k].x), "+v"(ql[k].y), "+v"(ql[k].z), "+v"(ql[k].w));
+#pragma unroll
+    for (int k = 0; k < KR; ++k) asm volatile("" : "+v"(qr[k].x), "+v"(qr[k].y), "+v"(qr[k].z), "+v"(qr[k].w));
+
     acc o[OB];
 #pragma unroll
     for (int i = 0; i < OB; ++i) o[i] = acc{};
     float m = kNoMax, l = 0.0f;
 
-    // ---- one tile of 32 tokens from tb on
-    // Reads of LDS run a few steps ahead of the products that take them
-    // (kAhead registers' worth), and sched_barrier keeps them there: left
-    // alone, the scheduler saves registers by waiting for every read.
-    auto compute = [&](uint32_t tile, int tb) {
+    // ---- The parts of a step. Reads of LDS run a few products ahead of those
+    // that take them, and sched_barrier keeps them there: left alone, the
+    // scheduler saves registers by waiting for every read. `beside(i)` is other
+    // work for the time of product i.
+    constexpr int PER_LOAD = FP8 ? 2 : 1;
+    constexpr int LOADS = KR + KL / PER_LOAD, PER = KR + KL;
+    constexpr int NA = SUB * PER, TA = SUB * LOADS;  // products of S^T, rotary ones first; their loads
+    constexpr int NP = OB * PK;                      // products of O^T: block n / PK, step n % PK
+    constexpr int DV = kAheadValues < NP ? kAheadValues : NP;
+    uint4 val[DV];
+    auto scores = [&](uint32_t tile, acc (&c)[SUB], auto beside) {
       const float* scales = reinterpret_cast<const float*>(lds + tile + SCALES) + 4 * h;
-
-      // ---- S^T: products n = 0 .. NA - 1, rotary steps first
-      constexpr int PER_LOAD = FP8 ? 2 : 1;
-      constexpr int LOADS = KR + KL / PER_LOAD, PER = KR + KL;
-      constexpr int NA = SUB * PER, TA = SUB * LOADS;
       constexpr int DA = kAheadKeys<FP8> < TA ? kAheadKeys<FP8> : TA;
       uint4 raw[DA];
       auto load_key = [&](int i) {
         const int sub = i / LOADS, r = i % LOADS;
         return r < KR ? L.rope(lds, tile, sub, r) : L.key(lds, tile, sub, r - KR);
       };
-      auto load_of = [](int n) { return n / PER * LOADS + (n % PER < KR ? n % PER : KR + (n % PER - KR) / PER_LOAD); };
-      auto operand = [&](int n) {
-        const uint4 x = raw[load_of(n) % DA];
+      auto load_of = [](int k) { return k / PER * LOADS + (k % PER < KR ? k % PER : KR + (k % PER - KR) / PER_LOAD); };
+      auto operand = [&](int k) {
+        const uint4 x = raw[load_of(k) % DA];
         if constexpr (FP8) {
-          if (n % PER >= KR) return (n % PER - KR) % 2 ? widen8(make_uint2(x.z, x.w)) : widen8(make_uint2(x.x, x.y));
+          if (k % PER >= KR) return (k % PER - KR) % 2 ? widen8(make_uint2(x.z, x.w)) : widen8(make_uint2(x.x, x.y));
         }
         return x;
       };
 #pragma unroll
       for (int i = 0; i < DA; ++i) raw[i] = load_key(i);
       __builtin_amdgcn_sched_barrier(0);
-      acc c[SUB], d[2];
+      acc d[2];
       uint4 next = operand(0);
 #pragma unroll
-      for (int n = 0; n < NA; ++n) {
-        const int sub = n / PER, r = n % PER;
+      for (int k = 0; k < NA; ++k) {
+        const int sub = k / PER, r = k % PER;
         const uint4 x = next;
-        if (n + 1 < NA) {
-          if (load_of(n + 1) != load_of(n) && load_of(n) + DA < TA) raw[load_of(n) % DA] = load_key(load_of(n) + DA);
-          next = operand(n + 1);
+        if (k + 1 < NA) {
+          if (load_of(k + 1) != load_of(k) && load_of(k) + DA < TA) raw[load_of(k) % DA] = load_key(load_of(k) + DA);
+          next = operand(k + 1);
         }
         if (r < KR) {
           c[sub] = r == 0 ? S::first(x, qr[0]) : S::mul(x, qr[r], c[sub]);
@@ -383,10 +459,10 @@ struct Kernel {
         } else {
           // a group's partial scores in d, scaled into c while the next group's are summed
           constexpr int G = KL / GROUPS;
-          const int k = r - KR, g = k / G;
-          if (k % G == 0) d[g & 1] = S::first(x, ql[k]);
-          else if (k % G == 1 && g > 0) d[g & 1] = S::mul_holding(x, ql[k], d[g & 1], d[(g - 1) & 1]);
-          else d[g & 1] = S::mul(x, ql[k], d[g & 1]);
+          const int i = r - KR, g = i / G;
+          if (i % G == 0) d[g & 1] = S::first(x, ql[i]);
+          else if (i % G == 1 && g > 0) d[g & 1] = S::mul_holding(x, ql[i], d[g & 1], d[(g - 1) & 1]);
+          else d[g & 1] = S::mul(x, ql[i], d[g & 1]);
           auto scale_in = [&](int group, int reg) {
             const int q = sub * (M::REGS / 4) + reg / 4;
             const float2 f = *reinterpret_cast<const float2*>(scales + group * TOK + q * M::QSTEP + reg % 4);
@@ -397,7 +473,7 @@ struct Kernel {
             // from the group's third product on the last of the group before has been written
 #pragma unroll
             for (int reg = 0; reg < M::REGS; reg += 2)
-              if (2 + reg / 2 * (G - 2) / (M::REGS / 2) == k % G) scale_in(g - 1, reg);
+              if (2 + reg / 2 * (G - 2) / (M::REGS / 2) == i % G) scale_in(g - 1, reg);
           }
           if (r == PER - 1) {
             S::settle(d[g & 1]);
@@ -405,34 +481,33 @@ struct Kernel {
             for (int reg = 0; reg < M::REGS; reg += 2) scale_in(g, reg);
           }
         }
+        beside(k);
         __builtin_amdgcn_sched_barrier(0);
       }
-
-      // ---- the first values are on their way during the softmax
-      constexpr int NP = OB * PK;  // products of the second kind: block n / PK, step n % PK
-      constexpr int DV = kAheadValues<FP8> < NP ? kAheadValues<FP8> : NP;
-      uint4 val[DV];
+    };
+    auto first_values = [&](uint32_t tile) {
 #pragma unroll
-      for (int n = 0; n < DV; ++n) val[n] = L.value(lds, tile, n / PK, n % PK);
+      for (int k = 0; k < DV; ++k) val[k] = L.value(lds, tile, k / PK, k % PK);
+    };
+    auto settle = [&](acc (&c)[SUB]) {
       if constexpr (!FP8) {
 #pragma unroll
         for (int sub = 0; sub < SUB; ++sub) S::settle(c[sub]);
       }
       __builtin_amdgcn_sched_barrier(0);
-
-      // ---- softmax, one row a lane
-      float s[QUADS * 4];
+    };
+    float s[QUADS * 4];
+    auto mask = [&](int tb) {
 #pragma unroll
-      for (int r = 0; r < QUADS * 4; ++r) s[r] = c[r / M::REGS][r % M::REGS] * a.scale_log2;
-      if (tb + TOK > all_see) {
-#pragma unroll
-        for (int r = 0; r < QUADS * 4; ++r)
-          s[r] = tb + (r / 4) * M::QSTEP + 4 * h + r % 4 < limit ? s[r] : -INFINITY;
-      }
+      for (int r = 0; r < QUADS * 4; ++r) s[r] = tb + (r / 4) * M::QSTEP + 4 * h + r % 4 < limit ? s[r] : -INFINITY;
+    };
+    auto maximum = [&]() {
       float top = s[0];
 #pragma unroll
       for (int r = 1; r < QUADS * 4; ++r) top = fmaxf(top, s[r]);
-      top = row_max<MR>(top);
+      return top;
+    };
+    auto refer = [&](float top) {  // top: of the row
       if (__any(top > m + kSlack<DT, FP8>)) {
         const float to = fmaxf(m, top), alpha = __builtin_amdgcn_exp2f(m - to);
         m = to;
@@ -445,98 +520,151 @@ struct Kernel {
           asm volatile("" : "+a"(o[j]));
         }
       }
-#pragma unroll
-      for (int r = 0; r < QUADS * 4; ++r) {
-        s[r] = __builtin_amdgcn_exp2f(s[r] - m);
-        l += s[r];
+    };
+    uint32_t p[FP8 ? 2 : 1][PK * 4];  // P^T of a group of value columns, and of the next
+    auto weights = [&](uint32_t tile, int g, int i) {  // dword i: registers 2 i and 2 i + 1
+      float x0 = s[2 * i], x1 = s[2 * i + 1];
+      if constexpr (FP8) {
+        const float* scales = reinterpret_cast<const float*>(lds + tile + SCALES) + 4 * h;
+        const float2 f = *reinterpret_cast<const float2*>(scales + g * TOK + (2 * i / 4) * M::QSTEP + 2 * i % 4);
+        x0 *= f.x * kScaleUp<DT>;
+        x1 *= f.y * kScaleUp<DT>;
       }
-
-      // ---- O^T += V^T P^T
-      uint32_t p[2][PK * 4];  // P^T of a group of value columns, and of the next
-      auto weights = [&](int g, int i) {  // dword i: registers 2 i and 2 i + 1
-        float x0 = s[2 * i], x1 = s[2 * i + 1];
-        if constexpr (FP8) {
-          const float2 f = *reinterpret_cast<const float2*>(scales + g * TOK + (2 * i / 4) * M::QSTEP + 2 * i % 4);
-          x0 *= f.x * kScaleUp<DT>;
-          x1 *= f.y * kScaleUp<DT>;
-        }
-        p[g & 1][i] = Elem<DT>::narrow2(x0, x1);
-      };
-#pragma unroll
-      for (int i = 0; i < PK * 4; ++i) weights(0, i);
-      auto value_operand = [&](int n) {
-        const uint4 x = val[n % DV];
+      p[FP8 ? g & 1 : 0][i] = Elem<DT>::narrow2(x0, x1);
+    };
+    auto values = [&](uint32_t tile, auto beside) {  // O^T += V^T P^T
+      auto operand = [&](int k) {
+        const uint4 x = val[k % DV];
         if constexpr (FP8) return widen8(make_uint2(x.x, x.y));
         else return x;
       };
-      next = value_operand(0);
-      __builtin_amdgcn_sched_barrier(0);
+      uint4 next = operand(0);
 #pragma unroll
-      for (int n = 0; n < NP; ++n) {
+      for (int k = 0; k < NP; ++k) {
         constexpr int PER_GROUP = NP / (FP8 ? GROUPS : 1);
-        const int j = n / PK, kk = n % PK, g = n / PER_GROUP;
+        const int j = k / PK, kk = k % PK, g = FP8 ? k / PER_GROUP : 0;
         const uint4 x = next;
-        if (n + DV < NP) val[n % DV] = L.value(lds, tile, (n + DV) / PK, (n + DV) % PK);
-        if (n + 1 < NP) next = value_operand(n + 1);
+        if (k + DV < NP) val[k % DV] = L.value(lds, tile, (k + DV) / PK, (k + DV) % PK);
+        if (k + 1 < NP) next = operand(k + 1);
         const uint32_t* w = p[g & 1] + 4 * kk;
         o[j] = M::mul(x, make_uint4(w[0], w[1], w[2], w[3]), o[j]);
         if constexpr (FP8) {
           if (g + 1 < GROUPS) {
 #pragma unroll
             for (int i = 0; i < PK * 4; ++i)
-              if (i * PER_GROUP / (PK * 4) == n % PER_GROUP) weights(g + 1, i);
+              if (i * PER_GROUP / (PK * 4) == k % PER_GROUP) weights(tile, g + 1, i);
           }
         }
+        beside(k);
         __builtin_amdgcn_sched_barrier(0);
       }
     };
+    auto nothing = [](int) {};
 
-    // ---- the loop over tiles, window by window of the page table
-    const int32_t* table = a.table + b * a.table_stride;
-    int32_t* pages = reinterpret_cast<int32_t*>(lds + BODY);
-    const uint32_t ring = wt * NB * TILE;  // the dynamic LDS starts at address 0 (see decode_kernel)
-    int done = len > 0 ? 0 : n;
+    // ---- the loop over steps, window by window of the page table
     while (done < n) {
-      const int first_t = (s0 + done) * STEP;
-      Source src{pages, a.page_index(first_t), len};
-      // steps whose tokens all lie within the window's pages (one at least:
-      // a step is at most 128 tokens, the window 256 pages)
-      const int64_t covered = (static_cast<int64_t>(src.first) + PAGES) * a.page;
-      int upto = covered >= len ? n : static_cast<int>(covered / STEP) - s0;
-      if (upto > n) upto = n;
-      __syncthreads();
-      {
-        const int last = a.page_index(len - 1), at = src.first + tid;
-        pages[tid] = table[at < last ? at : last];
+      if (done > 0) {
+        __syncthreads();
+        entry = window();
+        start();
       }
-      __syncthreads();
       const int count = upto - done;
-      auto start = [&](int i) {  // i: step of this window
-        issue(a, src, ring + i % NB * TILE, (s0 + done + i) * STEP + wt * TOK, wr, lane);
-      };
-      auto wait = [&](int later) {  // copies of `later` further steps may be in flight
-        if (NB > 2 && later >= 2) wait_copies<2 * COPIES <= 63 ? 2 * COPIES : 63>();
-        else if (later == 1) wait_copies<COPIES>();
-        else wait_copies<0>();
-      };
-      constexpr int AHEAD = WR > 1 ? NB - 1 : NB;
-      static_assert(AHEAD <= 3 || WR == 1, "wait() counts up to two further steps");
-      for (int i = 0; i < AHEAD && i < count; ++i) start(i);
-      for (int i = 0; i < count; ++i) {
-        const int later = count - 1 - i < AHEAD - 1 ? count - 1 - i : AHEAD - 1;
-        wait(later);
-        if constexpr (WR > 1) {
-          // the tile is there for all waves, and all have left the one before it
-          asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-          if (i + AHEAD < count) start(i + AHEAD);
-        }
-        const int tb = (s0 + done + i) * STEP + wt * TOK;
-        if (WT == 1 || tb < len) compute(ring + i % NB * TILE, tb);
-        if constexpr (WR == 1) {
-          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-          if (i + AHEAD < count) start(i + AHEAD);
+      // the tile has arrived for all waves of its group, and all have left the one before it
+      auto barrier = [] { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
+      if constexpr (PIPE) {
+        acc c[1];
+        auto to_scores = [&](int k) { s[k] = c[0][k] * a.scale_log2; };
+        auto look = [&](int i, float top) {  // before step i's weights: its mask and reference point
+          const int tb = first_token(i);
+          if (tb + TOK > all_see) {
+            mask(tb);
+            top = maximum();
+          }
+          refer(row_max<MR>(top));
+        };
+        wait_copies<(AHEAD - 1) * COPIES>();
+        barrier();
+        scores(tile_of(0), c, nothing);
+        settle(c);
+#pragma unroll
+        for (int k = 0; k < 16; ++k) to_scores(k);
+        look(0, maximum());
+        auto step = [&](int i, auto more) {
+          constexpr bool MORE = decltype(more)::value;  // another step follows
+          auto weigh = [&](int k) {                     // element k of step i's weights
+            s[k] = __builtin_amdgcn_exp2f(s[k] - m);
+            l += s[k];
+            if (k & 1) weights(0, 0, k / 2);
+          };
+          if constexpr (MORE) {
+            wait_copies<(AHEAD - 2) * COPIES>();
+            barrier();
+            Copies copies;
+            scores(tile_of(i + 1), c, [&](int k) {
+              if (k == 1) copies.prepare(a, src, first_token(i + AHEAD), wr, lane);
+              copies.emit_at(k, NA, tile_of(i + AHEAD), wr, lane);
+              if (k % (NA / 16) == 0 && k / (NA / 16) < 16) weigh(k / (NA / 16));
+              if (k == NA - 3) first_values(tile_of(i));
+            });
+            settle(c);
+            float top[2] = {kNoMax, kNoMax};
+            values(tile_of(i), [&](int k) {
+              if (k % (NP / 16) == 0) {
+                const int e = k / (NP / 16);
+                to_scores(e);
+                top[e & 1] = fmaxf(top[e & 1], s[e]);
+              }
+            });
+            look(i + 1, fmaxf(top[0], top[1]));
+          } else {
+            first_values(tile_of(i));
+#pragma unroll
+            for (int k = 0; k < 16; ++k) weigh(k);
+            values(tile_of(i), nothing);
+          }
+        };
+        for (int i = 0; i + 1 < count; ++i) step(i, std::true_type{});
+        step(count - 1, std::false_type{});
+      } else {
+        for (int i = 0; i < count; ++i) {
+          wait_copies<(AHEAD - 1) * COPIES>();
+          if constexpr (WR > 1) barrier();
+          const uint32_t tile = tile_of(i);
+          const int tb = first_token(i);
+          Copies copies;
+          acc c[SUB];
+          auto ahead = [&](int k) {
+            if constexpr (WR > 1) {
+              if (k == 1) copies.prepare(a, src, first_token(i + AHEAD), wr, lane);
+              copies.emit_at(k, NA, tile_of(i + AHEAD), wr, lane);
+            }
+          };
+          scores(tile, c, ahead);
+          first_values(tile);
+          settle(c);
+#pragma unroll
+          for (int r = 0; r < QUADS * 4; ++r) s[r] = c[r / M::REGS][r % M::REGS] * a.scale_log2;
+          if (tb + TOK > all_see) mask(tb);
+          refer(row_max<MR>(maximum()));
+#pragma unroll
+          for (int r = 0; r < QUADS * 4; ++r) {
+            s[r] = __builtin_amdgcn_exp2f(s[r] - m);
+            l += s[r];
+          }
+#pragma unroll
+          for (int k = 0; k < PK * 4; ++k) weights(tile, 0, k);
+          values(tile, [&](int k) {
+            if constexpr (WR == 1) {
+              if (k == 2) copies.prepare(a, src, first_token(i + AHEAD), wr, lane);
+            }
+          });
+          if constexpr (WR == 1) {
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            copies.emit_all(tile_of(i + AHEAD), wr, lane);
+          }
         }
       }
+      wait_copies<0>();  // the copies past the last step: LDS has other uses next
       done = upto;
     }
     l = row_sum<MR>(l);
@@ -544,53 +672,66 @@ struct Kernel {
     // ---- epilogue: the waves' rows meet in LDS and leave as whole rows
     const bool whole = n == steps;
     float* ep = reinterpret_cast<float*>(lds);
-    float2* ml = reinterpret_cast<float2*>(lds + 4 * MR * PITCH * 4);
-    constexpr float down = FP8 ? 1.0f / kScaleUp<DT> : 1.0f;
+    float2* ml = reinterpret_cast<float2*>(lds + 4 * MR * PITCH * 4);  // of each wave's rows; then factors and sums
+    int64_t* place = reinterpret_cast<int64_t*>(ml + 4 * MR);          // where a row of the tile goes; -1: nowhere
+    __syncthreads();
+    if (lane < MR) ml[wave * MR + ln] = make_float2(m, l);
+    __syncthreads();
+    float factor = 1.0f;  // of this lane's row
+    {
+      float big = kNoMax, total = 0.0f;
+#pragma unroll
+      for (int t = 0; t < WT; ++t) big = fmaxf(big, ml[(t * WR + wr) * MR + ln].x);
+#pragma unroll
+      for (int t = 0; t < WT; ++t) {
+        const float2 s = ml[(t * WR + wr) * MR + ln];
+        total += __builtin_amdgcn_exp2f(s.x - big) * s.y;
+      }
+      factor = __builtin_amdgcn_exp2f(m - big);
+      if (whole) factor *= total > 0.0f ? 1.0f / total : total == 0.0f ? 0.0f : NAN;
+      if constexpr (FP8) factor *= 1.0f / kScaleUp<DT>;
+      if (wt == 0 && lane < MR) {
+        const int64_t at = static_cast<int64_t>(slot) * ROWS + wr * MR + ln;
+        if (whole) {
+          place[wr * MR + ln] = live ? b * a.ob + tok_new * a.os + head * a.oh : -1;
+          if (live && a.lse)
+            a.lse[b * a.lb + tok_new * a.ls + head * a.lh] = total == 0.0f ? -INFINITY : (big + log2f(total)) * kLn2;
+        } else {
+          place[wr * MR + ln] = live ? at * DL : -1;
+          a.part_ml[at] = make_float2(big, total);
+        }
+      }
+    }
 #pragma unroll
     for (int d0 = 0; d0 < DL; d0 += DC) {
-      __syncthreads();
+      if (d0) __syncthreads();
 #pragma unroll
       for (int j = 0; j < DC / MR; ++j) {
 #pragma unroll
         for (int q = 0; q < M::REGS / 4; ++q) {
           const acc& x = o[d0 / MR + j];
           float* d = ep + (wave * MR + ln) * PITCH + j * MR + q * 8 + 4 * h;
-          *reinterpret_cast<float4*>(d) = make_float4(x[4 * q] * down, x[4 * q + 1] * down, x[4 * q + 2] * down,
-                                                      x[4 * q + 3] * down);
+          *reinterpret_cast<float4*>(d) = make_float4(x[4 * q] * factor, x[4 * q + 1] * factor, x[4 * q + 2] * factor,
+                                                      x[4 * q + 3] * factor);
         }
       }
-      if (lane < MR) ml[wave * MR + ln] = make_float2(m, l);
       __syncthreads();
+#pragma unroll 4
       for (int i = tid; i < ROWS * (DC / 4); i += NT) {
         const int r = i / (DC / 4), d = 4 * (i % (DC / 4));
-        const int rr = rt * ROWS + r;
-        if (rr >= a.rows) continue;
-        const int src = (r / MR) * MR + r % MR;  // wave wr = r / MR of the first token group
-        float big = kNoMax;
-#pragma unroll
-        for (int t = 0; t < WT; ++t) big = fmaxf(big, ml[t * WR * MR + src].x);
+        const int64_t to = place[r];
         float4 x = make_float4(0, 0, 0, 0);
-        float total = 0.0f;
 #pragma unroll
         for (int t = 0; t < WT; ++t) {
-          const float2 s = ml[t * WR * MR + src];
-          const float f = exp2f(s.x - big);
-          const float4 y = *reinterpret_cast<const float4*>(ep + (t * WR * MR + src) * PITCH + d);
-          x.x += f * y.x; x.y += f * y.y; x.z += f * y.z; x.w += f * y.w;
-          total += f * s.y;
+          const float4 y = *reinterpret_cast<const float4*>(ep + (t * ROWS + r) * PITCH + d);
+          x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
         }
-        if (whole) {
-          const int sn = rr / a.heads, hd = rr % a.heads;
-          const float inv = total > 0.0f ? 1.0f / total : total == 0.0f ? 0.0f : NAN;
-          const uint2 out = make_uint2(Elem<DT>::narrow2(x.x * inv, x.y * inv), Elem<DT>::narrow2(x.z * inv, x.w * inv));
-          *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + b * a.ob + sn * a.os + hd * a.oh + d0 + d) = out;
-          if (a.lse && d0 + d == 0)
-            a.lse[b * a.lb + sn * a.ls + hd * a.lh] = total == 0.0f ? -INFINITY : (big + log2f(total)) * kLn2;
-        } else {
-          const int64_t at = slot * ROWS + r;
-          *reinterpret_cast<float4*>(a.parts + at * DL + d0 + d) = x;
-          if (d0 + d == 0) a.part_ml[at] = make_float2(big, total);
-        }
+        if (to < 0) continue;
+        if (whole)
+          *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + to + d0 + d) =
+              make_uint2(Elem<DT>::narrow2(x.x, x.y), Elem<DT>::narrow2(x.z, x.w));
+        else
+          *reinterpret_cast<float4*>(a.parts + to + d0 + d) = x;
       }
     }
     __syncthreads();
@@ -604,63 +745,163 @@ __global__ __launch_bounds__(NT, 1) void decode_kernel(Args a) {
   Kernel<DT, FP8, DL, DR, MR, WR>::run(a, lds);
 }
 
-// Joins the pieces of a (sequence, row tile): one workgroup a row, its waves
-// take the pieces in turn, each lane DL / 64 columns.
+// Joins the pieces of the (sequence, row tile)s that more than one workgroup
+// worked on: o = sum_i 2^(m_i - m) o_i / sum_i 2^(m_i - m) l_i. Every workgroup
+// lists the joins from the main kernel's notes. Few pieces: a wave takes a row,
+// all pieces' loads at once. Many (a long context split over the whole device):
+// a workgroup takes a row's 128 columns, and eight groups of lanes share the
+// pieces.
+constexpr int kFewPieces = 8;
+constexpr int kJoinGroups = 1024;  // four workgroups a CU
+
+struct Joins {
+  int4 join[2][NT];  // few pieces, many: {sequence, row tile, 1, last workgroup}
+  int first[2][NT];  // workgroup of the second piece
+  int count[2][NT / 64];
+  float weight[NT + 1];
+  float red[NT / 64];
+  float4 sums[8][32];
+};
+
 template <int DT, int DL>
-__global__ __launch_bounds__(NT) void combine_kernel(Args a, int tile_rows, int step) {
-  constexpr int V = DL / 64;
-  __shared__ float sums[NT / 64][DL];
-  __shared__ float2 ml[NT / 64];
-  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-  const int64_t units = a.plan[0], groups = a.plan[1];
-  for (int64_t i = blockIdx.x; i < a.batch * a.rows; i += gridDim.x) {
-    const int64_t b = i / a.rows;
-    const int row = static_cast<int>(i % a.rows), rt = row / tile_rows, r = row % tile_rows;
-    const int steps = steps_of(length_of(a, b), step);
-    const int64_t u0 = a.plan[2 + b] + int64_t{rt} * steps, u1 = u0 + steps;
-    const int64_t w0 = group_of(u0, units, groups), w1 = group_of(u1 - 1, units, groups);
-    if (w0 == w1) continue;  // one workgroup had it all and wrote it
-    float m = kNoMax, l = 0.0f, x[V];
+__global__ __launch_bounds__(NT) void combine_kernel(Args a, int tile_rows) {
+  __shared__ Joins L;
+  const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64;
+
+  // ---- the lists, in the same order in every workgroup
+  const int4 mine = tid < a.groups ? a.joins[tid] : make_int4(0, 0, -1, 0);
+  const bool some = mine.z >= 0, many = mine.w - tid + 2 > kFewPieces;
+  const uint64_t masks[2] = {__ballot(some && !many), __ballot(some && many)};
+  if (lane < 2) L.count[lane][wave] = __popcll(masks[lane]);
+  __syncthreads();
+  int total[2] = {0, 0}, before[2] = {0, 0};
 #pragma unroll
-    for (int k = 0; k < V; ++k) x[k] = 0.0f;
-    for (int64_t w = w0 + wave; w <= w1; w += NT / 64) {
-      const int64_t slot = first_unit(w, units, groups) >= u0 ? 2 * w : 2 * w + 1;
-      const int64_t at = slot * tile_rows + r;
-      const float2 s = a.part_ml[at];
-      const float* p = a.parts + at * DL + lane * 4;
-      float y[V];
-#pragma unroll
-      for (int k = 0; k < V; k += 4) *reinterpret_cast<float4*>(y + k) = *reinterpret_cast<const float4*>(p + k * 64);
-      const float top = fmaxf(m, s.x), f = exp2f(m - top), g = exp2f(s.x - top);
-      m = top;
-      l = l * f + s.y * g;
-#pragma unroll
-      for (int k = 0; k < V; ++k) x[k] = x[k] * f + y[k] * g;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < V; k += 4) *reinterpret_cast<float4*>(&sums[wave][k * 64 + lane * 4]) = *reinterpret_cast<float4*>(x + k);
-    if (lane == 0) ml[wave] = make_float2(m, l);
-    __syncthreads();
-    float big = kNoMax, total = 0.0f;
-#pragma unroll
-    for (int w = 0; w < NT / 64; ++w) big = fmaxf(big, ml[w].x);
-    float f[NT / 64];
+  for (int k = 0; k < 2; ++k)
 #pragma unroll
     for (int w = 0; w < NT / 64; ++w) {
-      f[w] = exp2f(ml[w].x - big);
-      total += f[w] * ml[w].y;
+      before[k] += w < wave ? L.count[k][w] : 0;
+      total[k] += L.count[k][w];
     }
-    const float inv = total > 0.0f ? 1.0f / total : total == 0.0f ? 0.0f : NAN;
-    const int sn = row / a.heads, hd = row % a.heads;
-    for (int d = threadIdx.x; d < DL; d += NT) {
-      float v = 0.0f;
+  if (some) {
+    const int k = many, at = before[k] + __popcll(masks[k] & ((uint64_t{1} << lane) - 1));
+    L.join[k][at] = mine;
+    L.first[k][at] = tid;
+  }
+  __syncthreads();
+
+  auto address = [&](const int4& j, int r, int64_t& out, int64_t& lse) {  // false: no such row
+    const int row = j.y * tile_rows + r, sn = row / a.heads, hd = row % a.heads;
+    out = j.x * a.ob + sn * a.os + hd * a.oh;
+    lse = j.x * a.lb + sn * a.ls + hd * a.lh;
+    return row < a.rows;
+  };
+  // piece i: the first one was cut at its end, the others at their start
+  auto slot_of = [](int first, int i) { return int64_t{i == 0 ? 2 * (first - 1) + 1 : 2 * (first + i - 1)}; };
+  auto finish = [&](int64_t lse, float m, float l) {
+    if (a.lse) a.lse[lse] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
+  };
+  auto inverse = [](float l) { return l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : NAN; };
+
+  // ---- few pieces: a wave a row
+  for (int i = blockIdx.x * (NT / 64) + wave; i < total[0] * tile_rows; i += gridDim.x * (NT / 64)) {
+    const int4 j = L.join[0][i / tile_rows];
+    const int first = L.first[0][i / tile_rows], r = i % tile_rows, n = j.w - first + 2;
+    int64_t out, lse;
+    if (!address(j, r, out, lse)) continue;
+    constexpr int V = DL / 256;
+    float4 x[kFewPieces][V];
+    float2 s[kFewPieces];
 #pragma unroll
-      for (int w = 0; w < NT / 64; ++w) v += f[w] * sums[w][d];
-      store_elem<DT>(a.out, b * a.ob + sn * a.os + hd * a.oh + d, v * inv);
+    for (int p = 0; p < kFewPieces; ++p) {
+      const int64_t at = slot_of(first, p < n ? p : 0) * tile_rows + r;
+      s[p] = a.part_ml[at];
+      if (p >= n) s[p] = make_float2(kNoMax, 0.0f);
+      if (p < n) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) x[p][v] = *reinterpret_cast<const float4*>(a.parts + at * DL + v * 256 + lane * 4);
+      }
     }
-    if (a.lse && threadIdx.x == 0)
-      a.lse[b * a.lb + sn * a.ls + hd * a.lh] = total == 0.0f ? -INFINITY : (big + log2f(total)) * kLn2;
+    float m = kNoMax, l = 0.0f;
+#pragma unroll
+    for (int p = 0; p < kFewPieces; ++p) m = fmaxf(m, s[p].x);
+    float4 o[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) o[v] = make_float4(0, 0, 0, 0);
+#pragma unroll
+    for (int p = 0; p < kFewPieces; ++p) {
+      if (p >= n) break;
+      const float f = __builtin_amdgcn_exp2f(s[p].x - m);
+      l += f * s[p].y;
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        o[v].x += f * x[p][v].x; o[v].y += f * x[p][v].y; o[v].z += f * x[p][v].z; o[v].w += f * x[p][v].w;
+      }
+    }
+    const float inv = inverse(l);
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + out + v * 256 + lane * 4) =
+          make_uint2(Elem<DT>::narrow2(o[v].x * inv, o[v].y * inv), Elem<DT>::narrow2(o[v].z * inv, o[v].w * inv));
+    if (lane == 0) finish(lse, m, l);
+  }
+
+  // ---- many: a workgroup for 128 columns of a row
+  constexpr int SLICES = DL / 128;
+  for (int i = blockIdx.x; i < total[1] * tile_rows * SLICES; i += gridDim.x) {
+    const int t = i / (tile_rows * SLICES), r = i / SLICES % tile_rows, slice = i % SLICES;
+    const int4 j = L.join[1][t];
+    const int first = L.first[1][t], n = j.w - first + 2;  // up to one more than there are threads
+    int64_t out, lse;
+    if (!address(j, r, out, lse)) continue;
+    float2 s[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int p = tid + k * NT;
+      s[k] = p < n ? a.part_ml[slot_of(first, p) * tile_rows + r] : make_float2(kNoMax, 0.0f);
+    }
+    float m = fmaxf(s[0].x, s[1].x);
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
+    if (lane == 0) L.red[wave] = m;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < NT / 64; ++w) m = fmaxf(m, L.red[w]);
+    float l = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const float f = __builtin_amdgcn_exp2f(s[k].x - m);
+      l += f * s[k].y;
+      if (tid + k * NT < n) L.weight[tid + k * NT] = f;
+    }
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) l += __shfl_xor(l, d, 64);
+    __syncthreads();
+    if (lane == 0) L.red[wave] = l;
+    __syncthreads();
+    l = 0.0f;
+#pragma unroll
+    for (int w = 0; w < NT / 64; ++w) l += L.red[w];
+    const int col = slice * 128 + tid % 32 * 4;
+    float4 o = make_float4(0, 0, 0, 0);
+#pragma unroll 4
+    for (int p = tid / 32; p < n; p += 8) {
+      const float f = L.weight[p];
+      const float4 x = *reinterpret_cast<const float4*>(a.parts + (slot_of(first, p) * tile_rows + r) * DL + col);
+      o.x += f * x.x; o.y += f * x.y; o.z += f * x.z; o.w += f * x.w;
+    }
+    L.sums[tid / 32][tid % 32] = o;
+    __syncthreads();
+    if (tid < 32) {
+#pragma unroll
+      for (int p = 1; p < 8; ++p) {
+        const float4 x = L.sums[p][tid];
+        o.x += x.x; o.y += x.y; o.z += x.z; o.w += x.w;
+      }
+      const float inv = inverse(l);
+      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + out + col) =
+          make_uint2(Elem<DT>::narrow2(o.x * inv, o.y * inv), Elem<DT>::narrow2(o.z * inv, o.w * inv));
+      if (tid == 0 && slice == 0) finish(lse, m, l);
+    }
     __syncthreads();
   }
 }

@@ -17,27 +17,27 @@ extern template int launch<kF16, 256, 32>(const Args&, Shape, bool, hipStream_t)
 
 constexpr int64_t kGroups = 256;  // one workgroup (four waves, most of the LDS) a CU
 
-struct Division {
+struct Layout {
   Shape shape;
-  int64_t row_tiles, groups, min_units;
+  int64_t row_tiles, groups, min_steps;
   bool split;  // pieces may have to be joined
-  int64_t plan_bytes, ml_bytes, part_bytes;
-  int64_t bytes() const { return split ? plan_bytes + ml_bytes + part_bytes : 0; }
+  int64_t join_bytes, ml_bytes, part_bytes;
+  int64_t bytes() const { return split ? join_bytes + ml_bytes + part_bytes : 0; }
 };
 
 // From sizes that the host knows: the table's capacity bounds the lengths.
-Division divide(int64_t batch, int64_t rows, int64_t latent_dim, int64_t capacity) {
-  Division d;
+Layout lay_out(int64_t batch, int64_t rows, int64_t latent_dim, int64_t capacity) {
+  Layout d;
   d.shape = shape_for(rows);
   const int64_t tile = d.shape.tile_rows(), step = d.shape.step();
   d.row_tiles = (rows + tile - 1) / tile;
   const int64_t steps = capacity > step ? (capacity + step - 1) / step : 1;
-  d.min_units = 128 / step;
-  const int64_t units = batch * d.row_tiles * steps;
-  d.groups = (units + d.min_units - 1) / d.min_units;
+  d.min_steps = 128 / step;
+  const int64_t tiles = batch * d.row_tiles, wanted = (tiles * steps + d.min_steps - 1) / d.min_steps;
+  d.groups = wanted > tiles ? wanted : tiles;
   if (d.groups > kGroups) d.groups = kGroups;
   d.split = steps > 1 && d.groups > 1;
-  d.plan_bytes = ((2 + batch) * 8 + 255) / 256 * 256;
+  d.join_bytes = (d.groups * 16 + 255) / 256 * 256;
   d.ml_bytes = 2 * d.groups * tile * 8;
   d.part_bytes = 2 * d.groups * tile * latent_dim * 4;
   return d;
@@ -53,7 +53,8 @@ int check_sizes(int64_t batch, int64_t new_tokens, int64_t heads, int64_t latent
   if (latent_dim != 512 && latent_dim != 256)
     return set_error(PCAMD_ERR_UNSUPPORTED, "latent width must be 512 or 256, got %lld", (long long)latent_dim);
   if (batch > (1 << 20) || new_tokens > (1 << 20) || heads > (1 << 20) || new_tokens * heads > (1 << 24) ||
-      max_pages > INT32_MAX / page_size)
+      max_pages > INT32_MAX / page_size ||
+      batch * ((new_tokens * heads + 15) / 16) * ((page_size * max_pages) / 32 + 32) > INT32_MAX)
     return set_error(PCAMD_ERR_UNSUPPORTED, "latent decode: too many rows or tokens a sequence");
   return PCAMD_OK;
 }
@@ -68,7 +69,7 @@ extern "C" int64_t pcamd_latent_decode_workspace(int64_t batch, int64_t new_toke
   const int rc = decode::check_sizes(batch, new_tokens, heads, latent_dim, page_size, max_pages);
   if (rc != PCAMD_OK) return rc;
   if (batch == 0 || new_tokens * heads == 0) return 0;
-  return decode::divide(batch, new_tokens * heads, latent_dim, page_size * max_pages).bytes();
+  return decode::lay_out(batch, new_tokens * heads, latent_dim, page_size * max_pages).bytes();
 }
 
 extern "C" int pcamd_latent_decode(
@@ -100,34 +101,40 @@ extern "C" int pcamd_latent_decode(
       !decode::aligned16(cache_rope) || (reinterpret_cast<uintptr_t>(out) & 7) || qlb % 8 || qls % 8 || qlh % 8 ||
       qrb % 8 || qrs % 8 || qrh % 8 || clp % per16 || clt % per16 || crp % 8 || crt % 8 || ob % 4 || os % 4 || oh % 4)
     return set_error(PCAMD_ERR_INVALID, "rows of queries and cache must be 16-byte aligned, of the output 8-byte");
+  for (const int64_t stride : {clp, clt, crp, crt, csp, cst})
+    if (stride < 0 || stride > INT32_MAX) return set_error(PCAMD_ERR_UNSUPPORTED, "latent decode: a cache stride past 2^31 elements");
+  if (pages > UINT32_MAX) return set_error(PCAMD_ERR_UNSUPPORTED, "latent decode: more than 2^32 - 1 pages");
   decode::Args a{};
   a.q_latent = q_latent; a.q_rope = q_rope;
   a.qlb = qlb; a.qls = qls; a.qlh = qlh; a.qrb = qrb; a.qrs = qrs; a.qrh = qrh;
   a.latent = cache_latent; a.rope = cache_rope; a.scale = cache_scale;
-  a.slp = clp; a.slt = clt; a.srp = crp; a.srt = crt; a.ssp = csp; a.sst = cst;
+  a.slp = static_cast<uint32_t>(clp); a.slt = static_cast<uint32_t>(clt);
+  a.srp = static_cast<uint32_t>(crp); a.srt = static_cast<uint32_t>(crt);
+  a.ssp = static_cast<uint32_t>(csp); a.sst = static_cast<uint32_t>(cst);
   a.table = table; a.table_stride = table_stride; a.lens = lens;
   a.out = out; a.ob = ob; a.os = os; a.oh = oh;
   a.lse = lse; a.lb = lb; a.ls = ls; a.lh = lh;
-  a.batch = batch; a.pages = pages;
+  a.batch = static_cast<int>(batch); a.pages = static_cast<uint32_t>(pages);
   a.new_tokens = static_cast<int>(new_tokens);
   a.heads = static_cast<int>(heads);
   a.rows = static_cast<int>(new_tokens * heads);
   a.page = static_cast<int>(page_size);
-  a.page_shift = (page_size & (page_size - 1)) == 0 ? __builtin_ctzll(page_size) : -1;
+  while ((int64_t{1} << a.page_shift) < page_size) ++a.page_shift;
+  a.page_mul = static_cast<uint32_t>(((int64_t{1} << (31 + a.page_shift)) + page_size - 1) / page_size);
   a.capacity = pages ? static_cast<int>(page_size * max_pages) : 0;  // no pool: every sequence is empty
   a.scale_log2 = softmax_scale * 1.4426950408889634f;
-  const decode::Division d = decode::divide(batch, a.rows, latent_dim, page_size * max_pages);
+  const decode::Layout d = decode::lay_out(batch, a.rows, latent_dim, page_size * max_pages);
   a.row_tiles = static_cast<int>(d.row_tiles);
   a.groups = static_cast<int>(d.groups);
-  a.min_units = static_cast<int>(d.min_units);
+  a.min_steps = static_cast<int>(d.min_steps);
   if (d.split) {
     if (!workspace || workspace_bytes < d.bytes() || !decode::aligned16(workspace))
       return set_error(PCAMD_ERR_INVALID, "latent decode needs a 16-byte aligned workspace of %lld bytes, got %lld",
                        (long long)d.bytes(), (long long)workspace_bytes);
     uint8_t* w = static_cast<uint8_t*>(workspace);
-    a.plan = reinterpret_cast<int64_t*>(w);
-    a.part_ml = reinterpret_cast<float2*>(w + d.plan_bytes);
-    a.parts = reinterpret_cast<float*>(w + d.plan_bytes + d.ml_bytes);
+    a.joins = reinterpret_cast<int4*>(w);
+    a.part_ml = reinterpret_cast<float2*>(w + d.join_bytes);
+    a.parts = reinterpret_cast<float*>(w + d.join_bytes + d.ml_bytes);
   }
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (dtype == kBF16)

@@ -12,20 +12,29 @@ struct Args {
   const void* q_latent; const void* q_rope;
   int64_t qlb, qls, qlh, qrb, qrs, qrh;
   const void* latent; const void* rope; const float* scale;
-  int64_t slp, slt, srp, srt, ssp, sst;
+  uint32_t slp, slt, srp, srt, ssp, sst;
   const int32_t* table; int64_t table_stride; const int32_t* lens;
   void* out; int64_t ob, os, oh;
   float* lse; int64_t lb, ls, lh;
-  int64_t batch, pages;
-  int new_tokens, heads, rows, row_tiles, page, page_shift, capacity;
+  uint32_t pages, page_mul;
+  int batch, new_tokens, heads, rows, row_tiles, page, page_shift, capacity;
   float scale_log2;
   // the division of the work, and where its pieces meet
-  int groups, min_units;
-  int64_t* plan; float* parts; float2* part_ml;
+  int groups, min_steps;
+  int4* joins; float* parts; float2* part_ml;
 
-  // place in the page table of the page that holds token t
-  __device__ __forceinline__ int page_index(int t) const { return page_shift >= 0 ? t >> page_shift : t / page; }
+  // place in the page table of the page that holds token t, t / page: with l =
+  // ceil(log2 page) = page_shift and page_mul = ceil(2^(31 + l) / page), exact
+  // for every t below 2^31
+  __device__ __forceinline__ int page_index(int t) const {
+    return static_cast<int>(__umulhi(2u * static_cast<uint32_t>(t), page_mul) >> page_shift);
+  }
 };
+
+// What a piece costs whatever its length (queries in, output out, latencies),
+// in steps of its kernel
+template <int MR>
+constexpr int kFixed = MR == 32 ? 10 : 2;
 
 // Rows of a tile and tokens of a step for `rows` rows a sequence: up to 16 (32,
 // 64) rows fill one (two, four) waves of 16 rows, and the other waves of a

@@ -28,9 +28,10 @@ int launch(const Args& a, Shape shape, bool fp8, hipStream_t st) {
   else if (shape.wr == 2) rc = fp8 ? launch_shape<DT, true, DL, DR, 16, 2>(a, st) : launch_shape<DT, false, DL, DR, 16, 2>(a, st);
   else rc = fp8 ? launch_shape<DT, true, DL, DR, 16, 1>(a, st) : launch_shape<DT, false, DL, DR, 16, 1>(a, st);
   if (rc != PCAMD_OK || !a.parts) return rc;
-  const int64_t rows = a.batch * a.rows;
-  const uint32_t grid = static_cast<uint32_t>(rows < (1 << 20) ? rows : (1 << 20));
-  combine_kernel<DT, DL><<<grid, NT, 0, st>>>(a, shape.tile_rows(), shape.step());
+  // as many workgroups as the joins can keep busy: one at most a boundary between pieces
+  const int64_t tiles = a.batch * a.row_tiles, joins = tiles < a.groups - 1 ? tiles : a.groups - 1;
+  const int64_t most = joins * shape.tile_rows() * (DL / 128);
+  combine_kernel<DT, DL><<<static_cast<uint32_t>(most < kJoinGroups ? most : kJoinGroups), NT, 0, st>>>(a, shape.tile_rows());
   return check_launch("combine_kernel");
 }
 
