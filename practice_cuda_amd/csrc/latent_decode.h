@@ -114,11 +114,16 @@ struct Kernel {
   static_assert(!PIPE || NB == 4, "the overlapped loop holds two tiles while two more are on their way");
   static constexpr int PAGES = 256;  // page numbers kept in LDS
   static constexpr int RING = WT * NB * TILE;
-  // epilogue, in the ring's place: DC columns of every row at a time
-  static constexpr int DC = MR == 32 && DL > 256 ? 256 : DL;
-  static constexpr int PITCH = DC + 4;
-  static constexpr int EPI = 4 * MR * PITCH * 4 + 4 * MR * 8 + ROWS * 8;
-  static constexpr int BODY = RING > EPI ? RING : EPI;
+  // epilogue, in the ring's place: the rows of EW waves at a time. Whole rows,
+  // because half rows of all of them would keep half of the memory channels idle.
+  static constexpr int EW = MR == 32 && DL > 256 ? 2 : 4;
+  static constexpr int PITCH = DL + 4;
+  static constexpr int EPI = EW * MR * PITCH * 4 + 4 * MR * 8 + ROWS * 8;
+  // prologue, there too: each wave's query rows, [block][row][128 bytes]
+  static constexpr int QBLOCKS = DL / 64, QBLOCK = MR * 128;
+  static constexpr int QUERIES = (QBLOCKS + 1) * QBLOCK;
+  static constexpr int BODY0 = RING > EPI ? RING : EPI;
+  static constexpr int BODY = BODY0 > 4 * QUERIES ? BODY0 : 4 * QUERIES;
   static constexpr int LDS = BODY + PAGES * 4 + 64;  // and a few words of the division of the work
 
   // Chunk c of row t lies at c ^ f(t). Rows are 128 bytes apart, so t & 1 is a
@@ -128,10 +133,10 @@ struct Kernel {
   //   16-bit values: rows 4 h .. + 3 (MR 32: 64 bytes each; MR 16, two h: 32
   //   bytes each) - the reversed bits of t / 2;
   //   8-bit values: rows 4 h .. + 3 and QSTEP further on, 32 (16) bytes each.
+  static PCAMD_DEV int swizzle16(int t) { return ((t & 2) << 1) | ((t >> 1) & 2) | ((t >> 3) & 1); }
   static PCAMD_DEV int swizzle(int t) {
-    const int u = t >> 1;
-    if constexpr (FP8) return ((u & 1) << 2) | ((((u >> 2) ^ (u >> 3)) & 1) << 1) | ((u >> 1) & 1);
-    else return ((u & 1) << 2) | (u & 2) | ((u >> 2) & 1);
+    if constexpr (FP8) return ((t & 2) << 1) | (((t >> 2) ^ (t >> 3)) & 2) | ((t >> 2) & 1);
+    else return swizzle16(t);
   }
 
   // ---- global -> LDS copies: 8 rows x 128 bytes each. The WR waves of a token
@@ -173,6 +178,8 @@ struct Kernel {
     place = t - n * a.page;
   }
 
+  static PCAMD_DEV int rotation() { return __builtin_amdgcn_readfirstlane(threadIdx.x / 64) * (BLOCKS > 4 ? 2 : 1); }
+
   // the addresses of a tile's copies, and the copies
   struct Copies {
     const uint8_t* latent[RR];
@@ -198,12 +205,16 @@ struct Kernel {
         scale[i] = a.scale + uint64_t{page} * a.ssp + uint64_t{place} * a.sst + j / TOK;
       }
     }
-    // copy k of COPIES into the tile at LDS address `tile`
+    // Copy k of COPIES into the tile at LDS address `tile`. The latent rows'
+    // blocks come in an order that starts elsewhere in every wave: eight rows'
+    // equal 128 bytes lie in few memory channels, and waves that asked for the
+    // same block at the same time would leave the other channels idle.
     template <int K>
     PCAMD_DEV void emit(uint32_t tile, int wr, int lane) const {
       if constexpr (K < RR * BLOCKS) {
-        constexpr int i = K / BLOCKS, b = K % BLOCKS;
-        copy16<b * 128>(latent[i], tile + b * BLOCK + (wr * RW + 8 * i) * 128);
+        constexpr int i = K / BLOCKS;
+        const int b = (K + rotation()) % BLOCKS;
+        copy16<0>(latent[i] + b * 128, tile + b * BLOCK + (wr * RW + 8 * i) * 128);
       } else if constexpr (K < RR * (BLOCKS + 1)) {
         constexpr int i = K - RR * BLOCKS;
         if (CR == 8 || rope[i]) copy16<0>(rope[i], tile + ROPE + (wr * RW + 8 * i) * 128);
@@ -279,7 +290,6 @@ struct Kernel {
     int* wave_total = reinterpret_cast<int*>(lds + BODY + PAGES * 4);
     int* found = wave_total + NT / 64;
     const int tid = threadIdx.x;
-    constexpr int FIXED = kFixed<MR>;
 
     // ---- this workgroup's piece of the list
     int sum = 0, steps_all;
@@ -289,12 +299,16 @@ struct Kernel {
     const int wanted = (steps_all * a.row_tiles + a.min_steps - 1) / a.min_steps;
     int groups = wanted > tiles ? wanted : tiles;
     if (groups > a.groups) groups = a.groups;
+    // with few tiles every workgroup has one piece of one: nothing to weigh
+    const int FIXED = tiles * 16 >= groups ? kFixed<MR> : 0;
     const Division div(a.row_tiles * (steps_all + a.batch * FIXED), groups);
-    const int w = blockIdx.x;
-    if (w >= groups) {
-      if (a.parts && tid == 0) a.joins[w] = make_int4(0, 0, -1, 0);
+    if (static_cast<int>(blockIdx.x) >= groups) {
+      if (a.parts && tid == 0) a.joins[blockIdx.x] = make_int4(0, 0, -1, 0);
       return;
     }
+    // Neighbouring pieces belong to the same sequence: put them on the same XCD
+    // (workgroups go round the eight of them), whose L2 then holds its queries.
+    const int w = groups % 8 ? blockIdx.x : blockIdx.x % 8 * (groups / 8) + blockIdx.x / 8;
     const int begin = div.first(w), end = div.first(w + 1);
     int base = 0;
     for (int b0 = 0; b0 < a.batch; b0 += NT) {
@@ -353,10 +367,9 @@ struct Kernel {
     const bool live = row < a.rows;
     const int tok_new = live ? row / a.heads : 0, head = live ? row % a.heads : 0;
 
-    // ---- the page numbers, then the queries, then the first tiles: their
-    // latencies overlap. Queries stay in registers for the whole segment, in the
-    // order in which the keys are read: 16 bytes of a key row a lane (with fp8
-    // two products' worth).
+    // ---- the page numbers and the queries, then the first tiles. Queries stay
+    // in registers for the whole segment, in the order in which the keys are
+    // read: 16 bytes of a key row a lane (with fp8 two products' worth).
     const int32_t* table = a.table + static_cast<int64_t>(b) * a.table_stride;
     int32_t* pages = reinterpret_cast<int32_t*>(lds + BODY);
     Source src{pages, 0, 0};
@@ -373,19 +386,44 @@ struct Kernel {
     };
     int entry = 0;
     if (len > 0) entry = window();
+    // The queries pass through LDS: whole 128-byte lines come in, and a lane
+    // takes its row's pieces from there.
+    {
+      const uint32_t to = wave * QUERIES;
+#pragma unroll
+      for (int i = 0; i < MR / 8; ++i) {
+        const int r = 8 * i + lane / 8, c = (lane % 8) ^ swizzle16(r);
+        int from = rt * ROWS + wr * MR + r;
+        if (from >= a.rows) from = a.rows - 1;  // a spare row computes what another one does, and is not stored
+        const int tn = from / a.heads, hd = from - tn * a.heads;
+        const uint16_t* p = static_cast<const uint16_t*>(a.q_latent) + b * a.qlb + tn * a.qls + hd * a.qlh + 8 * c;
+#pragma unroll
+        for (int k = 0; k < QBLOCKS; ++k) {
+          const int blk = (k + rotation()) % QBLOCKS;  // as for the tiles
+          copy16<0>(p + blk * 64, to + blk * QBLOCK + 8 * i * 128);
+        }
+        if (c < CR)
+          copy16<0>(static_cast<const uint16_t*>(a.q_rope) + b * a.qrb + tn * a.qrs + hd * a.qrh + 8 * c,
+                    to + QBLOCKS * QBLOCK + 8 * i * 128);
+      }
+    }
+    wait_copies<0>();
     uint4 ql[KL], qr[KR];
     {
-      const uint16_t* p = static_cast<const uint16_t*>(a.q_latent) + b * a.qlb + tok_new * a.qls + head * a.qlh;
-      const uint16_t* r = static_cast<const uint16_t*>(a.q_rope) + b * a.qrb + tok_new * a.qrs + head * a.qrh;
+      const uint8_t* from = lds + wave * QUERIES + ln * 128;
+      auto piece = [&](int c) {  // c: a constant and h
+        return *reinterpret_cast<const uint4*>(from + c / 8 * QBLOCK + ((c % 8 ^ swizzle16(ln)) << 4));
+      };
 #pragma unroll
-      for (int k = 0; k < KL; ++k) {
-        const int at = FP8 ? (k / 2 * LANES_K + h) * 16 + k % 2 * 8 : (k * LANES_K + h) * 8;
-        ql[k] = live ? *reinterpret_cast<const uint4*>(p + at) : make_uint4(0, 0, 0, 0);
-      }
+      for (int k = 0; k < KL; ++k) ql[k] = piece(FP8 ? 2 * (k / 2 * LANES_K + h) + k % 2 : k * LANES_K + h);
 #pragma unroll
-      for (int k = 0; k < KR; ++k)
-        qr[k] = live ? *reinterpret_cast<const uint4*>(r + k * M::K + 8 * h) : make_uint4(0, 0, 0, 0);
+      for (int k = 0; k < KR; ++k) qr[k] = piece(QBLOCKS * 8 + k * LANES_K + h);
+#pragma unroll
+      for (int k = 0; k < KL; ++k) asm volatile("" : "+v"(ql[k].x), "+v"(ql[k].y), "+v"(ql[k].z), "+v"(ql[k].w));
+#pragma unroll
+      for (int k = 0; k < KR; ++k) asm volatile("" : "+v"(qr[k].x), "+v"(qr[k].y), "+v"(qr[k].z), "+v"(qr[k].w));
     }
+    __syncthreads();  // the tiles take the queries' place
     const int limit = live ? len - a.new_tokens + 1 + tok_new : len;  // tokens this row sees
     const int all_see = len - a.new_tokens + 1;                       // tokens that every row sees
     const uint32_t ring = wt * NB * TILE;  // the dynamic LDS starts at address 0 (see decode_kernel)
@@ -402,12 +440,6 @@ struct Kernel {
       }
     };
     if (len > 0) start();
-    // here, ahead of the loop: a wait for a query inside it would wait for the copies too
-#pragma unroll
-    for (int k = 0; k < KL; ++k) asm volatile("" : "+v"(ql[k].x), "+v"(ql[k].y), "+v"(ql[k].z), "+v"(ql[k].w));
-#pragma unroll
-    for (int k = 0; k < KR; ++k) asm volatile("" : "+v"(qr[k].x), "+v"(qr[k].y), "+v"(qr[k].z), "+v"(qr[k].w));
-
     acc o[OB];
 #pragma unroll
     for (int i = 0; i < OB; ++i) o[i] = acc{};
@@ -633,8 +665,13 @@ struct Kernel {
           const int tb = first_token(i);
           Copies copies;
           acc c[SUB];
+          // (the 128-row kernel of an fp8 cache has no registers for it beside the scores)
+          if constexpr (WR > 1 && MR == 32) {
+            copies.prepare(a, src, first_token(i + AHEAD), wr, lane);
+            copies.emit_all(tile_of(i + AHEAD), wr, lane);
+          }
           auto ahead = [&](int k) {
-            if constexpr (WR > 1) {
+            if constexpr (WR > 1 && MR == 16) {
               if (k == 1) copies.prepare(a, src, first_token(i + AHEAD), wr, lane);
               copies.emit_at(k, NA, tile_of(i + AHEAD), wr, lane);
             }
@@ -672,7 +709,7 @@ struct Kernel {
     // ---- epilogue: the waves' rows meet in LDS and leave as whole rows
     const bool whole = n == steps;
     float* ep = reinterpret_cast<float*>(lds);
-    float2* ml = reinterpret_cast<float2*>(lds + 4 * MR * PITCH * 4);  // of each wave's rows; then factors and sums
+    float2* ml = reinterpret_cast<float2*>(lds + EW * MR * PITCH * 4);  // of each wave's rows; then factors and sums
     int64_t* place = reinterpret_cast<int64_t*>(ml + 4 * MR);          // where a row of the tile goes; -1: nowhere
     __syncthreads();
     if (lane < MR) ml[wave * MR + ln] = make_float2(m, l);
@@ -703,23 +740,25 @@ struct Kernel {
       }
     }
 #pragma unroll
-    for (int d0 = 0; d0 < DL; d0 += DC) {
-      if (d0) __syncthreads();
+    for (int w0 = 0; w0 < 4; w0 += EW) {
+      if (w0) __syncthreads();
+      if (wave >= w0 && wave < w0 + EW) {
 #pragma unroll
-      for (int j = 0; j < DC / MR; ++j) {
+        for (int j = 0; j < OB; ++j) {
 #pragma unroll
-        for (int q = 0; q < M::REGS / 4; ++q) {
-          const acc& x = o[d0 / MR + j];
-          float* d = ep + (wave * MR + ln) * PITCH + j * MR + q * 8 + 4 * h;
-          *reinterpret_cast<float4*>(d) = make_float4(x[4 * q] * factor, x[4 * q + 1] * factor, x[4 * q + 2] * factor,
-                                                      x[4 * q + 3] * factor);
+          for (int q = 0; q < M::REGS / 4; ++q) {
+            float* d = ep + ((wave - w0) * MR + ln) * PITCH + j * MR + q * 8 + 4 * h;
+            *reinterpret_cast<float4*>(d) = make_float4(o[j][4 * q] * factor, o[j][4 * q + 1] * factor,
+                                                        o[j][4 * q + 2] * factor, o[j][4 * q + 3] * factor);
+          }
         }
       }
       __syncthreads();
+      constexpr int PASS = ROWS < EW * MR ? ROWS : EW * MR;  // rows of this pass
 #pragma unroll 4
-      for (int i = tid; i < ROWS * (DC / 4); i += NT) {
-        const int r = i / (DC / 4), d = 4 * (i % (DC / 4));
-        const int64_t to = place[r];
+      for (int i = tid; i < PASS * (DL / 4); i += NT) {
+        const int r = i / (DL / 4), d = 4 * (i % (DL / 4));
+        const int64_t to = place[w0 * MR + r];
         float4 x = make_float4(0, 0, 0, 0);
 #pragma unroll
         for (int t = 0; t < WT; ++t) {
@@ -728,10 +767,10 @@ struct Kernel {
         }
         if (to < 0) continue;
         if (whole)
-          *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + to + d0 + d) =
+          *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + to + d) =
               make_uint2(Elem<DT>::narrow2(x.x, x.y), Elem<DT>::narrow2(x.z, x.w));
         else
-          *reinterpret_cast<float4*>(a.parts + to + d0 + d) = x;
+          *reinterpret_cast<float4*>(a.parts + to + d) = x;
       }
     }
     __syncthreads();
