@@ -168,15 +168,21 @@ struct Kernel {
     const int32_t* pages;  // in LDS: the table from page number `first` on
     int first, last;       // last: the last token that they and the sequence hold
   };
-  // Page and place of a token, cut to the last one: what lies behind it is not
-  // read, and a row that is there twice adds nothing, its second weight is zero.
-  static PCAMD_DEV void locate(const Args& a, const Source& src, int t, uint32_t& page, uint32_t& place) {
-    t = t < src.last ? t : src.last;
-    const int n = a.page_index(t);
-    page = static_cast<uint32_t>(src.pages[n - src.first]);
-    page = page < a.pages ? page : a.pages - 1;
-    place = t - n * a.page;
-  }
+  // Where a token is: its page's number and its place in the page. Cut to the
+  // last token: what lies behind it is not read, and a row that is there twice
+  // adds nothing, its second weight is zero.
+  struct Place {
+    uint32_t page, place;
+    PCAMD_DEV void find(const Args& a, const Source& src, int t) {
+      t = t < src.last ? t : src.last;
+      const int n = a.page_index(t);
+      page = static_cast<uint32_t>(src.pages[n - src.first]);
+      place = t - n * a.page;
+    }
+    PCAMD_DEV uint64_t at(const Args& a, uint32_t page_stride, uint32_t token_stride) const {
+      return uint64_t{page < a.pages ? page : a.pages - 1} * page_stride + uint64_t{place} * token_stride;
+    }
+  };
 
   static PCAMD_DEV int rotation() { return __builtin_amdgcn_readfirstlane(threadIdx.x / 64) * (BLOCKS > 4 ? 2 : 1); }
 
@@ -186,24 +192,29 @@ struct Kernel {
     const uint8_t* rope[RR];
     const float* scale[S_COPIES > 0 ? S_COPIES : 1];
 
-    PCAMD_DEV void prepare(const Args& a, const Source& src, int t0, int wr, int lane) {
+    Place of_row[RR], of_scale[S_COPIES > 0 ? S_COPIES : 1];
+
+    // in two parts: the page numbers come from LDS, and the first part's reads have arrived when the second uses them
+    PCAMD_DEV void find(const Args& a, const Source& src, int t0, int wr, int lane) {
+#pragma unroll
+      for (int i = 0; i < RR; ++i) of_row[i].find(a, src, t0 + wr * RW + 8 * i + lane / 8);
+#pragma unroll
+      for (int i = 0; i < S_COPIES; ++i) of_scale[i].find(a, src, t0 + (wr * S_LANES + i * 64 + lane) % TOK);
+    }
+    PCAMD_DEV void address(const Args& a, int wr, int lane) {
 #pragma unroll
       for (int i = 0; i < RR; ++i) {
-        const int row = wr * RW + 8 * i + lane / 8, c = (lane % 8) ^ swizzle(row);
-        uint32_t page, place;
-        locate(a, src, t0 + row, page, place);
-        latent[i] = static_cast<const uint8_t*>(a.latent) +
-                    (uint64_t{page} * a.slp + uint64_t{place} * a.slt) * (FP8 ? 1 : 2) + 16 * c;
-        rope[i] = c < CR ? static_cast<const uint8_t*>(a.rope) + (uint64_t{page} * a.srp + uint64_t{place} * a.srt) * 2 + 16 * c
-                         : nullptr;
+        const int c = (lane % 8) ^ swizzle(wr * RW + 8 * i + lane / 8);
+        latent[i] = static_cast<const uint8_t*>(a.latent) + of_row[i].at(a, a.slp, a.slt) * (FP8 ? 1 : 2) + 16 * c;
+        rope[i] = c < CR ? static_cast<const uint8_t*>(a.rope) + of_row[i].at(a, a.srp, a.srt) * 2 + 16 * c : nullptr;
       }
 #pragma unroll
-      for (int i = 0; i < S_COPIES; ++i) {
-        const int j = wr * S_LANES + i * 64 + lane;  // [group][token]
-        uint32_t page, place;
-        locate(a, src, t0 + j % TOK, page, place);
-        scale[i] = a.scale + uint64_t{page} * a.ssp + uint64_t{place} * a.sst + j / TOK;
-      }
+      for (int i = 0; i < S_COPIES; ++i)  // [group][token]
+        scale[i] = a.scale + of_scale[i].at(a, a.ssp, a.sst) + (wr * S_LANES + i * 64 + lane) / TOK;
+    }
+    PCAMD_DEV void prepare(const Args& a, const Source& src, int t0, int wr, int lane) {
+      find(a, src, t0, wr, lane);
+      address(a, wr, lane);
     }
     // Copy k of COPIES into the tile at LDS address `tile`. The latent rows'
     // blocks come in an order that starts elsewhere in every wave: eight rows'
@@ -230,11 +241,11 @@ struct Kernel {
         emit_all<K + 1>(tile, wr, lane);
       }
     }
-    // the copies that step n of `steps` gives time for: from step 4 on, evenly
+    // the copies that step n of `steps` gives time for: from step 8 on, evenly
     template <int K = 0>
     PCAMD_DEV void emit_at(int n, int steps, uint32_t tile, int wr, int lane) const {
       if constexpr (K < COPIES) {
-        if (4 + K * (steps - 5) / COPIES == n) emit<K>(tile, wr, lane);
+        if (8 + K * (steps - 9) / COPIES == n) emit<K>(tile, wr, lane);
         emit_at<K + 1>(n, steps, tile, wr, lane);
       }
     }
@@ -606,13 +617,13 @@ struct Kernel {
       if constexpr (PIPE) {
         acc c[1];
         auto to_scores = [&](int k) { s[k] = c[0][k] * a.scale_log2; };
-        auto look = [&](int i, float top) {  // before step i's weights: its mask and reference point
+        auto look = [&](int i, float top) {  // before step i's weights: its mask and reference point; top: the row's
           const int tb = first_token(i);
           if (tb + TOK > all_see) {
             mask(tb);
-            top = maximum();
+            top = row_max<MR>(maximum());
           }
-          refer(row_max<MR>(top));
+          refer(top);
         };
         wait_copies<(AHEAD - 1) * COPIES>();
         barrier();
@@ -620,11 +631,11 @@ struct Kernel {
         settle(c);
 #pragma unroll
         for (int k = 0; k < 16; ++k) to_scores(k);
-        look(0, maximum());
+        look(0, row_max<MR>(maximum()));
         auto step = [&](int i, auto more) {
           constexpr bool MORE = decltype(more)::value;  // another step follows
-          auto weigh = [&](int k) {                     // element k of step i's weights
-            s[k] = __builtin_amdgcn_exp2f(s[k] - m);
+          auto weigh = [&](int k) { s[k] = __builtin_amdgcn_exp2f(s[k] - m); };  // element k of step i's weights
+          auto add = [&](int k) {
             l += s[k];
             if (k & 1) weights(0, 0, k / 2);
           };
@@ -633,25 +644,36 @@ struct Kernel {
             barrier();
             Copies copies;
             scores(tile_of(i + 1), c, [&](int k) {
-              if (k == 1) copies.prepare(a, src, first_token(i + AHEAD), wr, lane);
+              if (k == 1) copies.find(a, src, first_token(i + AHEAD), wr, lane);
+              if (k == 6) copies.address(a, wr, lane);
               copies.emit_at(k, NA, tile_of(i + AHEAD), wr, lane);
-              if (k % (NA / 16) == 0 && k / (NA / 16) < 16) weigh(k / (NA / 16));
+              constexpr int EVERY = NA / 16;  // products an element
+              if (k % EVERY == 0 && k / EVERY < 16) weigh(k / EVERY);
+              if (k % EVERY == EVERY - 1 && k / EVERY < 16) add(k / EVERY);
               if (k == NA - 3) first_values(tile_of(i));
             });
             settle(c);
-            float top[2] = {kNoMax, kNoMax};
+            float top = kNoMax;
             values(tile_of(i), [&](int k) {
-              if (k % (NP / 16) == 0) {
-                const int e = k / (NP / 16);
-                to_scores(e);
-                top[e & 1] = fmaxf(top[e & 1], s[e]);
+              constexpr int EACH = NP < 32 ? 2 : 1;  // elements a product, from the second on
+              if (k > 0 && (k - 1) * EACH < 16) {
+#pragma unroll
+                for (int e = (k - 1) * EACH; e < k * EACH; ++e) to_scores(e);
               }
+              if (k > 1 && (k - 2) * EACH < 16) {
+#pragma unroll
+                for (int e = (k - 2) * EACH; e < (k - 1) * EACH; ++e) top = fmaxf(top, s[e]);
+              }
+              if (k == 16 / EACH + 3) top = row_max<MR>(top);
             });
-            look(i + 1, fmaxf(top[0], top[1]));
+            look(i + 1, top);
           } else {
             first_values(tile_of(i));
 #pragma unroll
-            for (int k = 0; k < 16; ++k) weigh(k);
+            for (int k = 0; k < 16; ++k) {
+              weigh(k);
+              add(k);
+            }
             values(tile_of(i), nothing);
           }
         };
@@ -672,7 +694,8 @@ struct Kernel {
           }
           auto ahead = [&](int k) {
             if constexpr (WR > 1 && MR == 16) {
-              if (k == 1) copies.prepare(a, src, first_token(i + AHEAD), wr, lane);
+              if (k == 1) copies.find(a, src, first_token(i + AHEAD), wr, lane);
+              if (k == 6) copies.address(a, wr, lane);
               copies.emit_at(k, NA, tile_of(i + AHEAD), wr, lane);
             }
           };
@@ -692,7 +715,8 @@ struct Kernel {
           for (int k = 0; k < PK * 4; ++k) weights(tile, 0, k);
           values(tile, [&](int k) {
             if constexpr (WR == 1) {
-              if (k == 2) copies.prepare(a, src, first_token(i + AHEAD), wr, lane);
+              if (k == 1) copies.find(a, src, first_token(i + AHEAD), wr, lane);
+              if (k == 8) copies.address(a, wr, lane);
             }
           });
           if constexpr (WR == 1) {
@@ -791,7 +815,7 @@ __global__ __launch_bounds__(NT, 1) void decode_kernel(Args a) {
 // a workgroup takes a row's 128 columns, and eight groups of lanes share the
 // pieces.
 constexpr int kFewPieces = 8;
-constexpr int kJoinGroups = 1024;  // four workgroups a CU
+constexpr int kJoinGroups = 1024;  // four workgroups a CU; twice as many take as long
 
 struct Joins {
   int4 join[2][NT];  // few pieces, many: {sequence, row tile, 1, last workgroup}
