@@ -9,8 +9,6 @@
 // second product: the order of tokens within a contraction is free, so V^T is
 // read in the order in which S^T came out. P never leaves the registers.
 //
-// Tiles lie in LDS as rows of 16-byte chunks, chunk c of row t at c ^ f(t):
-// rows that are read together start in different banks.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -126,29 +124,36 @@ struct ScoreMfma<DT, 32> {
   static PCAMD_DEV void settle(acc& c) { asm volatile("s_nop 15" : "+v"(c)); }
 };
 
-// f(t) for rows of CH chunks. ROWS: 16 consecutive rows are read at one chunk
-// (the S^T operand); they have to differ in their place within 256 bytes.
-// Rows of a multiple of 256 bytes: also the four rows t & ~3 .. +3 of a
-// transposing read, 64 bytes each, which bits 2-3 of f tell apart.
-template <int CH>
-PCAMD_DEV int swz(int t) {
-  if constexpr (CH % 16 == 0) return ((t & 3) << 2) | ((t >> 2) & 3);
-  else if constexpr (CH % 8 == 0) return (t >> 1) & 7;
-  else return (t >> 2) & 3;
-}
-// f(t) for values alone (transposing reads only): 128-byte rows
-template <int CH>
-PCAMD_DEV int swz_v(int t) {
-  if constexpr (CH % 16 == 0) return swz<CH>(t);
-  else return ((t >> 1) & 1) << 2;
-}
-
 // Four rows' 16-bit elements of one column, transposed within groups of 16
 // lanes: lane i addresses 8 bytes of row i / 4 at columns 4 (i % 4), and
 // receives column i of the four rows.
 PCAMD_DEV uint2 read_tr4(const uint8_t* p) {
   return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(p)));
 }
+
+// ---- global -> LDS copies. Lane i's 16 (4) bytes at p land at lds + 16 i
+// (4 i). Inline asm: the compiler would wait for every copy in flight before any
+// read of LDS.
+PCAMD_DEV void copy16(const void* p, uint32_t lds) {
+  asm volatile("global_load_lds_dwordx4 %0, off" ::"v"(p), "{m0}"(lds) : "memory");
+}
+PCAMD_DEV void copy4(const void* p, uint32_t lds) {
+  asm volatile("global_load_lds_dword %0, off" ::"v"(p), "{m0}"(lds) : "memory");
+}
+// until at most N copies are in flight
+template <int N>
+PCAMD_DEV void wait_copies() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+// all waves' reads of LDS are behind them, and their copies that they waited for are there
+PCAMD_DEV void tile_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// Tiles of 128-byte rows: chunk c (16 bytes) of row t lies at c ^ f(t). t & 1 is
+// a half of the 256 bytes that 16 lanes may read without conflict; the rest of
+// t spreads 16 consecutive rows' equal chunks (keys) over all eight places, and
+// the four rows that a transposing read takes at once (64 bytes each) over both
+// halves of a row: the reversed bits of t / 2.
+PCAMD_DEV int swizzle16(int t) { return ((t & 2) << 1) | ((t >> 1) & 2) | ((t >> 3) & 1); }
 
 // max / sum over the lane groups that share a row: swapping rows of 16 (32)
 // lanes between two copies leaves one group's values in each
@@ -183,11 +188,6 @@ template <int DT, bool HI>
 PCAMD_DEV uint32_t widen2(uint32_t c) {
   if constexpr (DT == kBF16) return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c, 1.0f, HI));
   else return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(c, 1.0f, HI));
-}
-
-PCAMD_DEV uint32_t lds_addr(const void* p) {
-  return __builtin_amdgcn_readfirstlane(
-      static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const uint8_t*)p)));
 }
 
 }  // namespace attn

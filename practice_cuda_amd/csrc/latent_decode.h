@@ -133,7 +133,6 @@ struct Kernel {
   //   16-bit values: rows 4 h .. + 3 (MR 32: 64 bytes each; MR 16, two h: 32
   //   bytes each) - the reversed bits of t / 2;
   //   8-bit values: rows 4 h .. + 3 and QSTEP further on, 32 (16) bytes each.
-  static PCAMD_DEV int swizzle16(int t) { return ((t & 2) << 1) | ((t >> 1) & 2) | ((t >> 3) & 1); }
   static PCAMD_DEV int swizzle(int t) {
     if constexpr (FP8) return ((t & 2) << 1) | (((t >> 2) ^ (t >> 3)) & 2) | ((t >> 2) & 1);
     else return swizzle16(t);
@@ -148,21 +147,6 @@ struct Kernel {
   static constexpr int S_COPIES = (S_LANES + 63) / 64;
   static constexpr int COPIES = RR * (BLOCKS + 1) + S_COPIES;
   static_assert((AHEAD - 1) * COPIES < 64, "the counter of copies in flight ends at 63");
-
-  // lane i's 16 (4) bytes at p + OFF land at lds + 16 i (4 i). Inline asm: the
-  // compiler would wait for every copy in flight before any read of LDS. The
-  // instruction adds its offset to both addresses.
-  template <int OFF>
-  static PCAMD_DEV void copy16(const void* p, uint32_t lds) {
-    asm volatile("global_load_lds_dwordx4 %0, off offset:%2" ::"v"(p), "{m0}"(lds - OFF), "n"(OFF) : "memory");
-  }
-  static PCAMD_DEV void copy4(const void* p, uint32_t lds) {
-    asm volatile("global_load_lds_dword %0, off" ::"v"(p), "{m0}"(lds) : "memory");
-  }
-  template <int N>
-  static PCAMD_DEV void wait_copies() {
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
-  }
 
   struct Source {
     const int32_t* pages;  // in LDS: the table from page number `first` on
@@ -225,10 +209,10 @@ struct Kernel {
       if constexpr (K < RR * BLOCKS) {
         constexpr int i = K / BLOCKS;
         const int b = (K + rotation()) % BLOCKS;
-        copy16<0>(latent[i] + b * 128, tile + b * BLOCK + (wr * RW + 8 * i) * 128);
+        copy16(latent[i] + b * 128, tile + b * BLOCK + (wr * RW + 8 * i) * 128);
       } else if constexpr (K < RR * (BLOCKS + 1)) {
         constexpr int i = K - RR * BLOCKS;
-        if (CR == 8 || rope[i]) copy16<0>(rope[i], tile + ROPE + (wr * RW + 8 * i) * 128);
+        if (CR == 8 || rope[i]) copy16(rope[i], tile + ROPE + (wr * RW + 8 * i) * 128);
       } else {
         constexpr int i = K - RR * (BLOCKS + 1);
         if (S_LANES % 64 == 0 || i * 64 + lane < S_LANES) copy4(scale[i], tile + SCALES + (wr * S_LANES + i * 64) * 4);
@@ -370,7 +354,7 @@ struct Kernel {
   // Steps s0 .. s0 + n - 1 of a row tile's `steps`.
   static PCAMD_DEV void segment(const Args& a, uint8_t* lds, int b, int rt, int s0, int n, int steps, int len,
                                 int slot) {
-    const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64;
+    const int tid = threadIdx.x, lane = tid % 64, wave = __builtin_amdgcn_readfirstlane(tid / 64);
     const int wr = wave % WR, wt = wave / WR;
     const Lane L(lane);
     const int h = L.h, ln = L.ln;
@@ -411,10 +395,10 @@ struct Kernel {
 #pragma unroll
         for (int k = 0; k < QBLOCKS; ++k) {
           const int blk = (k + rotation()) % QBLOCKS;  // as for the tiles
-          copy16<0>(p + blk * 64, to + blk * QBLOCK + 8 * i * 128);
+          copy16(p + blk * 64, to + blk * QBLOCK + 8 * i * 128);
         }
         if (c < CR)
-          copy16<0>(static_cast<const uint16_t*>(a.q_rope) + b * a.qrb + tn * a.qrs + hd * a.qrh + 8 * c,
+          copy16(static_cast<const uint16_t*>(a.q_rope) + b * a.qrb + tn * a.qrs + hd * a.qrh + 8 * c,
                     to + QBLOCKS * QBLOCK + 8 * i * 128);
       }
     }
@@ -612,8 +596,6 @@ struct Kernel {
         start();
       }
       const int count = upto - done;
-      // the tile has arrived for all waves of its group, and all have left the one before it
-      auto barrier = [] { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
       if constexpr (PIPE) {
         acc c[1];
         auto to_scores = [&](int k) { s[k] = c[0][k] * a.scale_log2; };
@@ -626,7 +608,7 @@ struct Kernel {
           refer(top);
         };
         wait_copies<(AHEAD - 1) * COPIES>();
-        barrier();
+        tile_barrier();
         scores(tile_of(0), c, nothing);
         settle(c);
 #pragma unroll
@@ -641,7 +623,7 @@ struct Kernel {
           };
           if constexpr (MORE) {
             wait_copies<(AHEAD - 2) * COPIES>();
-            barrier();
+            tile_barrier();
             Copies copies;
             scores(tile_of(i + 1), c, [&](int k) {
               if (k == 1) copies.find(a, src, first_token(i + AHEAD), wr, lane);
@@ -682,7 +664,7 @@ struct Kernel {
       } else {
         for (int i = 0; i < count; ++i) {
           wait_copies<(AHEAD - 1) * COPIES>();
-          if constexpr (WR > 1) barrier();
+          if constexpr (WR > 1) tile_barrier();
           const uint32_t tile = tile_of(i);
           const int tb = first_token(i);
           Copies copies;

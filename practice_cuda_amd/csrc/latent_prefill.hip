@@ -6,8 +6,9 @@
 //   s[i, j] = scale * q[i] . k[j], j <= i + (keys - queries) where causal
 //   o[i] = sum_j softmax(s[i])[j] v[j],   lse[i] = log sum_j exp(s[i, j])
 //
-// One workgroup holds 128 query rows of one head (32 a wave) and walks over
-// the keys it sees in tiles of 64 with a running maximum and sum.
+// One workgroup holds NR x 128 query rows of one head, NR x 32 a wave, and
+// walks over the keys they see in steps of 32 with a running maximum and sum.
+// With NR = 2 every operand read from LDS serves two matrix products.
 #include <hip/hip_runtime.h>
 
 #include <atomic>
@@ -22,22 +23,24 @@ namespace prefill {
 using namespace attn;
 
 constexpr int NT = 256;
-constexpr int BM = 128, BN = 64;
+constexpr int BN = 32;  // keys of a tile and step
 
 struct Args {
   const void* q; const void* k; const void* kr; const void* v;
-  int64_t sqt, sqh, skt, skh, srt, svt, svh;
+  int64_t sqt, sqh, skh, svh;
+  uint32_t skt, srt, svt;  // of a token, in bytes
   const int32_t* cu_q; const int32_t* cu_k;
   void* out; int64_t sot, soh;
   float* lse; int64_t slt, slh;
   int64_t total_q, total_k;
-  int sequences, heads, causal;
-  float scale_log2;
+  int sequences, heads, causal, max_tiles;  // max_tiles: bound of a head's row tiles
+  float scale_log2;                         // not negative: run() is told of a sign by `negate`
+  uint32_t negate;                          // sign bits of two elements, or 0
 };
 
 struct Tile {
   int64_t q0, k0;  // first token of the sequence's queries and keys
-  int qn, kn, row0;
+  int qn, kn;
 };
 
 PCAMD_DEV int64_t clamp64(int64_t v, int64_t lo, int64_t hi) { return v < lo ? lo : v > hi ? hi : v; }
@@ -55,26 +58,81 @@ PCAMD_DEV Tile sequence(const Args& a, int i) {
     t.k0 = clamp64(a.cu_k[i], 0, a.total_k);
     t.kn = static_cast<int>(clamp64(a.cu_k[i + 1], t.k0, a.total_k) - t.k0);
   }
-  t.row0 = 0;
   return t;
 }
 
-template <int DT, int DN, int DR, int DV>
+// How far (log2) a score may pass its row's reference point before that moves
+// (as in the decode kernels: weights are floating point).
+template <int DT>
+constexpr float kSlack = DT == kF16 ? 8.0f : 40.0f;
+
+template <int DT, int DN, int DR, int DV, int NR>
 struct Kernel {
   typedef Mfma<DT, 32> M;
+  static constexpr int BM = NR * 128;
   static constexpr int DK = DN + DR;
-  static constexpr int CN = DN / 8, CK = DK / 8, CV = DV / 8;
-  static constexpr int KS = DK / 16, OB = DV / 32, SUB = BN / 32;
-  static constexpr int KT = BN * DK * 2, VT = BN * DV * 2;
-  static constexpr int LDS = KT + VT;
+  static constexpr int KS = DK / 16, OB = DV / 32;
+  // A tile in LDS: blocks of 128 bytes a key, [block][key]: the key's own part,
+  // its rotary part (one block, half filled where it is 64 bytes), the value.
+  static constexpr int KB = DN / 64, VB = DV / 64, CR = DR / 8;
+  static constexpr int BLOCK = BN * 128, VALUES = (KB + 1) * BLOCK, TILE = (KB + 1 + VB) * BLOCK;
+  static constexpr int NB = 6;  // tiles: the one in use, the next, and four on their way
+  // in the ring's place: queries [block][row][128 bytes] first, output rows last
+  static constexpr int QROWS = NR * 32, QBLOCK = QROWS * 128, QUERIES = (KB + 1) * QBLOCK;
+  static constexpr int OPITCH = DV * 2 + 16, OUT = QROWS * OPITCH;
+  static constexpr int max3(int a, int b, int c) { return a > b ? (a > c ? a : c) : (b > c ? b : c); }
+  static constexpr int BODY = max3(NB * TILE, 4 * QUERIES, 4 * OUT);
+  static constexpr int LDS = BODY + 64;
+  static constexpr int COPIES = KB + 1 + VB;  // of a wave for a tile: 8 keys x 128 bytes each
+
+  // a wave's share of a tile's copies: 8 of its keys
+  struct Copies {
+    const uint8_t* k;
+    const uint8_t* r;
+    const uint8_t* v;
+    // Keys past the last are copies of it: their weights are zero.
+    PCAMD_DEV void address(const uint8_t* kn, const uint8_t* kr, const uint8_t* kv, const Args& a, int t0, int last,
+                           int wave, int lane) {
+      const int row = wave * 8 + lane / 8, c = (lane % 8) ^ swizzle16(row);
+      const uint32_t t = t0 + row < last ? t0 + row : last;
+      k = kn + uint64_t{t} * a.skt + 16 * c;
+      r = c < CR ? kr + uint64_t{t} * a.srt + 16 * c : nullptr;
+      v = kv + uint64_t{t} * a.svt + 16 * c;
+    }
+    template <int K>
+    PCAMD_DEV void emit(uint32_t tile, int wave) const {
+      const uint32_t to = tile + K * BLOCK + wave * 8 * 128;
+      if constexpr (K < KB) copy16(k + K * 128, to);
+      else if constexpr (K > KB) copy16(v + (K - KB - 1) * 128, to);
+      else if (CR == 8 || r) copy16(r, to);
+    }
+    template <int K = 0>
+    PCAMD_DEV void emit_all(uint32_t tile, int wave) const {
+      if constexpr (K < COPIES) {
+        emit<K>(tile, wave);
+        emit_all<K + 1>(tile, wave);
+      }
+    }
+    template <int K = 0>
+    PCAMD_DEV void emit_at(int n, uint32_t tile, int wave) const {  // spread over the products, from the third on
+      if constexpr (K < COPIES) {
+        if (2 + K * (KS - 2) / COPIES == n) emit<K>(tile, wave);
+        emit_at<K + 1>(n, tile, wave);
+      }
+    }
+  };
 
   static PCAMD_DEV void run(const Args& a, uint8_t* lds) {
-    __shared__ int wave_total[NT / 64];
-    __shared__ int found[2];
-    const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64;
+    int* wave_total = reinterpret_cast<int*>(lds + BODY);
+    int* found = wave_total + NT / 64;
+    const int tid = threadIdx.x, lane = tid % 64, wave = __builtin_amdgcn_readfirstlane(tid / 64);
     const int h = lane / 32, ln = lane % 32;
-    const int head = blockIdx.x % a.heads;
-    const int want = blockIdx.x / a.heads;
+    // Workgroups go round the eight XCDs: each gets a run of neighbouring heads,
+    // one head's tiles after the other's, so that its L2 holds the keys in use
+    // and they lie in all of its channels.
+    const int per = gridDim.x / 8, item = blockIdx.x % 8 * per + blockIdx.x / 8;
+    const int head = item / a.max_tiles, want = item - head * a.max_tiles;
+    if (head >= a.heads) return;
 
     // ---- the tile's sequence: a running count of tiles over the sequences
     if (tid == 0) found[0] = -1;
@@ -106,134 +164,315 @@ struct Kernel {
       if (found[0] >= 0) break;
     }
     if (found[0] < 0) return;
-    Tile t = sequence(a, found[0]);
-    t.row0 = found[1] * BM;
-
-    // ---- this lane's row
-    const int row = t.row0 + wave * 32 + ln;
-    const bool live = row < t.qn;
+    const Tile t = sequence(a, found[0]);
+    const int row0 = found[1] * BM;
     const int past = t.kn - t.qn;
-    const int limit = !live ? 0 : a.causal ? row + past + 1 : t.kn;
-    uint4 q[KS];
-    {
-      const uint16_t* p = static_cast<const uint16_t*>(a.q) + (t.q0 + row) * a.sqt + head * a.sqh;
+
+    // ---- queries: whole lines into LDS, a lane's row from there
+    const uint8_t* qp = static_cast<const uint8_t*>(a.q) + 2 * (t.q0 * a.sqt + head * a.sqh);
 #pragma unroll
-      for (int k = 0; k < KS; ++k)
-        q[k] = live ? *reinterpret_cast<const uint4*>(p + 16 * k + 8 * h) : make_uint4(0, 0, 0, 0);
+    for (int i = 0; i < QROWS / 8; ++i) {
+      const int r = 8 * i + lane / 8, c = (lane % 8) ^ swizzle16(r);
+      int row = row0 + wave * QROWS + r;
+      if (row >= t.qn) row = t.qn - 1;  // a spare row computes what another one does, and is not stored
+      const uint8_t* p = qp + 2 * row * a.sqt + 16 * c;
+      const uint32_t to = wave * QUERIES + 8 * i * 128;
+#pragma unroll
+      for (int b = 0; b < KB; ++b) copy16(p + b * 128, to + b * QBLOCK);
+      if (c < CR) copy16(p + DN * 2, to + KB * QBLOCK);
     }
-    const int last = t.row0 + BM < t.qn ? t.row0 + BM : t.qn;  // end of the tile's rows
-    int keys = a.causal ? last + past : t.kn;
+    wait_copies<0>();
+    uint4 q[NR][KS];
+#pragma unroll
+    for (int u = 0; u < NR; ++u)
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        const int c = 2 * k < DN / 8 ? 2 * k : 2 * k - DN / 8, b = 2 * k < DN / 8 ? c / 8 : KB;
+        uint4 x = *reinterpret_cast<const uint4*>(lds + wave * QUERIES + b * QBLOCK + (u * 32 + ln) * 128 +
+                                                  (((c % 8 + h) ^ swizzle16(ln)) << 4));
+        x.x ^= a.negate; x.y ^= a.negate; x.z ^= a.negate; x.w ^= a.negate;
+        q[u][k] = x;
+      }
+#pragma unroll
+    for (int u = 0; u < NR; ++u)
+#pragma unroll
+      for (int k = 0; k < KS; ++k) asm volatile("" : "+v"(q[u][k].x), "+v"(q[u][k].y), "+v"(q[u][k].z), "+v"(q[u][k].w));
+    __syncthreads();  // the tiles take the queries' place
+
+    int row[NR], limit[NR];  // this lane's rows, and how many keys they see
+#pragma unroll
+    for (int u = 0; u < NR; ++u) {
+      row[u] = row0 + wave * QROWS + u * 32 + ln;
+      const int n = a.causal ? row[u] + past + 1 : t.kn;
+      limit[u] = n < t.kn ? n : t.kn;
+    }
+    const int first = row0 + wave * QROWS + past + 1;
+    const int all_see = a.causal && first < t.kn ? first : t.kn;  // keys that every row of the wave sees
+    const int end = row0 + BM < t.qn ? row0 + BM : t.qn;          // of the tile's rows
+    int keys = a.causal ? end + past : t.kn;
     if (keys > t.kn) keys = t.kn;
-    const uint16_t* kn = static_cast<const uint16_t*>(a.k) + t.k0 * a.skt + head * a.skh;
-    const uint16_t* kr = static_cast<const uint16_t*>(a.kr) + t.k0 * a.srt;
-    const uint16_t* kv = static_cast<const uint16_t*>(a.v) + t.k0 * a.svt + head * a.svh;
+    const int tiles = keys > 0 ? (keys + BN - 1) / BN : 0;
+    const uint8_t* kn = static_cast<const uint8_t*>(a.k) + t.k0 * a.skt + 2 * head * a.skh;
+    const uint8_t* kr = static_cast<const uint8_t*>(a.kr) + t.k0 * a.srt;
+    const uint8_t* kv = static_cast<const uint8_t*>(a.v) + t.k0 * a.svt + 2 * head * a.svh;
 
-    f32x16 o[OB];
+    f32x16 o[NR][OB];
+    float m[NR], nm[NR], l[NR];  // reference point (in units of s), minus its log2, sum of weights
 #pragma unroll
-    for (int j = 0; j < OB; ++j) o[j] = f32x16{};
-    float m = kNoMax, l = 0.0f;
-    for (int t0 = 0; t0 < keys; t0 += BN) {
-      __syncthreads();
-      for (int j = tid; j < BN * CK; j += NT) {
-        const int r = j / CK, c = j % CK;
-        uint4 x = make_uint4(0, 0, 0, 0);
-        if (t0 + r < t.kn)
-          x = *reinterpret_cast<const uint4*>(c < CN ? kn + (t0 + r) * a.skt + 8 * c : kr + (t0 + r) * a.srt + 8 * (c - CN));
-        *reinterpret_cast<uint4*>(lds + r * (DK * 2) + ((c ^ swz<CK>(r)) << 4)) = x;
-      }
-      for (int j = tid; j < BN * CV; j += NT) {
-        const int r = j / CV, c = j % CV;
-        uint4 x = make_uint4(0, 0, 0, 0);
-        if (t0 + r < t.kn) x = *reinterpret_cast<const uint4*>(kv + (t0 + r) * a.svt + 8 * c);
-        *reinterpret_cast<uint4*>(lds + KT + r * (DV * 2) + ((c ^ swz_v<CV>(r)) << 4)) = x;
-      }
-      __syncthreads();
-
-      f32x16 s[SUB];
+    for (int u = 0; u < NR; ++u) {
 #pragma unroll
-      for (int sub = 0; sub < SUB; ++sub) {
-        s[sub] = f32x16{};
-#pragma unroll
-        for (int k = 0; k < KS; ++k) {
-          const int r = sub * 32 + ln;
-          const uint4 x = *reinterpret_cast<const uint4*>(lds + r * (DK * 2) + (((2 * k + h) ^ swz<CK>(r)) << 4));
-          s[sub] = M::mul(x, q[k], s[sub]);
-        }
-      }
-      float top = m;
-#pragma unroll
-      for (int sub = 0; sub < SUB; ++sub)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int key = t0 + sub * 32 + (r / 4) * 8 + 4 * h + r % 4;
-          s[sub][r] = key < limit ? s[sub][r] * a.scale_log2 : -INFINITY;
-          top = fmaxf(top, s[sub][r]);
-        }
-      top = row_max<32>(top);
-      const float alpha = exp2f(m - top);
-      m = top;
-      float part = 0.0f;
-#pragma unroll
-      for (int sub = 0; sub < SUB; ++sub)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          s[sub][r] = exp2f(s[sub][r] - m);
-          part += s[sub][r];
-        }
-      l = l * alpha + part;
-#pragma unroll
-      for (int j = 0; j < OB; ++j) o[j] *= alpha;
-#pragma unroll
-      for (int kk = 0; kk < BN / 16; ++kk) {
-        const f32x16& x = s[kk / 2];
-        const int r0 = (kk & 1) * 8;
-        const uint4 p = make_uint4(Elem<DT>::narrow2(x[r0], x[r0 + 1]), Elem<DT>::narrow2(x[r0 + 2], x[r0 + 3]),
-                                   Elem<DT>::narrow2(x[r0 + 4], x[r0 + 5]), Elem<DT>::narrow2(x[r0 + 6], x[r0 + 7]));
-#pragma unroll
-        for (int j = 0; j < OB; ++j) {
-          const int i16 = lane % 16, g16 = lane / 16;
-          const int col = j * 32 + 16 * (g16 & 1) + 4 * (i16 & 3);
-          uint2 w[2];
-#pragma unroll
-          for (int y = 0; y < 2; ++y) {
-            const int r = kk * 16 + y * 8 + 4 * h + i16 / 4;
-            w[y] = read_tr4(lds + KT + r * (DV * 2) + (((col >> 3) ^ swz_v<CV>(r)) << 4) + ((col & 4) << 1));
-          }
-          o[j] = M::mul(make_uint4(w[0].x, w[0].y, w[1].x, w[1].y), p, o[j]);
-        }
-      }
+      for (int j = 0; j < OB; ++j) o[u][j] = f32x16{};
+      m[u] = kNoMax;
+      nm[u] = 0.0f;
+      l[u] = 0.0f;
     }
-    l = row_sum<32>(l);
-    if (!live) return;
-    const float inv = l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : NAN;
-    uint16_t* out = static_cast<uint16_t*>(a.out) + (t.q0 + row) * a.sot + head * a.soh;
+
+    // ---- The parts of a step. As in the decode kernels, reads of LDS run ahead
+    // of the products that take them, held in place by sched_barrier; `beside(i)`
+    // is other work for the time of the products with operand i.
+    const uint32_t lane_k = ln * 128 + ((h ^ swizzle16(ln)) << 4);
+    const int i16 = lane % 16, tv = 4 * h + (i16 >> 2);
+    const uint32_t lane_v =
+        VALUES + tv * 128 + (((2 * ((lane / 16) & 1) + ((i16 >> 1) & 1)) ^ swizzle16(tv)) << 4) + 8 * (i16 & 1);
+    auto key = [&](uint32_t tile, int k) {
+      const int c = 2 * k < DN / 8 ? 2 * k : 2 * k - DN / 8, b = 2 * k < DN / 8 ? c / 8 : KB;
+      return *reinterpret_cast<const uint4*>(lds + ((tile + lane_k) ^ (c % 8 << 4)) + b * BLOCK);
+    };
+    auto value = [&](uint32_t tile, int j, int kk) {
+      const int x = 4 * j % 8 << 4, at = 4 * j / 8 * BLOCK + kk * 16 * 128;
+      const uint2 y = read_tr4(lds + ((tile + lane_v) ^ x) + at);
+      const uint2 z = read_tr4(lds + ((tile + lane_v) ^ (x ^ 16)) + at + 8 * 128);
+      return make_uint4(y.x, y.y, z.x, z.y);
+    };
+    constexpr int DA = KS < 5 ? KS : 5;                      // key operands read ahead
+    constexpr int NP = 2 * OB, DVA = NP < 4 ? NP : 4;        // value operands (contraction step n / OB, block n % OB), ahead
+    uint4 val[DVA];
+    f32x16 c[NR];
+    float s[NR][16];
+    uint32_t p[NR][8];
+    auto scores = [&](uint32_t tile, auto beside) {
+      uint4 raw[DA];
 #pragma unroll
-    for (int j = 0; j < OB; ++j)
+      for (int k = 0; k < DA; ++k) raw[k] = key(tile, k);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int y = 0; y < 4; ++y) {
-        const uint2 w = make_uint2(Elem<DT>::narrow2(o[j][4 * y] * inv, o[j][4 * y + 1] * inv),
-                                   Elem<DT>::narrow2(o[j][4 * y + 2] * inv, o[j][4 * y + 3] * inv));
-        *reinterpret_cast<uint2*>(out + 32 * j + 8 * y + 4 * h) = w;
+      for (int k = 0; k < KS; ++k) {
+        const uint4 x = raw[k % DA];
+#pragma unroll
+        for (int u = 0; u < NR; ++u) c[u] = M::mul(x, q[u][k], k == 0 ? f32x16{} : c[u]);
+        if (k + DA < KS) raw[k % DA] = key(tile, k + DA);
+        beside(k);
+        __builtin_amdgcn_sched_barrier(0);
       }
-    if (a.lse && h == 0) a.lse[(t.q0 + row) * a.slt + head * a.slh] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
+    };
+    auto first_values = [&](uint32_t tile) {
+#pragma unroll
+      for (int n = 0; n < DVA; ++n) val[n] = value(tile, n % OB, n / OB);
+    };
+    auto values = [&](uint32_t tile, auto beside) {
+#pragma unroll
+      for (int n = 0; n < NP; ++n) {
+        const int j = n % OB, kk = n / OB;
+        const uint4 x = val[n % DVA];
+#pragma unroll
+        for (int u = 0; u < NR; ++u) {
+          const uint32_t* w = p[u] + 4 * kk;
+          o[u][j] = M::mul(x, make_uint4(w[0], w[1], w[2], w[3]), o[u][j]);
+        }
+        if (n + DVA < NP) val[n % DVA] = value(tile, (n + DVA) % OB, (n + DVA) / OB);
+        beside(n);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    };
+    // element e of NR * 16: row u = e / 16, register e % 16
+    auto take = [&](int e) { s[e / 16][e % 16] = c[e / 16][e % 16]; };
+    auto weigh = [&](int e) {
+      const int u = e / 16, r = e % 16;
+      s[u][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][r], a.scale_log2, nm[u]));
+    };
+    auto add = [&](int e) {  // two elements at a time
+      const int u = e / 16, r = e % 16;
+      if (r & 1) {
+        l[u] += s[u][r - 1] + s[u][r];
+        p[u][r / 2] = Elem<DT>::narrow2(s[u][r - 1], s[u][r]);
+      }
+    };
+    float top[NR];
+    auto look = [&](int t0) {  // before the weights of the step at key t0: its mask and reference point
+      if (t0 + 32 > all_see) {
+#pragma unroll
+        for (int u = 0; u < NR; ++u) {
+          top[u] = kNoMax;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            s[u][r] = t0 + (r / 4) * 8 + 4 * h + r % 4 < limit[u] ? s[u][r] : -INFINITY;
+            top[u] = fmaxf(top[u], s[u][r]);
+          }
+          top[u] = row_max<32>(top[u]);
+        }
+      }
+      bool passed = false;
+#pragma unroll
+      for (int u = 0; u < NR; ++u) passed |= (top[u] - m[u]) * a.scale_log2 > kSlack<DT>;
+      if (__any(passed)) {
+#pragma unroll
+        for (int u = 0; u < NR; ++u) {
+          const float to = fmaxf(m[u], top[u]), alpha = __builtin_amdgcn_exp2f((m[u] - to) * a.scale_log2);
+          m[u] = to;
+          nm[u] = -to * a.scale_log2;
+          l[u] *= alpha;
+#pragma unroll
+          for (int j = 0; j < OB; ++j) {
+            // block by block through the vector registers, back to where the products keep it
+            asm volatile("" : "+a"(o[u][j]));
+            o[u][j] *= alpha;
+            asm volatile("" : "+a"(o[u][j]));
+          }
+        }
+      }
+    };
+    auto maxima = [&]() {
+#pragma unroll
+      for (int u = 0; u < NR; ++u) {
+        top[u] = s[u][0];
+#pragma unroll
+        for (int r = 1; r < 16; ++r) top[u] = fmaxf(top[u], s[u][r]);
+        top[u] = row_max<32>(top[u]);
+      }
+    };
+    auto nothing = [](int) {};
+    constexpr int E = NR * 16;
+    // the step with a tile whose scores are in s; the next tile's scores are computed beside
+    auto step = [&](uint32_t tile, int t0, uint32_t next, auto more, auto copies) {
+      if constexpr (decltype(more)::value) {
+        scores(next, [&](int k) {
+          copies(k);
+          // E elements over KS operands' time, each pair's sum and rounding one operand later
+#pragma unroll
+          for (int e = 0; e < E; ++e) {
+            if (e * (KS - 1) / E == k) weigh(e);
+            if (e * (KS - 1) / E + 1 == k) add(e);
+          }
+          if (k == KS - 2) first_values(tile);
+        });
+#pragma unroll
+        for (int u = 0; u < NR; ++u) top[u] = kNoMax;
+        values(tile, [&](int n) {
+          constexpr int FROM = 1, OVER = NP - 2;  // elements over products FROM .. FROM + OVER - 1
+#pragma unroll
+          for (int e = 0; e < E; ++e)
+            if (FROM + e * OVER / E == n) {
+              take(e);
+              top[e / 16] = fmaxf(top[e / 16], s[e / 16][e % 16]);
+            }
+          if (n == NP - 1) {
+#pragma unroll
+            for (int u = 0; u < NR; ++u) top[u] = row_max<32>(top[u]);
+          }
+        });
+        // in ordinary registers from here on, not in those of the products' sums
+#pragma unroll
+        for (int e = 0; e < E; ++e) asm volatile("" : "+v"(s[e / 16][e % 16]));
+        look(t0 + 32);
+      } else {
+        first_values(tile);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          weigh(e);
+          add(e);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        values(tile, nothing);
+      }
+    };
+
+    if (tiles > 0) {
+      Copies copies;
+#pragma unroll
+      for (int i = 0; i < NB - 1; ++i) {
+        copies.address(kn, kr, kv, a, i * BN, t.kn - 1, wave, lane);
+        copies.emit_all(i * TILE, wave);
+      }
+      wait_copies<(NB - 2) * COPIES>();
+      tile_barrier();
+      scores(0, nothing);
+#pragma unroll
+      for (int e = 0; e < E; ++e) take(e);
+      maxima();
+      look(0);
+      uint32_t tile = 0, into = (NB - 1) * TILE;
+      for (int i = 0; i + 1 < tiles; ++i) {
+        // The next tile has arrived for all waves, and all have left the one
+        // before this: a tile further on takes its place.
+        wait_copies<(NB - 3) * COPIES>();
+        tile_barrier();
+        const uint32_t next = tile + TILE < NB * TILE ? tile + TILE : 0;
+        step(tile, i * BN, next, std::true_type{}, [&](int k) {
+          if (k == 1) copies.address(kn, kr, kv, a, (i + NB - 1) * BN, t.kn - 1, wave, lane);
+          copies.emit_at(k, into, wave);
+        });
+        into = tile;
+        tile = next;
+      }
+      step(tile, (tiles - 1) * BN, 0, std::false_type{}, nothing);
+      wait_copies<0>();
+    }
+
+    // ---- epilogue: output rows gather in LDS and leave as whole lines
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < NR; ++u) {
+      const float sum = row_sum<32>(l[u]);
+      const float inv = sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : NAN;
+      if (a.lse && h == 0 && row[u] < t.qn)
+        a.lse[(t.q0 + row[u]) * a.slt + head * a.slh] =
+            sum == 0.0f ? -INFINITY : (m[u] * a.scale_log2 + log2f(sum)) * kLn2;
+#pragma unroll
+      for (int j = 0; j < OB; ++j)
+#pragma unroll
+        for (int y = 0; y < 4; ++y)
+          *reinterpret_cast<uint2*>(lds + wave * OUT + (u * 32 + ln) * OPITCH + 64 * j + 16 * y + 8 * h) =
+              make_uint2(Elem<DT>::narrow2(o[u][j][4 * y] * inv, o[u][j][4 * y + 1] * inv),
+                         Elem<DT>::narrow2(o[u][j][4 * y + 2] * inv, o[u][j][4 * y + 3] * inv));
+    }
+    // each wave's rows are its own
+    uint16_t* out = static_cast<uint16_t*>(a.out) + t.q0 * a.sot + head * a.soh;
+    constexpr int PER = DV / 4;  // 8-byte pieces of a row
+#pragma unroll 4
+    for (int i = lane; i < QROWS * PER; i += 64) {
+      const int r = i / PER, d = i % PER, to = row0 + wave * QROWS + r;
+      const uint2 x = *reinterpret_cast<const uint2*>(lds + wave * OUT + r * OPITCH + 8 * d);
+      if (to < t.qn) *reinterpret_cast<uint2*>(out + to * a.sot + 4 * d) = x;
+    }
   }
 };
 
-template <int DT, int DN, int DR, int DV>
-__global__ __launch_bounds__(NT, 2) void prefill_kernel(Args a) {
+template <int DT, int DN, int DR, int DV, int NR>
+__global__ __launch_bounds__(NT, 1) void prefill_kernel(Args a) {
+  // all of the kernel's LDS, so that it starts at address 0: copies and tile addresses count on it
   extern __shared__ __align__(16) uint8_t lds[];
-  Kernel<DT, DN, DR, DV>::run(a, lds);
+  Kernel<DT, DN, DR, DV, NR>::run(a, lds);
+}
+
+template <int DT, int DN, int DR, int DV, int NR>
+int launch_rows(Args a, hipStream_t st) {
+  static std::atomic<uint64_t> done{0};
+  typedef Kernel<DT, DN, DR, DV, NR> K;
+  const auto kern = prefill_kernel<DT, DN, DR, DV, NR>;
+  const int rc = ensure_dynamic_lds(reinterpret_cast<const void*>(kern), K::LDS, st, done);
+  if (rc != PCAMD_OK) return rc;
+  const int64_t max_tiles = a.total_q / K::BM + a.sequences + 1, per = (max_tiles * a.heads + 7) / 8;
+  if (per * 8 >= (int64_t{1} << 32) / NT)
+    return set_error(PCAMD_ERR_UNSUPPORTED, "latent prefill: grid too large (%lld workgroups)", (long long)per * 8);
+  a.max_tiles = static_cast<int>(max_tiles);
+  kern<<<static_cast<uint32_t>(per * 8), NT, K::LDS, st>>>(a);
+  return check_launch("prefill_kernel");
 }
 
 template <int DT, int DN, int DR, int DV>
-int launch(const Args& a, int64_t grid, hipStream_t st) {
-  static std::atomic<uint64_t> done{0};
-  const auto kern = prefill_kernel<DT, DN, DR, DV>;
-  constexpr int bytes = Kernel<DT, DN, DR, DV>::LDS;
-  const int rc = ensure_dynamic_lds(reinterpret_cast<const void*>(kern), bytes, st, done);
-  if (rc != PCAMD_OK) return rc;
-  kern<<<static_cast<uint32_t>(grid), NT, bytes, st>>>(a);
-  return check_launch("prefill_kernel");
+int launch(const Args& a, hipStream_t st) {
+  // 128-row tiles where 256-row ones would leave CUs idle
+  return a.total_q * a.heads <= 256 * 256 ? launch_rows<DT, DN, DR, DV, 1>(a, st) : launch_rows<DT, DN, DR, DV, 2>(a, st);
 }
 
 }  // namespace prefill
@@ -255,8 +494,8 @@ extern "C" int pcamd_latent_prefill(const void* q, const void* k_nope, const voi
   if (!wide && !narrow)
     return set_error(PCAMD_ERR_UNSUPPORTED, "key, rotary and value widths must be 128, 64, 128 or 64, 32, 64; got %lld, %lld, %lld",
                      (long long)nope_dim, (long long)rope_dim, (long long)v_dim);
-  if (total_q > INT32_MAX || total_k > INT32_MAX || sequences > INT32_MAX / 2)
-    return set_error(PCAMD_ERR_UNSUPPORTED, "latent prefill: more than 2^31 - 1 tokens");
+  if (total_q > (1 << 30) || total_k > (1 << 30) || sequences > (1 << 30) || heads > (1 << 20))
+    return set_error(PCAMD_ERR_UNSUPPORTED, "latent prefill: more than 2^30 tokens or sequences, or 2^20 heads");
   if (total_q == 0 || heads == 0) return PCAMD_OK;
   if (!q || !cu_q || !cu_k || !out || (total_k && (!k_nope || !k_rope || !v)))
     return set_error(PCAMD_ERR_INVALID, "null pointer");
@@ -264,14 +503,22 @@ extern "C" int pcamd_latent_prefill(const void* q, const void* k_nope, const voi
   if (odd(q, 16) || odd(k_nope, 16) || odd(k_rope, 16) || odd(v, 16) || odd(out, 8) || sqt % 8 || sqh % 8 || skt % 8 ||
       skh % 8 || srt % 8 || svt % 8 || svh % 8 || sot % 4 || soh % 4)
     return set_error(PCAMD_ERR_INVALID, "rows of queries, keys and values must be 16-byte aligned, of the output 8-byte");
-  const int64_t grid = heads * (total_q / prefill::BM + sequences + 1);
-  if (grid >= (int64_t{1} << 32) / prefill::NT)
-    return set_error(PCAMD_ERR_UNSUPPORTED, "latent prefill: grid too large (%lld workgroups)", (long long)grid);
-  prefill::Args a{q, k_nope, k_rope, v, sqt, sqh, skt, skh, srt, svt, svh, cu_q, cu_k, out, sot, soh, lse, slt, slh,
-                  total_q, total_k, static_cast<int>(sequences), static_cast<int>(heads), causal != 0,
-                  softmax_scale * attn::kLog2e};
+  for (const int64_t stride : {skt, srt, svt})
+    if (stride < 0 || stride > (1 << 30)) return set_error(PCAMD_ERR_UNSUPPORTED, "latent prefill: a token stride past 2^30 elements");
+  prefill::Args a{};
+  a.q = q; a.k = k_nope; a.kr = k_rope; a.v = v;
+  a.sqt = sqt; a.sqh = sqh; a.skh = skh; a.svh = svh;
+  a.skt = static_cast<uint32_t>(2 * skt); a.srt = static_cast<uint32_t>(2 * srt); a.svt = static_cast<uint32_t>(2 * svt);
+  a.cu_q = cu_q; a.cu_k = cu_k;
+  a.out = out; a.sot = sot; a.soh = soh; a.lse = lse; a.slt = slt; a.slh = slh;
+  a.total_q = total_q; a.total_k = total_k;
+  a.sequences = static_cast<int>(sequences); a.heads = static_cast<int>(heads); a.causal = causal != 0;
+  // The kernel compares scores before they are scaled: a negative scale's sign
+  // goes to the queries, and none is so small that a masked score's times it is not -inf.
+  a.scale_log2 = fabsf(softmax_scale) * attn::kLog2e;
+  if (a.scale_log2 < 1e-30f) a.scale_log2 = 1e-30f;
+  a.negate = softmax_scale < 0.0f ? 0x80008000u : 0u;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (dtype == kBF16)
-    return wide ? prefill::launch<kBF16, 128, 64, 128>(a, grid, st) : prefill::launch<kBF16, 64, 32, 64>(a, grid, st);
-  return wide ? prefill::launch<kF16, 128, 64, 128>(a, grid, st) : prefill::launch<kF16, 64, 32, 64>(a, grid, st);
+  if (dtype == kBF16) return wide ? prefill::launch<kBF16, 128, 64, 128>(a, st) : prefill::launch<kBF16, 64, 32, 64>(a, st);
+  return wide ? prefill::launch<kF16, 128, 64, 128>(a, st) : prefill::launch<kF16, 64, 32, 64>(a, st);
 }
