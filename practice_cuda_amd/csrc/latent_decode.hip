@@ -96,11 +96,17 @@ extern "C" int pcamd_latent_decode(
   if (!q_latent || !q_rope || !lens || !out || (max_pages && !table) ||
       (pages && (!cache_latent || !cache_rope || (f8 && !cache_scale))))
     return set_error(PCAMD_ERR_INVALID, "null pointer");
+  // a dimension with one place has any stride
+  auto bad = [](int64_t places, int64_t stride, int64_t unit) { return places > 1 && stride % unit; };
   const int64_t per16 = f8 ? 16 : 8;
   if (!decode::aligned16(q_latent) || !decode::aligned16(q_rope) || !decode::aligned16(cache_latent) ||
-      !decode::aligned16(cache_rope) || (reinterpret_cast<uintptr_t>(out) & 7) || qlb % 8 || qls % 8 || qlh % 8 ||
-      qrb % 8 || qrs % 8 || qrh % 8 || clp % per16 || clt % per16 || crp % 8 || crt % 8 || ob % 4 || os % 4 || oh % 4)
+      !decode::aligned16(cache_rope) || (reinterpret_cast<uintptr_t>(out) & 7) || bad(batch, qlb, 8) ||
+      bad(new_tokens, qls, 8) || bad(heads, qlh, 8) || bad(batch, qrb, 8) || bad(new_tokens, qrs, 8) ||
+      bad(heads, qrh, 8) || bad(pages, clp, per16) || bad(page_size, clt, per16) || bad(pages, crp, 8) ||
+      bad(page_size, crt, 8) || bad(batch, ob, 4) || bad(new_tokens, os, 4) || bad(heads, oh, 4))
     return set_error(PCAMD_ERR_INVALID, "rows of queries and cache must be 16-byte aligned, of the output 8-byte");
+  if (pages <= 1) clp = crp = csp = 0;
+  if (page_size == 1) clt = crt = cst = 0;
   for (const int64_t stride : {clp, clt, crp, crt, csp, cst})
     if (stride < 0 || stride > INT32_MAX) return set_error(PCAMD_ERR_UNSUPPORTED, "latent decode: a cache stride past 2^31 elements");
   if (pages > UINT32_MAX) return set_error(PCAMD_ERR_UNSUPPORTED, "latent decode: more than 2^32 - 1 pages");

@@ -459,11 +459,11 @@ int launch_rows(Args a, hipStream_t st) {
   static std::atomic<uint64_t> done{0};
   typedef Kernel<DT, DN, DR, DV, NR> K;
   const auto kern = prefill_kernel<DT, DN, DR, DV, NR>;
-  const int rc = ensure_dynamic_lds(reinterpret_cast<const void*>(kern), K::LDS, st, done);
-  if (rc != PCAMD_OK) return rc;
   const int64_t max_tiles = a.total_q / K::BM + a.sequences + 1, per = (max_tiles * a.heads + 7) / 8;
   if (per * 8 >= (int64_t{1} << 32) / NT)
     return set_error(PCAMD_ERR_UNSUPPORTED, "latent prefill: grid too large (%lld workgroups)", (long long)per * 8);
+  const int rc = ensure_dynamic_lds(reinterpret_cast<const void*>(kern), K::LDS, st, done);
+  if (rc != PCAMD_OK) return rc;
   a.max_tiles = static_cast<int>(max_tiles);
   kern<<<static_cast<uint32_t>(per * 8), NT, K::LDS, st>>>(a);
   return check_launch("prefill_kernel");
@@ -500,9 +500,12 @@ extern "C" int pcamd_latent_prefill(const void* q, const void* k_nope, const voi
   if (!q || !cu_q || !cu_k || !out || (total_k && (!k_nope || !k_rope || !v)))
     return set_error(PCAMD_ERR_INVALID, "null pointer");
   auto odd = [](const void* p, int64_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) != 0; };
-  if (odd(q, 16) || odd(k_nope, 16) || odd(k_rope, 16) || odd(v, 16) || odd(out, 8) || sqt % 8 || sqh % 8 || skt % 8 ||
-      skh % 8 || srt % 8 || svt % 8 || svh % 8 || sot % 4 || soh % 4)
+  auto bad = [](int64_t places, int64_t stride, int64_t unit) { return places > 1 && stride % unit; };  // one place: any stride
+  if (odd(q, 16) || odd(k_nope, 16) || odd(k_rope, 16) || odd(v, 16) || odd(out, 8) || bad(total_q, sqt, 8) ||
+      bad(heads, sqh, 8) || bad(total_k, skt, 8) || bad(heads, skh, 8) || bad(total_k, srt, 8) || bad(total_k, svt, 8) ||
+      bad(heads, svh, 8) || bad(total_q, sot, 4) || bad(heads, soh, 4))
     return set_error(PCAMD_ERR_INVALID, "rows of queries, keys and values must be 16-byte aligned, of the output 8-byte");
+  if (total_k <= 1) skt = srt = svt = 0;
   for (const int64_t stride : {skt, srt, svt})
     if (stride < 0 || stride > (1 << 30)) return set_error(PCAMD_ERR_UNSUPPORTED, "latent prefill: a token stride past 2^30 elements");
   prefill::Args a{};

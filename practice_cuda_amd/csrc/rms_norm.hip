@@ -283,8 +283,10 @@ int launch_norm(const NormArgs& a, hipStream_t st) {
   using std::integral_constant;
   if (a.n <= 512) return go(integral_constant<int, 64>{}, integral_constant<int, 1>{});
   if (a.n <= 2048) return go(integral_constant<int, 64>{}, integral_constant<int, 4>{});
-  if (a.n <= 8192) return go(integral_constant<int, 256>{}, integral_constant<int, 4>{});
-  if (a.n <= 16384) return go(integral_constant<int, 256>{}, integral_constant<int, 8>{});
+  if (a.n <= 4096) return go(integral_constant<int, 256>{}, integral_constant<int, 2>{});
+  // 4096 x 7168 bf16 with a residual: 512 lanes 50.3 us, 256 lanes (4 chunks each) 54.7, 1024 (1 each) 62.6
+  if (a.n <= 8192) return go(integral_constant<int, 512>{}, integral_constant<int, 2>{});
+  if (a.n <= 16384) return go(integral_constant<int, 512>{}, integral_constant<int, 4>{});
   if (a.n <= 65536) return go(integral_constant<int, 1024>{}, integral_constant<int, 8>{});
   return go(integral_constant<int, 1024>{}, integral_constant<int, 0>{});
 }

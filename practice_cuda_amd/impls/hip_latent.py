@@ -67,34 +67,41 @@ class LatentCache:
 
 
 def _check_cache(cache: LatentCache, dtype: torch.dtype, device: torch.device):
-    """(latent width, rotary width, pages, page size, scale strides) of a well-formed cache."""
+    """(latent width, rotary width, pages, page size, arguments) of a well-formed cache; the
+    arguments are its addresses, dtype and strides in the entry points' order."""
     latent, rope, scale = cache.latent, cache.rope, cache.scale
-    if latent.ndim != 3 or rope.ndim != 3 or latent.shape[:2] != rope.shape[:2]:
+    shape, sl, sr = latent.shape, latent.stride(), rope.stride()
+    if len(shape) != 3 or rope.ndim != 3 or shape[:2] != rope.shape[:2]:
         raise ValueError("a cache's latent and rope must be [pages, page_size, width]; got "
                          f"{tuple(latent.shape)} and {tuple(rope.shape)}")
-    pages, page, dl = latent.shape
+    pages, page, dl = shape
+    kind = latent.dtype
     if page < 1:
         raise ValueError("a cache's pages must hold at least one token")
     if rope.dtype != dtype:
         raise ValueError(f"the cache's rope must have the tokens' dtype {dtype}, got {rope.dtype}")
-    if latent.stride(2) != 1 or rope.stride(2) != 1:
+    if sl[2] != 1 or sr[2] != 1:
         raise ValueError("a cache must be contiguous along its last dimension")
     if latent.device != device or rope.device != device:
         raise ValueError(f"the cache must be on {device}, got {latent.device} and {rope.device}")
-    if latent.dtype == torch.float8_e4m3fn:
+    if kind == torch.float8_e4m3fn:
         if scale is None:
             raise ValueError("an fp8 cache needs its scales")
         if scale.shape != (pages, page, dl // 128) or scale.dtype != torch.float32 or scale.device != device:
             raise ValueError(f"the cache's scale must be float32 with shape {(pages, page, dl // 128)} on {device}, "
                              f"got {scale.dtype}, {tuple(scale.shape)}, {scale.device}")
-        if scale.stride(2) != 1:
+        ss = scale.stride()
+        if ss[2] != 1 and dl > 128:
             raise ValueError("the cache's scale must be contiguous along its last dimension")
-        return dl, rope.shape[2], pages, page, scale.stride()[:2]
-    if latent.dtype != dtype:
-        raise ValueError(f"the cache's latent must be {dtype} or float8_e4m3fn, got {latent.dtype}")
-    if scale is not None:
-        raise ValueError("only an fp8 cache has scales")
-    return dl, rope.shape[2], pages, page, (0, 0)
+        scale_args = (scale.data_ptr(), ss[0], ss[1])
+    else:
+        if kind != dtype:
+            raise ValueError(f"the cache's latent must be {dtype} or float8_e4m3fn, got {kind}")
+        if scale is not None:
+            raise ValueError("only an fp8 cache has scales")
+        scale_args = (0, 0, 0)
+    return dl, rope.shape[2], pages, page, (latent.data_ptr(), _lib.dtype_code(kind), sl[0], sl[1],
+                                            rope.data_ptr(), sr[0], sr[1], *scale_args, pages, page)
 
 
 def hip_latent_append(
@@ -128,7 +135,7 @@ def hip_latent_append(
                          f"{tuple(slots.shape)}")
     if slots.device != latent.device or rope.device != latent.device:
         raise ValueError(f"slots and rope must be on {latent.device}, got {slots.device} and {rope.device}")
-    dl, dr, pages, page, (csp, cst) = _check_cache(cache, latent.dtype, latent.device)
+    dl, dr, _, _, cache_args = _check_cache(cache, latent.dtype, latent.device)
     if latent.shape[1] != dl or rope.shape[1] != dr:
         raise ValueError(f"the cache holds widths {dl} and {dr}, got {latent.shape[1]} and {rope.shape[1]}")
     if weight is not None:
@@ -139,15 +146,13 @@ def hip_latent_append(
             raise ValueError(f"weight must be on {latent.device}, got {weight.device}")
     if eps < 0 or norm_eps < 0:
         raise ValueError(f"eps and norm_eps must not be negative, got {eps} and {norm_eps}")
-    _lib.require_gpu_tensor(latent, "latent")
+    if not latent.is_cuda:
+        _lib.require_gpu_tensor(latent, "latent")
     rc = _lib.launch(
         _lib.lib().pcamd_latent_append, latent,
         latent.data_ptr(), rope.data_ptr(), _lib.dtype_code(latent.dtype), tokens, dl, dr,
         latent.stride(0), rope.stride(0), _lib.ptr(weight), 0 if weight is None else _lib.dtype_code(weight.dtype),
-        slots.data_ptr(), slots.element_size(),
-        cache.latent.data_ptr(), _lib.dtype_code(cache.latent.dtype), cache.latent.stride(0), cache.latent.stride(1),
-        cache.rope.data_ptr(), cache.rope.stride(0), cache.rope.stride(1),
-        _lib.ptr(cache.scale), csp, cst, pages, page, float(norm_eps), float(eps))
+        slots.data_ptr(), slots.element_size(), *cache_args, norm_eps, eps)
     if rc == _lib.ERR_UNSUPPORTED:
         raise ValueError(_lib.lib().pcamd_last_error().decode())
     _lib.check(rc, "pcamd_latent_append")
@@ -165,7 +170,7 @@ def _check_out(out: Optional[torch.Tensor], shape: tuple, like: torch.Tensor) ->
     return out
 
 
-def _check_aligned(*rows) -> None:
+def _check_aligned(rows) -> None:
     """Rows that the kernels read in 16-byte pieces (names with their tensors)."""
     for name, t in rows:
         size = t.element_size()
@@ -208,12 +213,13 @@ def hip_latent_decode(
     dtype, device = q_latent.dtype, q_latent.device
     if dtype not in _TOKEN_DTYPES or q_rope.dtype != dtype:
         raise ValueError(f"queries must both be bfloat16 or float16, got {dtype} and {q_rope.dtype}")
-    if q_latent.stride(3) != 1 or q_rope.stride(3) != 1:
+    sl, sr = q_latent.stride(), q_rope.stride()
+    if sl[3] != 1 or sr[3] != 1:
         raise ValueError("queries must be contiguous along their last dimension")
     if q_rope.device != device:
         raise ValueError(f"q_rope must be on {device}, got {q_rope.device}")
     batch, new, heads, width = q_latent.shape
-    dl, dr, pages, page, (csp, cst) = _check_cache(cache, dtype, device)
+    dl, dr, _, page, cache_args = _check_cache(cache, dtype, device)
     if (dl, dr) not in DECODE_WIDTHS:
         raise ValueError(f"latent and rotary widths must be one of {DECODE_WIDTHS}, got {(dl, dr)}")
     if width != dl or q_rope.shape[3] != dr:
@@ -227,9 +233,11 @@ def hip_latent_decode(
         raise ValueError(f"seq_lens must be contiguous int32 with shape ({batch},) on {device}; "
                          f"got {seq_lens.dtype}, {tuple(seq_lens.shape)}, {seq_lens.device}")
     out = _check_out(out, (batch, new, heads, dl), q_latent)
-    _check_aligned(("q_latent", q_latent), ("q_rope", q_rope), ("the cache's latent", cache.latent),
-                   ("the cache's rope", cache.rope), ("out", out))
-    _lib.require_gpu_tensor(q_latent, "q_latent")
+    rows = (("q_latent", q_latent), ("q_rope", q_rope), ("the cache's latent", cache.latent),
+            ("the cache's rope", cache.rope), ("out", out))
+    if not q_latent.is_cuda:
+        _check_aligned(rows)
+        _lib.require_gpu_tensor(q_latent, "q_latent")
     lse = torch.empty((batch, new, heads), dtype=torch.float32, device=device) if return_lse else None
     L = _lib.lib()
     max_pages = block_table.shape[1]
@@ -237,22 +245,26 @@ def hip_latent_decode(
     if need < 0:
         raise ValueError(L.pcamd_last_error().decode())
     workspace = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    so = out.stride()
     rc = _lib.launch(
         L.pcamd_latent_decode, q_latent,
         q_latent.data_ptr(), q_rope.data_ptr(), _lib.dtype_code(dtype), batch, new, heads, dl, dr,
-        *_strides(q_latent), *_strides(q_rope),
-        cache.latent.data_ptr(), _lib.dtype_code(cache.latent.dtype), *_strides(cache.latent),
-        cache.rope.data_ptr(), *_strides(cache.rope), _lib.ptr(cache.scale), csp, cst, pages, page,
+        sl[0], sl[1], sl[2], sr[0], sr[1], sr[2], *cache_args,
         block_table.data_ptr(), block_table.stride(0), max_pages, seq_lens.data_ptr(),
-        out.data_ptr(), *_strides(out), _lib.ptr(lse), new * heads, heads, 1,
-        float(softmax_scale), _lib.ptr(workspace), need)
-    _lib.check(rc, "pcamd_latent_decode")
+        out.data_ptr(), so[0], so[1], so[2], _lib.ptr(lse), new * heads, heads, 1,
+        softmax_scale, _lib.ptr(workspace), need)
+    if rc != 0:
+        _refused(rc, "pcamd_latent_decode", rows)
     return (out, lse) if return_lse else out
 
 
-def _strides(t: torch.Tensor) -> tuple:
-    """The strides of all dimensions but the last; 0 where one has a single place (its stride may be anything)."""
-    return tuple(s if n > 1 else 0 for s, n in zip(t.stride()[:-1], t.shape))
+def _refused(rc: int, what: str, rows) -> None:
+    """What a launch did not take: bad alignment and sizes past the kernels' are the caller's values."""
+    if rc == _lib.ERR_INVALID:
+        _check_aligned(rows)
+    if rc == _lib.ERR_UNSUPPORTED:
+        raise ValueError(_lib.lib().pcamd_last_error().decode())
+    _lib.check(rc, what)
 
 
 def hip_latent_prefill(
@@ -301,26 +313,28 @@ def hip_latent_prefill(
     for t, name in ((k_nope, "k_nope"), (k_rope, "k_rope"), (v, "v")):
         if t.dtype != dtype or t.device != device:
             raise ValueError(f"{name} must be {dtype} on {device}, got {t.dtype} on {t.device}")
-    for t, name in ((q, "q"), (k_nope, "k_nope"), (k_rope, "k_rope"), (v, "v")):
-        if t.stride(-1) != 1:
-            raise ValueError(f"{name} must be contiguous along its last dimension; strides={t.stride()}")
+    sq, sk, sr, sv = q.stride(), k_nope.stride(), k_rope.stride(), v.stride()
+    for strides, name in ((sq, "q"), (sk, "k_nope"), (sr, "k_rope"), (sv, "v")):
+        if strides[-1] != 1:
+            raise ValueError(f"{name} must be contiguous along its last dimension; strides={strides}")
     for t, name in ((cu_q, "cu_q"), (cu_k, "cu_k")):
         if (t.ndim != 1 or t.shape != cu_q.shape or t.shape[0] < 1 or t.dtype != torch.int32 or t.device != device
                 or t.stride(0) != 1):
             raise ValueError(f"cu_q and cu_k must be contiguous int32 [n + 1] on {device}; {name} is {t.dtype}, "
                              f"{tuple(t.shape)}, {t.device}")
     out = _check_out(out, (total_q, heads, dv), q)
-    _check_aligned(("q", q), ("k_nope", k_nope), ("k_rope", k_rope), ("v", v), ("out", out))
-    _lib.require_gpu_tensor(q, "q")
+    rows = (("q", q), ("k_nope", k_nope), ("k_rope", k_rope), ("v", v), ("out", out))
+    if not q.is_cuda:
+        _check_aligned(rows)
+        _lib.require_gpu_tensor(q, "q")
     lse = torch.empty((total_q, heads), dtype=torch.float32, device=device) if return_lse else None
-    L = _lib.lib()
+    so = out.stride()
     rc = _lib.launch(
-        L.pcamd_latent_prefill, q,
+        _lib.lib().pcamd_latent_prefill, q,
         q.data_ptr(), k_nope.data_ptr(), k_rope.data_ptr(), v.data_ptr(), _lib.dtype_code(dtype),
-        total_q, total_k, heads, dn, dr, dv, *_strides(q), *_strides(k_nope), *_strides(k_rope), *_strides(v),
-        cu_q.data_ptr(), cu_k.data_ptr(), cu_q.shape[0] - 1, out.data_ptr(), *_strides(out), _lib.ptr(lse), heads, 1,
-        1.0 / math.sqrt(dk) if softmax_scale is None else float(softmax_scale), int(causal))
-    if rc == _lib.ERR_UNSUPPORTED:
-        raise ValueError(L.pcamd_last_error().decode())
-    _lib.check(rc, "pcamd_latent_prefill")
+        total_q, total_k, heads, dn, dr, dv, sq[0], sq[1], sk[0], sk[1], sr[0], sv[0], sv[1],
+        cu_q.data_ptr(), cu_k.data_ptr(), cu_q.shape[0] - 1, out.data_ptr(), so[0], so[1], _lib.ptr(lse), heads, 1,
+        1.0 / math.sqrt(dk) if softmax_scale is None else softmax_scale, 1 if causal else 0)
+    if rc != 0:
+        _refused(rc, "pcamd_latent_prefill", rows)
     return (out, lse) if return_lse else out

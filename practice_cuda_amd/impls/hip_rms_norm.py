@@ -25,9 +25,7 @@ from . import _common as C
 _GROUP = 128
 
 
-def _rows(t: torch.Tensor) -> tuple[int, int]:
-    """(batch, row) strides of a 2D or 3D tensor."""
-    return (0, t.stride(0)) if t.ndim == 2 else (t.stride(0), t.stride(1))
+_NAMES = {t: str(t) for t in C._FP8_DTYPES}
 
 
 def hip_rms_norm_quant(
@@ -50,45 +48,53 @@ def hip_rms_norm_quant(
     quantization. A group with a NaN keeps it as a NaN code; its scale is that
     of the other values."""
     C.check_quant_input(x, fp8_dtype, "rms norm quant")
-    n = x.shape[-1]
-    if weight.shape != (n,) or weight.stride(0) != 1 and n > 1:
+    shape, strides, dtype, device = x.shape, x.stride(), x.dtype, x.device
+    n = shape[-1]
+    if weight.shape != (n,) or n > 1 and weight.stride(0) != 1:
         raise ValueError(f"weight must be contiguous with shape ({n},), got {tuple(weight.shape)}, "
                          f"strides={weight.stride()}")
     if weight.dtype not in C._INPUT_DTYPES:
         raise ValueError(f"weight dtype must be float32, bfloat16 or float16, got {weight.dtype}")
-    if x.stride(-1) != 1 and n > 1:
-        raise ValueError(f"x must be contiguous along its last dimension; strides={x.stride()}")
+    if strides[-1] != 1 and n > 1:
+        raise ValueError(f"x must be contiguous along its last dimension; strides={strides}")
     if eps < 0 or norm_eps < 0:
         raise ValueError(f"eps and norm_eps must not be negative, got {eps} and {norm_eps}")
-    if weight.device != x.device:
-        raise ValueError(f"weight must be on {x.device}, got {weight.device}")
+    if weight.device != device:
+        raise ValueError(f"weight must be on {device}, got {weight.device}")
+    flat = len(shape) == 2  # rows without a batch dimension: batch stride 0
+    batch, m = (1, shape[0]) if flat else shape[:2]
     if residual is None:
         if residual_out is not None:
             raise ValueError("residual_out needs a residual")
-        srb = srm = sob = som = 0
+        residual_args, out_args = (0, 0, 0), (0, 0, 0)
     else:
         if residual_out is None:
-            residual_out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        for t, name in ((residual, "residual"), (residual_out, "residual_out")):
-            if t.shape != x.shape or t.dtype != x.dtype or t.device != x.device:
-                raise ValueError(f"{name} must be like x ({tuple(x.shape)}, {x.dtype}, {x.device}), got "
-                                 f"{tuple(t.shape)}, {t.dtype}, {t.device}")
-            if t.stride(-1) != 1 and n > 1:
-                raise ValueError(f"{name} must be contiguous along its last dimension; strides={t.stride()}")
-        (srb, srm), (sob, som) = _rows(residual), _rows(residual_out)
-    _lib.require_gpu_tensor(x, "x")
+            residual_out = torch.empty(shape, dtype=dtype, device=device)
+        residual_args = _like(residual, "residual", shape, dtype, device, flat)
+        out_args = _like(residual_out, "residual_out", shape, dtype, device, flat)
+    if not x.is_cuda:
+        _lib.require_gpu_tensor(x, "x")
     groups = -(-n // _GROUP)
-    q = torch.empty(x.shape, dtype=fp8_dtype, device=x.device)
-    scale = torch.empty((*x.shape[:-1], groups), dtype=torch.float32, device=x.device)
-    batch, m = (1, x.shape[0]) if x.ndim == 2 else (x.shape[0], x.shape[1])
+    q = torch.empty(shape, dtype=fp8_dtype, device=device)
+    scale = torch.empty((m, groups) if flat else (batch, m, groups), dtype=torch.float32, device=device)
     rc = _lib.launch(
         _lib.lib().pcamd_rms_norm_quant, x,
-        x.data_ptr(), _lib.dtype_code(x.dtype), batch, m, n, *_rows(x),
-        _lib.ptr(residual), srb, srm, weight.data_ptr(), _lib.dtype_code(weight.dtype),
+        x.data_ptr(), _lib.dtype_code(dtype), batch, m, n, 0 if flat else strides[0], strides[-2],
+        *residual_args, weight.data_ptr(), _lib.dtype_code(weight.dtype),
         q.data_ptr(), _lib.dtype_code(fp8_dtype), m * n, n, scale.data_ptr(), m * groups, groups,
-        _lib.ptr(residual_out), sob, som, float(norm_eps), _lib.FP8_MAX[fp8_dtype], float(eps))
+        *out_args, norm_eps, _lib.FP8_MAX[fp8_dtype], eps)
     _lib.check(rc, "pcamd_rms_norm_quant")
-    result = QuantResult(
-        tensor=q, dequant_scale=scale, impl="hip_rms_norm", granularity="block",
-        meta={"logical_shape": tuple(x.shape), "fp8_dtype": str(fp8_dtype), "block_m": 1, "block_n": _GROUP})
-    return result, residual_out
+    return QuantResult(q, scale, "hip_rms_norm", "block",
+                       {"logical_shape": tuple(shape), "fp8_dtype": _NAMES[fp8_dtype], "block_m": 1,
+                        "block_n": _GROUP}), residual_out
+
+
+def _like(t: torch.Tensor, name: str, shape, dtype, device, flat: bool) -> tuple[int, int, int]:
+    """(address, batch stride, row stride) of a tensor that has to be like x."""
+    if t.shape != shape or t.dtype != dtype or t.device != device:
+        raise ValueError(f"{name} must be like x ({tuple(shape)}, {dtype}, {device}), got "
+                         f"{tuple(t.shape)}, {t.dtype}, {t.device}")
+    strides = t.stride()
+    if strides[-1] != 1 and shape[-1] > 1:
+        raise ValueError(f"{name} must be contiguous along its last dimension; strides={strides}")
+    return t.data_ptr(), 0 if flat else strides[0], strides[-2]
