@@ -14,6 +14,7 @@
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
+#include <utility>
 
 #include "fp8_common.h"
 
@@ -28,6 +29,17 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4* lds_s16x4_ptr;
+
+// f(0), f(1), .. f(N - 1), each with its number as a type: unrolled whatever
+// the body's size
+template <typename F, int... I>
+PCAMD_DEV void unrolled(F& f, std::integer_sequence<int, I...>) {
+  (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, typename F>
+PCAMD_DEV void unrolled(F f) {
+  unrolled(f, std::make_integer_sequence<int, N>{});
+}
 
 // Scores are kept times log2(e). The running maximum starts at a finite value
 // below every score that is told apart from -inf, so that a row that has seen

@@ -168,8 +168,6 @@ struct Kernel {
     }
   };
 
-  static PCAMD_DEV int rotation() { return __builtin_amdgcn_readfirstlane(threadIdx.x / 64) * (BLOCKS > 4 ? 2 : 1); }
-
   // the addresses of a tile's copies, and the copies
   struct Copies {
     const uint8_t* latent[RR];
@@ -177,6 +175,8 @@ struct Kernel {
     const float* scale[S_COPIES > 0 ? S_COPIES : 1];
 
     Place of_row[RR], of_scale[S_COPIES > 0 ? S_COPIES : 1];
+    uint32_t rotation;  // a multiple of 256 bytes where a row has so many
+    PCAMD_DEV explicit Copies(int wave) : rotation(wave * (BLOCKS > 4 ? 2 : 1)) {}
 
     // in two parts: the page numbers come from LDS, and the first part's reads have arrived when the second uses them
     PCAMD_DEV void find(const Args& a, const Source& src, int t0, int wr, int lane) {
@@ -200,23 +200,24 @@ struct Kernel {
       find(a, src, t0, wr, lane);
       address(a, wr, lane);
     }
+    PCAMD_DEV void emit_latent(uint32_t tile, int wr, int i, uint32_t block) const {  // eight rows' 128 bytes
+      copy16(latent[i] + block * 128, tile + block * BLOCK + (wr * RW + 8 * i) * 128);
+    }
+    PCAMD_DEV void emit_rope(uint32_t tile, int wr, int i) const {
+      if (CR == 8 || rope[i]) copy16(rope[i], tile + ROPE + (wr * RW + 8 * i) * 128);
+    }
+    PCAMD_DEV void emit_scale(uint32_t tile, int wr, int lane, int i) const {
+      if (S_LANES % 64 == 0 || i * 64 + lane < S_LANES) copy4(scale[i], tile + SCALES + (wr * S_LANES + i * 64) * 4);
+    }
     // Copy k of COPIES into the tile at LDS address `tile`. The latent rows'
     // blocks come in an order that starts elsewhere in every wave: eight rows'
     // equal 128 bytes lie in few memory channels, and waves that asked for the
     // same block at the same time would leave the other channels idle.
     template <int K>
     PCAMD_DEV void emit(uint32_t tile, int wr, int lane) const {
-      if constexpr (K < RR * BLOCKS) {
-        constexpr int i = K / BLOCKS;
-        const int b = (K + rotation()) % BLOCKS;
-        copy16(latent[i] + b * 128, tile + b * BLOCK + (wr * RW + 8 * i) * 128);
-      } else if constexpr (K < RR * (BLOCKS + 1)) {
-        constexpr int i = K - RR * BLOCKS;
-        if (CR == 8 || rope[i]) copy16(rope[i], tile + ROPE + (wr * RW + 8 * i) * 128);
-      } else {
-        constexpr int i = K - RR * (BLOCKS + 1);
-        if (S_LANES % 64 == 0 || i * 64 + lane < S_LANES) copy4(scale[i], tile + SCALES + (wr * S_LANES + i * 64) * 4);
-      }
+      if constexpr (K < RR * BLOCKS) emit_latent(tile, wr, K / BLOCKS, (K + rotation) % BLOCKS);
+      else if constexpr (K < RR * (BLOCKS + 1)) emit_rope(tile, wr, K - RR * BLOCKS);
+      else emit_scale(tile, wr, lane, K - RR * (BLOCKS + 1));
     }
     template <int K = 0>
     PCAMD_DEV void emit_all(uint32_t tile, int wr, int lane) const {
@@ -295,7 +296,7 @@ struct Kernel {
     int groups = wanted > tiles ? wanted : tiles;
     if (groups > a.groups) groups = a.groups;
     // with few tiles every workgroup has one piece of one: nothing to weigh
-    const int FIXED = tiles * 16 >= groups ? kFixed<MR> : 0;
+    const int FIXED = tiles > 1 && tiles * 16 >= groups ? kFixed<MR> : 0;
     const Division div(a.row_tiles * (steps_all + a.batch * FIXED), groups);
     if (static_cast<int>(blockIdx.x) >= groups) {
       if (a.parts && tid == 0) a.joins[blockIdx.x] = make_int4(0, 0, -1, 0);
@@ -394,7 +395,7 @@ struct Kernel {
         const uint16_t* p = static_cast<const uint16_t*>(a.q_latent) + b * a.qlb + tn * a.qls + hd * a.qlh + 8 * c;
 #pragma unroll
         for (int k = 0; k < QBLOCKS; ++k) {
-          const int blk = (k + rotation()) % QBLOCKS;  // as for the tiles
+          const uint32_t blk = (k + 2 * wave) % QBLOCKS;  // in another order in every wave, as the tiles' copies
           copy16(p + blk * 64, to + blk * QBLOCK + 8 * i * 128);
         }
         if (c < CR)
@@ -429,7 +430,7 @@ struct Kernel {
       __syncthreads();
 #pragma unroll
       for (int i = 0; i < AHEAD; ++i) {
-        Copies c;
+        Copies c(wave);
         c.prepare(a, src, first_token(i), wr, lane);
         c.emit_all(tile_of(i), wr, lane);
       }
@@ -470,47 +471,59 @@ struct Kernel {
       for (int i = 0; i < DA; ++i) raw[i] = load_key(i);
       __builtin_amdgcn_sched_barrier(0);
       acc d[2];
+      float4 f;  // four tokens' scales of a group, read a step before their use
       uint4 next = operand(0);
-#pragma unroll
-      for (int k = 0; k < NA; ++k) {
-        const int sub = k / PER, r = k % PER;
+      unrolled<NA>([&](auto number) {
+        constexpr int k = decltype(number)::value, sub = k / PER, r = k % PER;
         const uint4 x = next;
         if (k + 1 < NA) {
           if (load_of(k + 1) != load_of(k) && load_of(k) + DA < TA) raw[load_of(k) % DA] = load_key(load_of(k) + DA);
           next = operand(k + 1);
         }
-        if (r < KR) {
+        if constexpr (r < KR) {
           c[sub] = r == 0 ? S::first(x, qr[0]) : S::mul(x, qr[r], c[sub]);
         } else if constexpr (!FP8) {
           c[sub] = S::mul(x, ql[r - KR], c[sub]);
         } else {
           // a group's partial scores in d, scaled into c while the next group's are summed
           constexpr int G = KL / GROUPS;
-          const int i = r - KR, g = i / G;
+          constexpr int i = r - KR, g = i / G;
           if (i % G == 0) d[g & 1] = S::first(x, ql[i]);
           else if (i % G == 1 && g > 0) d[g & 1] = S::mul_holding(x, ql[i], d[g & 1], d[(g - 1) & 1]);
           else d[g & 1] = S::mul(x, ql[i], d[g & 1]);
-          auto scale_in = [&](int group, int reg) {
-            const int q = sub * (M::REGS / 4) + reg / 4;
-            const float2 f = *reinterpret_cast<const float2*>(scales + group * TOK + q * M::QSTEP + reg % 4);
-            c[sub][reg] += f.x * d[group & 1][reg];
-            c[sub][reg + 1] += f.y * d[group & 1][reg + 1];
+          constexpr int QD = M::REGS / 4;  // quads of a sum
+          auto scales_of = [&](int group, int q) {
+            return *reinterpret_cast<const float4*>(scales + group * TOK + (sub * QD + q) * M::QSTEP);
           };
-          if (g > 0) {
-            // from the group's third product on the last of the group before has been written
+          auto scale_in = [&](int group, int q, float4 x) {
+            c[sub][4 * q] += x.x * d[group & 1][4 * q];
+            c[sub][4 * q + 1] += x.y * d[group & 1][4 * q + 1];
+            c[sub][4 * q + 2] += x.z * d[group & 1][4 * q + 2];
+            c[sub][4 * q + 3] += x.w * d[group & 1][4 * q + 3];
+          };
+          // from the group's third product on the last of the group before has been written
 #pragma unroll
-            for (int reg = 0; reg < M::REGS; reg += 2)
-              if (2 + reg / 2 * (G - 2) / (M::REGS / 2) == i % G) scale_in(g - 1, reg);
+          for (int q = 0; q < QD; ++q) {
+            const int at = 2 + q * (G - 2) / QD;
+            if (g > 0 && at == i % G) scale_in(g - 1, q, f);
+          }
+#pragma unroll
+          for (int q = 0; q < QD; ++q) {
+            const int at = 2 + q * (G - 2) / QD;
+            if (g > 0 && at == i % G + 1) f = scales_of(g - 1, q);
           }
           if (r == PER - 1) {
+            float4 last[QD];
+#pragma unroll
+            for (int q = 0; q < QD; ++q) last[q] = scales_of(g, q);
             S::settle(d[g & 1]);
 #pragma unroll
-            for (int reg = 0; reg < M::REGS; reg += 2) scale_in(g, reg);
+            for (int q = 0; q < QD; ++q) scale_in(g, q, last[q]);
           }
         }
         beside(k);
         __builtin_amdgcn_sched_barrier(0);
-      }
+      });
     };
     auto first_values = [&](uint32_t tile) {
 #pragma unroll
@@ -549,15 +562,21 @@ struct Kernel {
       }
     };
     uint32_t p[FP8 ? 2 : 1][PK * 4];  // P^T of a group of value columns, and of the next
-    auto weights = [&](uint32_t tile, int g, int i) {  // dword i: registers 2 i and 2 i + 1
-      float x0 = s[2 * i], x1 = s[2 * i + 1];
+    float4 fw;                        // with fp8: the scales of a quad of the weights' tokens
+    auto scales_of_weights = [&](uint32_t tile, int g, int q) {
+      if constexpr (FP8)
+        fw = *reinterpret_cast<const float4*>(lds + tile + SCALES + 4 * (4 * h + g * TOK + q * M::QSTEP));
+    };
+    auto weights = [&](int g, int q) {  // registers 4 q .. + 3
+      float x0 = s[4 * q], x1 = s[4 * q + 1], x2 = s[4 * q + 2], x3 = s[4 * q + 3];
       if constexpr (FP8) {
-        const float* scales = reinterpret_cast<const float*>(lds + tile + SCALES) + 4 * h;
-        const float2 f = *reinterpret_cast<const float2*>(scales + g * TOK + (2 * i / 4) * M::QSTEP + 2 * i % 4);
-        x0 *= f.x * kScaleUp<DT>;
-        x1 *= f.y * kScaleUp<DT>;
+        x0 *= fw.x * kScaleUp<DT>;
+        x1 *= fw.y * kScaleUp<DT>;
+        x2 *= fw.z * kScaleUp<DT>;
+        x3 *= fw.w * kScaleUp<DT>;
       }
-      p[FP8 ? g & 1 : 0][i] = Elem<DT>::narrow2(x0, x1);
+      p[FP8 ? g & 1 : 0][2 * q] = Elem<DT>::narrow2(x0, x1);
+      p[FP8 ? g & 1 : 0][2 * q + 1] = Elem<DT>::narrow2(x2, x3);
     };
     auto values = [&](uint32_t tile, auto beside) {  // O^T += V^T P^T
       auto operand = [&](int k) {
@@ -566,10 +585,9 @@ struct Kernel {
         else return x;
       };
       uint4 next = operand(0);
-#pragma unroll
-      for (int k = 0; k < NP; ++k) {
+      unrolled<NP>([&](auto number) {
         constexpr int PER_GROUP = NP / (FP8 ? GROUPS : 1);
-        const int j = k / PK, kk = k % PK, g = FP8 ? k / PER_GROUP : 0;
+        constexpr int k = decltype(number)::value, j = k / PK, kk = k % PK, g = FP8 ? k / PER_GROUP : 0;
         const uint4 x = next;
         if (k + DV < NP) val[k % DV] = L.value(lds, tile, (k + DV) / PK, (k + DV) % PK);
         if (k + 1 < NP) next = operand(k + 1);
@@ -577,14 +595,17 @@ struct Kernel {
         o[j] = M::mul(x, make_uint4(w[0], w[1], w[2], w[3]), o[j]);
         if constexpr (FP8) {
           if (g + 1 < GROUPS) {
+            // a quad of the next group's weights, its scales read a product before
 #pragma unroll
-            for (int i = 0; i < PK * 4; ++i)
-              if (i * PER_GROUP / (PK * 4) == k % PER_GROUP) weights(tile, g + 1, i);
+            for (int q = 0; q < QUADS; ++q) {
+              if (q * PER_GROUP / QUADS == k % PER_GROUP) scales_of_weights(tile, g + 1, q);
+              if (q * PER_GROUP / QUADS + 1 == k % PER_GROUP) weights(g + 1, q);
+            }
           }
         }
         beside(k);
         __builtin_amdgcn_sched_barrier(0);
-      }
+      });
     };
     auto nothing = [](int) {};
 
@@ -619,12 +640,12 @@ struct Kernel {
           auto weigh = [&](int k) { s[k] = __builtin_amdgcn_exp2f(s[k] - m); };  // element k of step i's weights
           auto add = [&](int k) {
             l += s[k];
-            if (k & 1) weights(0, 0, k / 2);
+            if (k % 4 == 3) weights(0, k / 4);
           };
           if constexpr (MORE) {
             wait_copies<(AHEAD - 2) * COPIES>();
             tile_barrier();
-            Copies copies;
+            Copies copies(wave);
             scores(tile_of(i + 1), c, [&](int k) {
               if (k == 1) copies.find(a, src, first_token(i + AHEAD), wr, lane);
               if (k == 6) copies.address(a, wr, lane);
@@ -667,7 +688,7 @@ struct Kernel {
           if constexpr (WR > 1) tile_barrier();
           const uint32_t tile = tile_of(i);
           const int tb = first_token(i);
-          Copies copies;
+          Copies copies(wave);
           acc c[SUB];
           // (the 128-row kernel of an fp8 cache has no registers for it beside the scores)
           if constexpr (WR > 1 && MR == 32) {
@@ -675,10 +696,10 @@ struct Kernel {
             copies.emit_all(tile_of(i + AHEAD), wr, lane);
           }
           auto ahead = [&](int k) {
-            if constexpr (WR > 1 && MR == 16) {
+            if constexpr (MR == 16) {
               if (k == 1) copies.find(a, src, first_token(i + AHEAD), wr, lane);
               if (k == 6) copies.address(a, wr, lane);
-              copies.emit_at(k, NA, tile_of(i + AHEAD), wr, lane);
+              if constexpr (WR > 1) copies.emit_at(k, NA, tile_of(i + AHEAD), wr, lane);
             }
           };
           scores(tile, c, ahead);
@@ -694,16 +715,31 @@ struct Kernel {
             l += s[r];
           }
 #pragma unroll
-          for (int k = 0; k < PK * 4; ++k) weights(tile, 0, k);
+          for (int q = 0; q < QUADS; ++q) {
+            scales_of_weights(tile, 0, q);
+            weights(0, q);
+          }
+          const uint32_t into = tile_of(i + AHEAD);
           values(tile, [&](int k) {
             if constexpr (WR == 1) {
-              if (k == 1) copies.find(a, src, first_token(i + AHEAD), wr, lane);
-              if (k == 8) copies.address(a, wr, lane);
+              // A wave of its own refills what it has read: the rotary rows
+              // during the first block's products, each block of the latent rows
+              // during the next one's.
+              constexpr int SB = NP / BLOCKS;  // products of a block
+#pragma unroll
+              for (int r = 0; r < RR; ++r) {
+                if (r * SB / RR + (SB > RR ? 1 : 0) != k % SB) continue;
+                if (k < SB) copies.emit_rope(into, wr, r);
+                else copies.emit_latent(into, wr, r, k / SB - 1);
+              }
             }
           });
           if constexpr (WR == 1) {
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-            copies.emit_all(tile_of(i + AHEAD), wr, lane);
+#pragma unroll
+            for (int r = 0; r < RR; ++r) copies.emit_latent(into, wr, r, BLOCKS - 1);
+#pragma unroll
+            for (int r = 0; r < S_COPIES; ++r) copies.emit_scale(into, wr, lane, r);
           }
         }
       }
