@@ -285,7 +285,17 @@ struct Kernel {
       }
     };
     // element e of NR * 16: row u = e / 16, register e % 16
-    auto take = [&](int e) { s[e / 16][e % 16] = c[e / 16][e % 16]; };
+    // A score out of the accumulation registers. Inline asm: the compiler would
+    // keep the copy there too. It does not see the product that wrote the score
+    // (12 wait states, 48 clocks), so two later ones (32 clocks each) stand in
+    // between, or settle().
+    auto take = [&](int e) {
+      asm volatile("v_accvgpr_read_b32 %0, %1" : "=v"(s[e / 16][e % 16]) : "a"(c[e / 16][e % 16]));
+    };
+    auto settle = [&]() {
+#pragma unroll
+      for (int u = 0; u < NR; ++u) asm volatile("s_nop 15" : "+a"(c[u]));
+    };
     auto weigh = [&](int e) {
       const int u = e / 16, r = e % 16;
       s[u][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[u][r], a.scale_log2, nm[u]));
@@ -294,12 +304,13 @@ struct Kernel {
       const int u = e / 16, r = e % 16;
       if (r & 1) {
         l[u] += s[u][r - 1] + s[u][r];
+        asm volatile("" : "+v"(l[u]));  // here, beside the products: left alone, it sinks to the end of the step
         p[u][r / 2] = Elem<DT>::narrow2(s[u][r - 1], s[u][r]);
       }
     };
     float top[NR];
-    auto look = [&](int t0) {  // before the weights of the step at key t0: its mask and reference point
-      if (t0 + 32 > all_see) {
+    auto look = [&](int t0, auto masked) {  // before the weights of the step at key t0: its mask and reference point
+      if constexpr (decltype(masked)::value) {
 #pragma unroll
         for (int u = 0; u < NR; ++u) {
           top[u] = kNoMax;
@@ -343,7 +354,7 @@ struct Kernel {
     auto nothing = [](int) {};
     constexpr int E = NR * 16;
     // the step with a tile whose scores are in s; the next tile's scores are computed beside
-    auto step = [&](uint32_t tile, int t0, uint32_t next, auto more, auto copies) {
+    auto step = [&](uint32_t tile, int t0, uint32_t next, auto more, auto masked, auto copies) {
       if constexpr (decltype(more)::value) {
         scores(next, [&](int k) {
           copies(k);
@@ -358,7 +369,7 @@ struct Kernel {
 #pragma unroll
         for (int u = 0; u < NR; ++u) top[u] = kNoMax;
         values(tile, [&](int n) {
-          constexpr int FROM = 1, OVER = NP - 2;  // elements over products FROM .. FROM + OVER - 1
+          constexpr int FROM = NR == 1 ? 2 : 1, OVER = NP - 1 - FROM;  // elements over operands FROM .. FROM + OVER - 1
 #pragma unroll
           for (int e = 0; e < E; ++e)
             if (FROM + e * OVER / E == n) {
@@ -370,10 +381,7 @@ struct Kernel {
             for (int u = 0; u < NR; ++u) top[u] = row_max<32>(top[u]);
           }
         });
-        // in ordinary registers from here on, not in those of the products' sums
-#pragma unroll
-        for (int e = 0; e < E; ++e) asm volatile("" : "+v"(s[e / 16][e % 16]));
-        look(t0 + 32);
+        look(t0 + 32, masked);
       } else {
         first_values(tile);
 #pragma unroll
@@ -396,25 +404,35 @@ struct Kernel {
       wait_copies<(NB - 2) * COPIES>();
       tile_barrier();
       scores(0, nothing);
+      settle();
 #pragma unroll
       for (int e = 0; e < E; ++e) take(e);
       maxima();
-      look(0);
+      if (all_see < BN) look(0, std::true_type{});
+      else look(0, std::false_type{});
       uint32_t tile = 0, into = (NB - 1) * TILE;
-      for (int i = 0; i + 1 < tiles; ++i) {
-        // The next tile has arrived for all waves, and all have left the one
-        // before this: a tile further on takes its place.
-        wait_copies<(NB - 3) * COPIES>();
-        tile_barrier();
-        const uint32_t next = tile + TILE < NB * TILE ? tile + TILE : 0;
-        step(tile, i * BN, next, std::true_type{}, [&](int k) {
-          if (k == 1) copies.address(kn, kr, kv, a, (i + NB - 1) * BN, t.kn - 1, wave, lane);
-          copies.emit_at(k, into, wave);
-        });
-        into = tile;
-        tile = next;
-      }
-      step(tile, (tiles - 1) * BN, 0, std::false_type{}, nothing);
+      int i = 0;
+      auto walk = [&](int to, auto masked) {  // up to step `to`, whose scores then wait in s
+        for (; i < to; ++i) {
+          // The next tile has arrived for all waves, and all have left the one
+          // before this: a tile further on takes its place.
+          wait_copies<(NB - 3) * COPIES>();
+          tile_barrier();
+          const uint32_t next = tile + TILE < NB * TILE ? tile + TILE : 0;
+          step(tile, i * BN, next, std::true_type{}, masked, [&](int k) {
+            if (k == 1) copies.address(kn, kr, kv, a, (i + NB - 1) * BN, t.kn - 1, wave, lane);
+            copies.emit_at(k, into, wave);
+          });
+          into = tile;
+          tile = next;
+        }
+      };
+      // Steps that some row of the wave does not see all of come last. Masking
+      // in a branch of one loop would cost every step copies of its scores.
+      const int whole = all_see / BN - 1;
+      walk(whole < tiles - 1 ? whole : tiles - 1, std::false_type{});
+      walk(tiles - 1, std::true_type{});
+      step(tile, i * BN, 0, std::false_type{}, std::false_type{}, nothing);
       wait_copies<0>();
     }
 
