@@ -126,7 +126,6 @@ struct Kernel {
     int* wave_total = reinterpret_cast<int*>(lds + BODY);
     int* found = wave_total + NT / 64;
     const int tid = threadIdx.x, lane = tid % 64, wave = __builtin_amdgcn_readfirstlane(tid / 64);
-    const int h = lane / 32, ln = lane % 32;
     // Workgroups go round the eight XCDs: each gets a run of neighbouring heads,
     // one head's tiles after the other's, so that its L2 holds the keys in use
     // and they lie in all of its channels.
@@ -166,6 +165,15 @@ struct Kernel {
     if (found[0] < 0) return;
     const Tile t = sequence(a, found[0]);
     const int row0 = found[1] * BM;
+    // a tile of at most 128 rows, the rest of a sequence, goes to all four waves too
+    if (NR == 2 && t.qn - row0 <= 128) Kernel<DT, DN, DR, DV, 1>::rows(a, lds, t, row0, head);
+    else rows(a, lds, t, row0, head);
+  }
+
+  // rows row0 .. of a sequence's queries
+  static PCAMD_DEV void rows(const Args& a, uint8_t* lds, const Tile& t, int row0, int head) {
+    const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const int h = lane / 32, ln = lane % 32;
     const int past = t.kn - t.qn;
 
     // ---- queries: whole lines into LDS, a lane's row from there
@@ -212,6 +220,12 @@ struct Kernel {
     int keys = a.causal ? end + past : t.kn;
     if (keys > t.kn) keys = t.kn;
     const int tiles = keys > 0 ? (keys + BN - 1) / BN : 0;
+    // The wave's own steps: up to the last key that one of its rows sees, none
+    // if it has no rows. It waits out the others' steps.
+    const int mine0 = row0 + wave * QROWS, mine1 = mine0 + QROWS < t.qn ? mine0 + QROWS : t.qn;
+    int seen = mine1 <= mine0 ? 0 : a.causal ? mine1 + past : t.kn;
+    if (seen > t.kn) seen = t.kn;
+    const int steps = seen > 0 ? (seen + BN - 1) / BN : 0;
     const uint8_t* kn = static_cast<const uint8_t*>(a.k) + t.k0 * a.skt + 2 * head * a.skh;
     const uint8_t* kr = static_cast<const uint8_t*>(a.kr) + t.k0 * a.srt;
     const uint8_t* kv = static_cast<const uint8_t*>(a.v) + t.k0 * a.svt + 2 * head * a.svh;
@@ -244,8 +258,8 @@ struct Kernel {
       const uint2 z = read_tr4(lds + ((tile + lane_v) ^ (x ^ 16)) + at + 8 * 128);
       return make_uint4(y.x, y.y, z.x, z.y);
     };
-    constexpr int DA = KS < 5 ? KS : 5;                      // key operands read ahead
-    constexpr int NP = 2 * OB, DVA = NP < 4 ? NP : 4;        // value operands (contraction step n / OB, block n % OB), ahead
+    constexpr int DA = KS < 8 ? KS : 8;                      // key operands read ahead
+    constexpr int NP = 2 * OB, DVA = NP < 6 ? NP : 6;        // value operands (contraction step n / OB, block n % OB), ahead
     uint4 val[DVA];
     f32x16 c[NR];
     float s[NR][16];
@@ -403,22 +417,18 @@ struct Kernel {
       }
       wait_copies<(NB - 2) * COPIES>();
       tile_barrier();
-      scores(0, nothing);
-      settle();
-#pragma unroll
-      for (int e = 0; e < E; ++e) take(e);
-      maxima();
-      if (all_see < BN) look(0, std::true_type{});
-      else look(0, std::false_type{});
       uint32_t tile = 0, into = (NB - 1) * TILE;
       int i = 0;
+      auto turn = [&]() {
+        // The next tile has arrived for all waves, and all have left the one
+        // before this: a tile further on takes its place.
+        wait_copies<(NB - 3) * COPIES>();
+        tile_barrier();
+        return tile + TILE < NB * TILE ? tile + TILE : 0;
+      };
       auto walk = [&](int to, auto masked) {  // up to step `to`, whose scores then wait in s
         for (; i < to; ++i) {
-          // The next tile has arrived for all waves, and all have left the one
-          // before this: a tile further on takes its place.
-          wait_copies<(NB - 3) * COPIES>();
-          tile_barrier();
-          const uint32_t next = tile + TILE < NB * TILE ? tile + TILE : 0;
+          const uint32_t next = turn();
           step(tile, i * BN, next, std::true_type{}, masked, [&](int k) {
             if (k == 1) copies.address(kn, kr, kv, a, (i + NB - 1) * BN, t.kn - 1, wave, lane);
             copies.emit_at(k, into, wave);
@@ -427,12 +437,28 @@ struct Kernel {
           tile = next;
         }
       };
-      // Steps that some row of the wave does not see all of come last. Masking
-      // in a branch of one loop would cost every step copies of its scores.
-      const int whole = all_see / BN - 1;
-      walk(whole < tiles - 1 ? whole : tiles - 1, std::false_type{});
-      walk(tiles - 1, std::true_type{});
-      step(tile, i * BN, 0, std::false_type{}, std::false_type{}, nothing);
+      if (steps > 0) {
+        scores(0, nothing);
+        settle();
+#pragma unroll
+        for (int e = 0; e < E; ++e) take(e);
+        maxima();
+        if (all_see < BN) look(0, std::true_type{});
+        else look(0, std::false_type{});
+        // Steps that some row of the wave does not see all of come last. Masking
+        // in a branch of one loop would cost every step copies of its scores.
+        const int whole = all_see / BN - 1;
+        walk(whole < steps - 1 ? whole : steps - 1, std::false_type{});
+        walk(steps - 1, std::true_type{});
+        step(tile, i * BN, 0, std::false_type{}, std::false_type{}, nothing);
+      }
+      for (; i + 1 < tiles; ++i) {
+        const uint32_t next = turn();
+        copies.address(kn, kr, kv, a, (i + NB - 1) * BN, t.kn - 1, wave, lane);
+        copies.emit_all(into, wave);
+        into = tile;
+        tile = next;
+      }
       wait_copies<0>();
     }
 
