@@ -39,7 +39,7 @@ struct Args {
 };
 
 struct Tile {
-  int64_t q0, k0;  // first token of the sequence's queries and keys
+  int64_t q0, k0;  // first token of the sequence's queries and keys (below 2^31)
   int qn, kn;
 };
 
@@ -77,11 +77,13 @@ struct Kernel {
   static constexpr int KB = DN / 64, VB = DV / 64, CR = DR / 8;
   static constexpr int BLOCK = BN * 128, VALUES = (KB + 1) * BLOCK, TILE = (KB + 1 + VB) * BLOCK;
   static constexpr int NB = 6;  // tiles: the one in use, the next, and four on their way
-  // in the ring's place: queries [block][row][128 bytes] first, output rows last
+  // In the ring's place: queries [block][row][128 bytes] first, behind the tiles
+  // that are copied meanwhile; output rows last
   static constexpr int QROWS = NR * 32, QBLOCK = QROWS * 128, QUERIES = (KB + 1) * QBLOCK;
+  static constexpr int EARLY = 2, QAT = EARLY * TILE;
   static constexpr int OPITCH = DV * 2 + 16, OUT = QROWS * OPITCH;
   static constexpr int max3(int a, int b, int c) { return a > b ? (a > c ? a : c) : (b > c ? b : c); }
-  static constexpr int BODY = max3(NB * TILE, 4 * QUERIES, 4 * OUT);
+  static constexpr int BODY = max3(NB * TILE, QAT + 4 * QUERIES, 4 * OUT);
   static constexpr int LDS = BODY + 64;
   static constexpr int COPIES = KB + 1 + VB;  // of a wave for a tile: 8 keys x 128 bytes each
 
@@ -133,38 +135,62 @@ struct Kernel {
     const int head = item / a.max_tiles, want = item - head * a.max_tiles;
     if (head >= a.heads) return;
 
-    // ---- the tile's sequence: a running count of tiles over the sequences
-    if (tid == 0) found[0] = -1;
-    int base = 0;
-    for (int i0 = 0; i0 <= a.sequences; i0 += NT) {
-      const int i = i0 + tid;
-      const int mine = i <= a.sequences ? (sequence(a, i).qn + BM - 1) / BM : 0;
+    // ---- the tile's sequence, found in a running count of tiles over the
+    // sequences, and its tile, the longest rows of a causal sequence first
+    Tile t;
+    int row0;
+    if (a.sequences < 64) {
+      // a sequence a lane; every wave finds it by itself
+      const Tile own = sequence(a, lane <= a.sequences ? lane : a.sequences);
+      const int mine = lane <= a.sequences ? (own.qn + BM - 1) / BM : 0;
       int inc = mine;
 #pragma unroll
       for (int d = 1; d < 64; d <<= 1) {
         const int o = __shfl_up(inc, d, 64);
         if (lane >= d) inc += o;
       }
-      __syncthreads();
-      if (lane == 63) wave_total[wave] = inc;
-      __syncthreads();
-      int before = base + inc - mine, total = 0;
+      const uint64_t here = __ballot(want >= inc - mine && want < inc);
+      if (!here) return;
+      const int from = __builtin_ctzll(here);
+      auto of = [&](int x) { return __builtin_amdgcn_readlane(x, from); };
+      t.q0 = of(static_cast<int>(own.q0));
+      t.k0 = of(static_cast<int>(own.k0));
+      t.qn = of(own.qn);
+      t.kn = of(own.kn);
+      row0 = (of(inc) - 1 - want) * BM;
+    } else {
+      if (tid == 0) found[0] = -1;
+      int base = 0;
+      for (int i0 = 0; i0 <= a.sequences; i0 += NT) {
+        const int i = i0 + tid;
+        const int mine = i <= a.sequences ? (sequence(a, i).qn + BM - 1) / BM : 0;
+        int inc = mine;
 #pragma unroll
-      for (int w = 0; w < NT / 64; ++w) {
-        if (w < wave) before += wave_total[w];
-        total += wave_total[w];
+        for (int d = 1; d < 64; d <<= 1) {
+          const int o = __shfl_up(inc, d, 64);
+          if (lane >= d) inc += o;
+        }
+        __syncthreads();
+        if (lane == 63) wave_total[wave] = inc;
+        __syncthreads();
+        int before = base + inc - mine, total = 0;
+#pragma unroll
+        for (int w = 0; w < NT / 64; ++w) {
+          if (w < wave) before += wave_total[w];
+          total += wave_total[w];
+        }
+        if (want >= before && want < before + mine) {
+          found[0] = i;
+          found[1] = mine - 1 - (want - before);
+        }
+        base += total;
+        __syncthreads();
+        if (found[0] >= 0) break;
       }
-      if (want >= before && want < before + mine) {
-        found[0] = i;
-        found[1] = mine - 1 - (want - before);  // the longest rows of a causal sequence first
-      }
-      base += total;
-      __syncthreads();
-      if (found[0] >= 0) break;
+      if (found[0] < 0) return;
+      t = sequence(a, found[0]);
+      row0 = found[1] * BM;
     }
-    if (found[0] < 0) return;
-    const Tile t = sequence(a, found[0]);
-    const int row0 = found[1] * BM;
     // a tile of at most 128 rows, the rest of a sequence, goes to all four waves too
     if (NR == 2 && t.qn - row0 <= 128) Kernel<DT, DN, DR, DV, 1>::rows(a, lds, t, row0, head);
     else rows(a, lds, t, row0, head);
@@ -184,19 +210,37 @@ struct Kernel {
       int row = row0 + wave * QROWS + r;
       if (row >= t.qn) row = t.qn - 1;  // a spare row computes what another one does, and is not stored
       const uint8_t* p = qp + 2 * row * a.sqt + 16 * c;
-      const uint32_t to = wave * QUERIES + 8 * i * 128;
+      const uint32_t to = QAT + wave * QUERIES + 8 * i * 128;
 #pragma unroll
       for (int b = 0; b < KB; ++b) copy16(p + b * 128, to + b * QBLOCK);
       if (c < CR) copy16(p + DN * 2, to + KB * QBLOCK);
     }
-    wait_copies<0>();
+    // ---- the first tiles' copies, behind the queries'
+    const uint8_t* kn = static_cast<const uint8_t*>(a.k) + t.k0 * a.skt + 2 * head * a.skh;
+    const uint8_t* kr = static_cast<const uint8_t*>(a.kr) + t.k0 * a.srt;
+    const uint8_t* kv = static_cast<const uint8_t*>(a.v) + t.k0 * a.svt + 2 * head * a.svh;
+    const int end = row0 + BM < t.qn ? row0 + BM : t.qn;  // of the tile's rows
+    int keys = a.causal ? end + past : t.kn;              // that they see
+    if (keys > t.kn) keys = t.kn;
+    const int tiles = keys > 0 ? (keys + BN - 1) / BN : 0;
+    Copies copies;
+    if (tiles > 0) {
+#pragma unroll
+      for (int i = 0; i < EARLY; ++i) {
+        copies.address(kn, kr, kv, a, i * BN, t.kn - 1, wave, lane);
+        copies.emit_all(i * TILE, wave);
+      }
+      wait_copies<EARLY * COPIES>();
+    } else {
+      wait_copies<0>();
+    }
     uint4 q[NR][KS];
 #pragma unroll
     for (int u = 0; u < NR; ++u)
 #pragma unroll
       for (int k = 0; k < KS; ++k) {
         const int c = 2 * k < DN / 8 ? 2 * k : 2 * k - DN / 8, b = 2 * k < DN / 8 ? c / 8 : KB;
-        uint4 x = *reinterpret_cast<const uint4*>(lds + wave * QUERIES + b * QBLOCK + (u * 32 + ln) * 128 +
+        uint4 x = *reinterpret_cast<const uint4*>(lds + QAT + wave * QUERIES + b * QBLOCK + (u * 32 + ln) * 128 +
                                                   (((c % 8 + h) ^ swizzle16(ln)) << 4));
         x.x ^= a.negate; x.y ^= a.negate; x.z ^= a.negate; x.w ^= a.negate;
         q[u][k] = x;
@@ -216,20 +260,12 @@ struct Kernel {
     }
     const int first = row0 + wave * QROWS + past + 1;
     const int all_see = a.causal && first < t.kn ? first : t.kn;  // keys that every row of the wave sees
-    const int end = row0 + BM < t.qn ? row0 + BM : t.qn;          // of the tile's rows
-    int keys = a.causal ? end + past : t.kn;
-    if (keys > t.kn) keys = t.kn;
-    const int tiles = keys > 0 ? (keys + BN - 1) / BN : 0;
     // The wave's own steps: up to the last key that one of its rows sees, none
     // if it has no rows. It waits out the others' steps.
     const int mine0 = row0 + wave * QROWS, mine1 = mine0 + QROWS < t.qn ? mine0 + QROWS : t.qn;
     int seen = mine1 <= mine0 ? 0 : a.causal ? mine1 + past : t.kn;
     if (seen > t.kn) seen = t.kn;
     const int steps = seen > 0 ? (seen + BN - 1) / BN : 0;
-    const uint8_t* kn = static_cast<const uint8_t*>(a.k) + t.k0 * a.skt + 2 * head * a.skh;
-    const uint8_t* kr = static_cast<const uint8_t*>(a.kr) + t.k0 * a.srt;
-    const uint8_t* kv = static_cast<const uint8_t*>(a.v) + t.k0 * a.svt + 2 * head * a.svh;
-
     f32x16 o[NR][OB];
     float m[NR], nm[NR], l[NR];  // reference point (in units of s), minus its log2, sum of weights
 #pragma unroll
@@ -409,9 +445,8 @@ struct Kernel {
     };
 
     if (tiles > 0) {
-      Copies copies;
 #pragma unroll
-      for (int i = 0; i < NB - 1; ++i) {
+      for (int i = EARLY; i < NB - 1; ++i) {
         copies.address(kn, kr, kv, a, i * BN, t.kn - 1, wave, lane);
         copies.emit_all(i * TILE, wave);
       }
