@@ -104,6 +104,16 @@ PCAMD_DEV float amax8(const float (&y)[8]) {
   return m;
 }
 
+// Scales of a group of y = t * inv, t = r * w: as block_scales of y, with inv
+// left out of the codes' factor where y's largest value sets it, so that codes
+// come of two roundings less. (inf * 0, of a row with an infinity, takes the
+// floor: its other values are zeros.)
+PCAMD_DEV Scales normed_scales(float amax_t, float inv, float fp8_max, float eps) {
+  const bool above = amax_t * inv >= eps;
+  const float qs = fp8_max / (above ? amax_t : eps);
+  return above ? Scales{qs, inv / qs} : Scales{qs * inv, 1.0f / qs};
+}
+
 // fp8 of clamp(y * qs); a NaN stays one (the clamp alone would make it -fp8_max)
 template <int FMT>
 PCAMD_DEV uint2 codes8(const float (&y)[8], float qs, float fp8_max) {
@@ -202,8 +212,8 @@ __global__ __launch_bounds__(TEAM < 256 ? 256 : TEAM) void norm_quant_kernel(Nor
       float w[8];
       load8_as(a.w_dtype, a.weight, 8 * c, valid, w);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] = y[i] * inv * w[i];
-      const Scales sc = block_scales(group_max<16>(amax8(y)), a.fp8_max, a.eps);
+      for (int i = 0; i < 8; ++i) y[i] *= w[i];
+      const Scales sc = normed_scales(group_max<16>(amax8(y)), inv, a.fp8_max, a.eps);
       if (!live || valid <= 0) return;
       if (lane % 16 == 0) a.scale[b * a.ssb + r * a.ssm + c / 16] = sc.ds;
       store_codes(a.y + b * a.syb + r * a.sym + 8 * c, valid, codes8<FMT>(y, sc.qs, a.fp8_max));
@@ -242,23 +252,26 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
     const int64_t valid = a.dl - 8 * lane;  // >= 8 or <= 0
     float v[8];
     load8<DT>(a.latent, t * a.slt + 8 * lane, valid > 0 ? valid : 0, v);
+    float inv = 1.0f;
     if (a.weight) {
       float s = 0.0f;
 #pragma unroll
       for (int i = 0; i < 8; ++i) s += v[i] * v[i];
-      const float inv = rsqrtf(wave_sum(s) / static_cast<float>(a.dl) + a.norm_eps);
+      inv = rsqrtf(wave_sum(s) / static_cast<float>(a.dl) + a.norm_eps);
       float w[8];
       load8_as(a.w_dtype, a.weight, 8 * lane, valid > 0 ? valid : 0, w);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = v[i] * inv * w[i];
+      for (int i = 0; i < 8; ++i) v[i] *= w[i];
     }
     if constexpr (FP8) {
-      const Scales sc = block_scales(group_max<16>(amax8(v)), fmt_max<kE4M3>(), a.eps);
+      const Scales sc = normed_scales(group_max<16>(amax8(v)), inv, fmt_max<kE4M3>(), a.eps);
       if (valid > 0) {
         if (lane % 16 == 0) a.c_scale[page * a.csp + at * a.cst + lane / 16] = sc.ds;
         store_codes(a.c_latent + page * a.clp + at * a.clt + 8 * lane, 8, codes8<kE4M3>(v, sc.qs, fmt_max<kE4M3>()));
       }
     } else if (valid > 0) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] *= inv;
       store8<DT>(a.c_latent, page * a.clp + at * a.clt + 8 * lane, 8, v);
     }
     for (int c = lane; 8 * c < a.dr; c += 64) {
