@@ -7,7 +7,8 @@ Public API (drop-in for xuOAO/practice_cuda's fp8_training/fp8_bench):
 * quantizers: per_block_quant, per_channel_quant, per_tensor_quant
 * BMMs: per_block_bmm, per_channel_bmm, per_tensor_bmm
 * latent attention in 8 bits (serving): rms_norm_quant, LatentCache,
-  latent_append, latent_decode, latent_prefill
+  latent_append, latent_decode, latent_prefill; latent_layer.LatentAttention
+  runs them as one layer
 
 The kernels live in the in-tree HIP library built by
 ``python -m practice_cuda_amd.build``; every entry point raises if it is

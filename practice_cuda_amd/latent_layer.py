@@ -1,0 +1,134 @@
+"""A latent-attention layer served in fp8: the package's operators in their order of use.
+
+One token's keys and values come from one latent vector; only that and a shared
+rotary key are kept. ``LatentAttention`` runs
+
+    x + residual -> rms_norm_quant -> query and latent projections (block-scaled
+    products) -> rotary positions -> latent_append into the paged cache
+
+and then, for prompts (``prefill``), expands keys and values and attends with
+``latent_prefill``, or, for new tokens (``decode``), moves the queries into the
+latent space with a head-batched block-scaled product, attends over the cache
+with ``latent_decode`` and applies the value maps the same way. Weights are
+quantized once, in 128 x 128 blocks; activations in 1 x 128 groups.
+
+The head-batched products are those of the reference's BMM benchmarks
+(fp8_training/fp8_bench, kernels/fp8_bmm); the layer around them has no
+counterpart there.
+"""
+from __future__ import annotations
+
+import math
+
+import torch
+import torch.nn as nn
+
+from .impls.hip_latent import LatentCache, hip_latent_append, hip_latent_decode, hip_latent_prefill
+from .impls.hip_per_block import hip_per_block_quant
+from .impls.hip_rms_norm import hip_rms_norm_quant
+from .modules import _block_scaled_bmm
+from .registry import QuantResult
+
+
+def _quant(x: torch.Tensor, block_m: int = 1) -> QuantResult:
+    return hip_per_block_quant(x, block_m=block_m, block_n=128, cache_outputs=True)
+
+
+def _product(a: QuantResult, w: QuantResult) -> torch.Tensor:
+    """``a @ w^T`` per batch: a [B, M, K] in 1 x 128 groups, w [B, N, K] in 128 x 128 blocks."""
+    return _block_scaled_bmm(a.tensor, a.dequant_scale, w.tensor.transpose(1, 2), w.dequant_scale.transpose(1, 2),
+                             None, 1, 128, 128, torch.bfloat16)
+
+
+class LatentAttention(nn.Module):
+    """hidden -> heads x (head_dim + rope_dim) queries, one latent_dim + rope_dim vector a token.
+
+    Widths as the attention kernels take them: latent 512, rotary 64, head 128,
+    or 256, 32 and 64. Inputs are bfloat16 [tokens, hidden]; both calls return
+    (the layer's output, the residual to add to it)."""
+
+    def __init__(self, hidden: int, heads: int, *, latent_dim: int = 512, rope_dim: int = 64, head_dim: int = 128,
+                 norm_eps: float = 1e-6, rope_base: float = 10000.0, device=None) -> None:
+        super().__init__()
+        self.hidden, self.heads = hidden, heads
+        self.latent_dim, self.rope_dim, self.head_dim = latent_dim, rope_dim, head_dim
+        self.norm_eps = norm_eps
+        self.softmax_scale = 1.0 / math.sqrt(head_dim + rope_dim)
+
+        def weight(*shape):
+            w = torch.empty(shape, dtype=torch.bfloat16, device=device)
+            return nn.Parameter(nn.init.normal_(w, std=shape[-1] ** -0.5), requires_grad=False)
+
+        kw = {"dtype": torch.bfloat16, "device": device}
+        self.norm = nn.Parameter(torch.ones(hidden, **kw), requires_grad=False)
+        self.latent_norm = nn.Parameter(torch.ones(latent_dim, **kw), requires_grad=False)
+        self.w_query = weight(1, heads * (head_dim + rope_dim), hidden)
+        self.w_latent = weight(1, latent_dim + rope_dim, hidden)
+        self.w_key = weight(heads, head_dim, latent_dim)    # key of head h: w_key[h] c
+        self.w_value = weight(heads, head_dim, latent_dim)  # value: w_value[h] c
+        self.w_out = weight(1, hidden, heads * head_dim)
+        freq = rope_base ** (-torch.arange(0, rope_dim, 2, device=device).float() / rope_dim)
+        self.register_buffer("freq", freq, persistent=False)
+        self._fp8 = None
+
+    def quantize(self) -> "LatentAttention":
+        """The weights' fp8 forms, once: call again after changing a weight."""
+        both = torch.cat([self.w_key, self.w_value], 1).reshape(1, -1, self.latent_dim)
+        self._fp8 = {
+            "query": _quant(self.w_query, 128), "latent": _quant(self.w_latent, 128),
+            "key_value": _quant(both, 128),  # [1, H * 2 head, latent], head after head
+            "absorb": _quant(self.w_key.transpose(1, 2).contiguous(), 128),  # [H, latent, head]
+            "value": _quant(self.w_value, 128), "out": _quant(self.w_out, 128),
+        }
+        return self
+
+    def _rotate(self, x: torch.Tensor, positions: torch.Tensor) -> torch.Tensor:
+        """Rotary positions over the halves of the last dimension; x [T, .., rope]."""
+        angle = positions.float()[:, None] * self.freq
+        shape = (x.shape[0],) + (1,) * (x.ndim - 2) + (-1,)
+        cos, sin = angle.cos().view(shape), angle.sin().view(shape)
+        a, b = x.float().chunk(2, -1)
+        return torch.cat([a * cos - b * sin, a * sin + b * cos], -1).to(x.dtype)
+
+    def _project(self, x, residual, cache, slots, positions):
+        """(queries [T, H, head + rope], latents, rotary keys, residual); the tokens are in the cache."""
+        if self._fp8 is None:
+            self.quantize()
+        normed, residual = hip_rms_norm_quant(x[None], self.norm, residual=residual[None], norm_eps=self.norm_eps)
+        q = _product(normed, self._fp8["query"])[0].view(-1, self.heads, self.head_dim + self.rope_dim)
+        both = _product(normed, self._fp8["latent"])[0]
+        latent, rope = both[:, :self.latent_dim], self._rotate(both[:, self.latent_dim:], positions)
+        q[..., self.head_dim:] = self._rotate(q[..., self.head_dim:], positions)
+        hip_latent_append(cache, latent, rope, slots, weight=self.latent_norm, norm_eps=self.norm_eps)
+        return q, latent, rope, residual[0]
+
+    def _output(self, o: torch.Tensor) -> torch.Tensor:  # [T, H, head]
+        return _product(_quant(o.reshape(1, o.shape[0], -1)), self._fp8["out"])[0]
+
+    def prefill(self, x, residual, cache: LatentCache, slots, positions, cu_seqlens):
+        """Whole prompts, packed: sequence i holds tokens cu_seqlens[i] .. cu_seqlens[i + 1] - 1 (int32)."""
+        q, latent, rope, residual = self._project(x, residual, cache, slots, positions)
+        c, _ = hip_rms_norm_quant(latent[None], self.latent_norm, norm_eps=self.norm_eps)
+        both = _product(c, self._fp8["key_value"])[0].view(-1, self.heads, 2 * self.head_dim)
+        o = hip_latent_prefill(q, both[..., :self.head_dim], rope, both[..., self.head_dim:], cu_seqlens, cu_seqlens,
+                               softmax_scale=self.softmax_scale)
+        return self._output(o), residual
+
+    def decode(self, x, residual, cache: LatentCache, slots, positions, block_table, seq_lens):
+        """New tokens, [B * S, hidden] for B = seq_lens.numel() sequences of S each; seq_lens counts them."""
+        batch, heads = seq_lens.shape[0], self.heads
+        q, _, _, residual = self._project(x, residual, cache, slots, positions)
+        tokens = q.shape[0]
+        nope = _quant(q[..., :self.head_dim].transpose(0, 1).contiguous())  # [H, T, head]
+        q_latent = _product(nope, self._fp8["absorb"])                      # [H, T, latent]
+        shape = (heads, batch, tokens // batch, self.latent_dim)
+        o = torch.empty_like(q_latent)
+        hip_latent_decode(q_latent.view(shape).permute(1, 2, 0, 3),
+                          q[..., self.head_dim:].view(batch, tokens // batch, heads, self.rope_dim), cache,
+                          block_table, seq_lens, softmax_scale=self.softmax_scale,
+                          out=o.view(shape).permute(1, 2, 0, 3))
+        values = _product(_quant(o), self._fp8["value"])                    # [H, T, head]
+        return self._output(values.transpose(0, 1)), residual
+
+
+__all__ = ["LatentAttention"]
