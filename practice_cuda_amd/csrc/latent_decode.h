@@ -42,8 +42,9 @@ constexpr int kAheadValues = 6;
 // The division of the work. One list of units: for each sequence, for each tile
 // of its rows, kFixed units for what a piece costs whatever its length (its
 // queries, its output) and one for each step over the tokens. Workgroup w takes
-// the w-th of `groups` equal pieces of the list, whatever the lengths are; what
-// more than one of them has worked on, combine_kernel joins.
+// the w-th of `groups` equal pieces of the list, whatever the lengths are (with
+// SPLIT, workgroups SPLIT w and on take its rows); what more than one piece has
+// a part of, combine_kernel joins.
 // ---------------------------------------------------------------------------
 struct Division {
   int units, groups, q, r;
@@ -80,11 +81,11 @@ PCAMD_DEV int block_scan(int v, int* wave_total, int& total) {
   return before + inc - v;
 }
 
-template <int DT, bool FP8, int DL, int DR, int MR, int WR>
+template <int DT, bool FP8, int DL, int DR, int MR, int WR, int SPLIT>
 struct Kernel {
   static constexpr int WT = 4 / WR;
   static constexpr int STEP = TOK * WT;
-  static constexpr int ROWS = MR * WR;
+  static constexpr int ROWS = MR * WR, TILE_ROWS = ROWS * SPLIT;
   static constexpr int GROUPS = DL / 128;
   typedef Mfma<DT, MR> M;
   typedef ScoreMfma<DT, MR> S;
@@ -108,15 +109,16 @@ struct Kernel {
   static constexpr int NB = FIT > 4 ? 4 : FIT;
   static_assert(NB >= (WR > 1 ? 2 : 1), "a shared ring needs two tiles");
   static constexpr int AHEAD = WR > 1 ? NB - 1 : NB;  // tiles on their way or in use
-  // The 128-row kernel of a 16-bit cache overlaps one tile's softmax with the
-  // next one's scores; it has the registers for it.
-  static constexpr bool PIPE = MR == 32 && !FP8;
+  // With 128 rows a workgroup and a 16-bit cache one tile's softmax overlaps the
+  // next one's scores.
+  static constexpr bool PIPE = MR == 32 && WR == 4 && !FP8;
   static_assert(!PIPE || NB == 4, "the overlapped loop holds two tiles while two more are on their way");
   static constexpr int PAGES = 256;  // page numbers kept in LDS
   static constexpr int RING = WT * NB * TILE;
-  // epilogue, in the ring's place: the rows of EW waves at a time. Whole rows,
+  // epilogue, in the ring's place: the rows of EW waves at a time, those that
+  // share rows among them. Whole rows,
   // because half rows of all of them would keep half of the memory channels idle.
-  static constexpr int EW = MR == 32 && DL > 256 ? 2 : 4;
+  static constexpr int EW = MR == 32 && DL > 256 ? 2 : 4, EWR = EW / WT;
   static constexpr int PITCH = DL + 4;
   static constexpr int EPI = EW * MR * PITCH * 4 + 4 * MR * 8 + ROWS * 8;
   // prologue, there too: each wave's query rows, [block][row][128 bytes]
@@ -296,15 +298,18 @@ struct Kernel {
     int groups = wanted > tiles ? wanted : tiles;
     if (groups > a.groups) groups = a.groups;
     // with few tiles every workgroup has one piece of one: nothing to weigh
-    const int FIXED = tiles > 1 && tiles * 16 >= groups ? kFixed<MR> : 0;
+    const int FIXED = tiles > 1 && tiles * 16 >= groups ? kFixed<MR, SPLIT> : 0;
     const Division div(a.row_tiles * (steps_all + a.batch * FIXED), groups);
-    if (static_cast<int>(blockIdx.x) >= groups) {
-      if (a.parts && tid == 0) a.joins[blockIdx.x] = make_int4(0, 0, -1, 0);
+    const int wgs = groups * SPLIT;
+    if (static_cast<int>(blockIdx.x) >= wgs) {
+      if (a.parts && tid == 0) a.joins[blockIdx.x / SPLIT] = make_int4(0, 0, -1, 0);
       return;
     }
-    // Neighbouring pieces belong to the same sequence: put them on the same XCD
-    // (workgroups go round the eight of them), whose L2 then holds its queries.
-    const int w = groups % 8 ? blockIdx.x : blockIdx.x % 8 * (groups / 8) + blockIdx.x / 8;
+    // Neighbouring pieces belong to the same sequence, and a piece's workgroups
+    // read the same tokens at the same time: put them on the same XCD (workgroups
+    // go round the eight of them), whose L2 then holds its queries and the tokens.
+    const int place = wgs % 8 ? blockIdx.x : blockIdx.x % 8 * (wgs / 8) + blockIdx.x / 8;
+    const int w = place / SPLIT, share = place % SPLIT * ROWS;  // its first row of the tile
     const int begin = div.first(w), end = div.first(w + 1);
     int base = 0;
     for (int b0 = 0; b0 < a.batch; b0 += NT) {
@@ -325,7 +330,7 @@ struct Kernel {
     }
     __syncthreads();
     int b = found[0], in_seq = found[1];
-    if (a.parts && tid == 0) {
+    if (a.parts && tid == 0 && share == 0) {
       // Where pieces meet: the first workgroup that starts inside a (sequence,
       // row tile) notes which it is and which workgroup holds the last piece;
       // the one before it holds the first.
@@ -342,7 +347,8 @@ struct Kernel {
       const int rt = in_seq / tile, at = in_seq - rt * tile;
       const int n = end - u < tile - at ? end - u : tile - at;
       const int s0 = at > FIXED ? at - FIXED : 0, s1 = at + n - FIXED;
-      if (s1 > s0) segment(a, lds, b, rt, s0, s1 - s0, steps, len, s0 > 0 ? 2 * w : 2 * w + 1);
+      const int row0 = rt * TILE_ROWS + share;
+      if (s1 > s0 && row0 < a.rows) segment(a, lds, b, row0, share, s0, s1 - s0, steps, len, s0 > 0 ? 2 * w : 2 * w + 1);
       u += n;
       in_seq += n;
       if (in_seq >= tile * a.row_tiles) {
@@ -353,13 +359,13 @@ struct Kernel {
   }
 
   // Steps s0 .. s0 + n - 1 of a row tile's `steps`.
-  static PCAMD_DEV void segment(const Args& a, uint8_t* lds, int b, int rt, int s0, int n, int steps, int len,
-                                int slot) {
+  static PCAMD_DEV void segment(const Args& a, uint8_t* lds, int b, int row0, int share, int s0, int n, int steps,
+                                int len, int slot) {
     const int tid = threadIdx.x, lane = tid % 64, wave = __builtin_amdgcn_readfirstlane(tid / 64);
     const int wr = wave % WR, wt = wave / WR;
     const Lane L(lane);
     const int h = L.h, ln = L.ln;
-    const int row = rt * ROWS + wr * MR + ln;  // this lane's row
+    const int row = row0 + wr * MR + ln;  // this lane's row
     const bool live = row < a.rows;
     const int tok_new = live ? row / a.heads : 0, head = live ? row % a.heads : 0;
 
@@ -389,7 +395,7 @@ struct Kernel {
 #pragma unroll
       for (int i = 0; i < MR / 8; ++i) {
         const int r = 8 * i + lane / 8, c = (lane % 8) ^ swizzle16(r);
-        int from = rt * ROWS + wr * MR + r;
+        int from = row0 + wr * MR + r;
         if (from >= a.rows) from = a.rows - 1;  // a spare row computes what another one does, and is not stored
         const int tn = from / a.heads, hd = from - tn * a.heads;
         const uint16_t* p = static_cast<const uint16_t*>(a.q_latent) + b * a.qlb + tn * a.qls + hd * a.qlh + 8 * c;
@@ -690,13 +696,13 @@ struct Kernel {
           const int tb = first_token(i);
           Copies copies(wave);
           acc c[SUB];
-          // (the 128-row kernel of an fp8 cache has no registers for it beside the scores)
-          if constexpr (WR > 1 && MR == 32) {
+          // (in waves of 32 rows an fp8 cache leaves no registers for it beside the scores)
+          if constexpr (WR > 1 && MR == 32 && FP8) {
             copies.prepare(a, src, first_token(i + AHEAD), wr, lane);
             copies.emit_all(tile_of(i + AHEAD), wr, lane);
           }
           auto ahead = [&](int k) {
-            if constexpr (MR == 16) {
+            if constexpr (MR == 16 || !FP8) {
               if (k == 1) copies.find(a, src, first_token(i + AHEAD), wr, lane);
               if (k == 6) copies.address(a, wr, lane);
               if constexpr (WR > 1) copies.emit_at(k, NA, tile_of(i + AHEAD), wr, lane);
@@ -770,7 +776,7 @@ struct Kernel {
       if (whole) factor *= total > 0.0f ? 1.0f / total : total == 0.0f ? 0.0f : NAN;
       if constexpr (FP8) factor *= 1.0f / kScaleUp<DT>;
       if (wt == 0 && lane < MR) {
-        const int64_t at = static_cast<int64_t>(slot) * ROWS + wr * MR + ln;
+        const int64_t at = static_cast<int64_t>(slot) * TILE_ROWS + share + wr * MR + ln;
         if (whole) {
           place[wr * MR + ln] = live ? b * a.ob + tok_new * a.os + head * a.oh : -1;
           if (live && a.lse)
@@ -782,21 +788,21 @@ struct Kernel {
       }
     }
 #pragma unroll
-    for (int w0 = 0; w0 < 4; w0 += EW) {
+    for (int w0 = 0; w0 < WR; w0 += EWR) {
       if (w0) __syncthreads();
-      if (wave >= w0 && wave < w0 + EW) {
+      if (wr >= w0 && wr < w0 + EWR) {
 #pragma unroll
         for (int j = 0; j < OB; ++j) {
 #pragma unroll
           for (int q = 0; q < M::REGS / 4; ++q) {
-            float* d = ep + ((wave - w0) * MR + ln) * PITCH + j * MR + q * 8 + 4 * h;
+            float* d = ep + ((wt * EWR + wr - w0) * MR + ln) * PITCH + j * MR + q * 8 + 4 * h;
             *reinterpret_cast<float4*>(d) = make_float4(o[j][4 * q] * factor, o[j][4 * q + 1] * factor,
                                                         o[j][4 * q + 2] * factor, o[j][4 * q + 3] * factor);
           }
         }
       }
       __syncthreads();
-      constexpr int PASS = ROWS < EW * MR ? ROWS : EW * MR;  // rows of this pass
+      constexpr int PASS = EWR * MR;  // rows of this pass
 #pragma unroll 4
       for (int i = tid; i < PASS * (DL / 4); i += NT) {
         const int r = i / (DL / 4), d = 4 * (i % (DL / 4));
@@ -804,7 +810,7 @@ struct Kernel {
         float4 x = make_float4(0, 0, 0, 0);
 #pragma unroll
         for (int t = 0; t < WT; ++t) {
-          const float4 y = *reinterpret_cast<const float4*>(ep + (t * ROWS + r) * PITCH + d);
+          const float4 y = *reinterpret_cast<const float4*>(ep + (t * PASS + r) * PITCH + d);
           x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
         }
         if (to < 0) continue;
@@ -819,11 +825,11 @@ struct Kernel {
   }
 };
 
-template <int DT, bool FP8, int DL, int DR, int MR, int WR>
+template <int DT, bool FP8, int DL, int DR, int MR, int WR, int SPLIT>
 __global__ __launch_bounds__(NT, 1) void decode_kernel(Args a) {
   // all of the kernel's LDS, so that it starts at address 0: copies and tile addresses count on it
   extern __shared__ __align__(16) uint8_t lds[];
-  Kernel<DT, FP8, DL, DR, MR, WR>::run(a, lds);
+  Kernel<DT, FP8, DL, DR, MR, WR, SPLIT>::run(a, lds);
 }
 
 // Joins the pieces of the (sequence, row tile)s that more than one workgroup

@@ -28,14 +28,14 @@ struct Layout {
 // From sizes that the host knows: the table's capacity bounds the lengths.
 Layout lay_out(int64_t batch, int64_t rows, int64_t latent_dim, int64_t capacity) {
   Layout d;
-  d.shape = shape_for(rows);
+  d.shape = shape_for(batch, rows);
   const int64_t tile = d.shape.tile_rows(), step = d.shape.step();
   d.row_tiles = (rows + tile - 1) / tile;
   const int64_t steps = capacity > step ? (capacity + step - 1) / step : 1;
   d.min_steps = 128 / step;
   const int64_t tiles = batch * d.row_tiles, wanted = (tiles * steps + d.min_steps - 1) / d.min_steps;
   d.groups = wanted > tiles ? wanted : tiles;
-  if (d.groups > kGroups) d.groups = kGroups;
+  if (d.groups > kGroups / d.shape.split) d.groups = kGroups / d.shape.split;
   d.split = steps > 1 && d.groups > 1;
   d.join_bytes = (d.groups * 16 + 255) / 256 * 256;
   d.ml_bytes = 2 * d.groups * tile * 8;

@@ -32,23 +32,35 @@ struct Args {
 };
 
 // What a piece costs whatever its length (queries in, output out, latencies),
-// in steps of its kernel
-template <int MR>
-constexpr int kFixed = MR == 32 ? 10 : 2;
+// in steps of its kernel. With two workgroups a tile: 8 takes 75.2 us for 48
+// sequences of up to 5003 tokens and 128 rows and 93.6 for 40 of up to 4096 in
+// fp8 with 512 rows; 4 takes 90 and 100, 12 takes 82 and 107.
+template <int MR, int SPLIT>
+constexpr int kFixed = MR == 32 ? (SPLIT == 2 ? 8 : 10) : 2;
 
-// Rows of a tile and tokens of a step for `rows` rows a sequence: up to 16 (32,
-// 64) rows fill one (two, four) waves of 16 rows, and the other waves of a
-// workgroup take other tokens; above that, four waves of 32 rows.
+// Rows of a tile and tokens of a step. Up to 16 (32, 64) rows a sequence fill
+// one (two, four) waves of 16 rows, and the other waves of a workgroup take
+// other tokens. Above that a tile has 128 rows, in waves of 32, as four waves
+// of one workgroup or as two workgroups side by side on the same tokens, each
+// with two waves on its 64 rows and two on other tokens of them. Two halve what
+// a piece reads of queries and writes of partial sums, but copy the cache twice
+// to LDS (the second time from the XCD's L2) and cannot overlap a tile's
+// softmax with the next one's scores: they win where sequences are cut into
+// pieces. 128 heads over a bf16 cache, us, two workgroups against one: 16
+// sequences of 4096 tokens 49 / 72, 48 of 2048 63 / 79, 128 of 4096 192 / 205,
+// 192 of 1024 and of 4096 113 / 125 and 308 / 298, 256 of 300 and of 8192
+// 66 / 58 and 686 / 615. fp8: 16 of 4096 55 / 71, 192 of 4096 334 / 331, 256 of
+// 2048 233 / 219.
 struct Shape {
-  int mr, wr;
-  int tile_rows() const { return mr * wr; }
+  int mr, wr, split;  // rows of a wave, waves over rows, workgroups over rows
+  int tile_rows() const { return mr * wr * split; }
   int step() const { return 32 * (4 / wr); }
 };
-inline Shape shape_for(int64_t rows) {
-  if (rows <= 16) return {16, 1};
-  if (rows <= 32) return {16, 2};
-  if (rows <= 64) return {16, 4};
-  return {32, 4};
+inline Shape shape_for(int64_t batch, int64_t rows) {
+  if (rows <= 16) return {16, 1, 1};
+  if (rows <= 32) return {16, 2, 1};
+  if (rows <= 64) return {16, 4, 1};
+  return batch * ((rows + 127) / 128) <= 192 ? Shape{32, 2, 2} : Shape{32, 4, 1};
 }
 
 // launches decode_kernel and, where a.parts is set, combine_kernel
