@@ -39,7 +39,8 @@ constexpr int kAheadKeys = FP8 ? 4 : 6;
 constexpr int kAheadValues = 6;
 
 // ---------------------------------------------------------------------------
-// The division of the work. One list of units: for each sequence, for each tile
+// The division of the work. Few row tiles are cut one by one into equal pieces,
+// one a workgroup. Many tiles are one list of units: for each sequence, for each tile
 // of its rows, kFixed units for what a piece costs whatever its length (its
 // queries, its output) and one for each step over the tokens. Workgroup w takes
 // the w-th of `groups` equal pieces of the list, whatever the lengths are (with
@@ -53,6 +54,7 @@ struct Division {
   PCAMD_DEV int group_of(int u) const { return u < r * (q + 1) ? u / (q + 1) : r + (u - r * (q + 1)) / q; }
 };
 
+// Sequence b's tokens
 PCAMD_DEV int length_of(const Args& a, int b) {
   const int n = a.lens[b];
   return n < 0 ? 0 : n > a.capacity ? a.capacity : n;
@@ -289,56 +291,95 @@ struct Kernel {
     int* found = wave_total + NT / 64;
     const int tid = threadIdx.x;
 
-    // ---- this workgroup's piece of the list
-    int sum = 0, steps_all;
-    for (int b = tid; b < a.batch; b += NT) sum += steps_of(length_of(a, b), STEP);
-    int before = block_scan(sum, wave_total, steps_all);
+    // ---- this workgroup's piece: steps [in_seq, in_seq + end - begin) of
+    // sequence b's row tiles one after the other, and of the sequences behind it
     const int tiles = a.batch * a.row_tiles;
-    const int wanted = (steps_all * a.row_tiles + a.min_steps - 1) / a.min_steps;
-    int groups = wanted > tiles ? wanted : tiles;
-    if (groups > a.groups) groups = a.groups;
-    // with few tiles every workgroup has one piece of one: nothing to weigh
-    const int FIXED = tiles > 1 && tiles * 16 >= groups ? kFixed<MR, SPLIT> : 0;
-    const Division div(a.row_tiles * (steps_all + a.batch * FIXED), groups);
-    const int wgs = groups * SPLIT;
-    if (static_cast<int>(blockIdx.x) >= wgs) {
-      if (a.parts && tid == 0) a.joins[blockIdx.x / SPLIT] = make_int4(0, 0, -1, 0);
-      return;
-    }
-    // Neighbouring pieces belong to the same sequence, and a piece's workgroups
-    // read the same tokens at the same time: put them on the same XCD (workgroups
-    // go round the eight of them), whose L2 then holds its queries and the tokens.
-    const int place = wgs % 8 ? blockIdx.x : blockIdx.x % 8 * (wgs / 8) + blockIdx.x / 8;
-    const int w = place / SPLIT, share = place % SPLIT * ROWS;  // its first row of the tile
-    const int begin = div.first(w), end = div.first(w + 1);
-    int base = 0;
-    for (int b0 = 0; b0 < a.batch; b0 += NT) {
-      const int b = b0 + tid;
-      const int mine = b < a.batch ? (steps_of(length_of(a, b), STEP) + FIXED) * a.row_tiles : 0;
-      int total;
-      if (a.batch <= NT) before = (before + tid * FIXED) * a.row_tiles;  // the first scan's answer, where it had one sequence a thread
-      else before = base + block_scan(mine, wave_total, total);
-      if (mine && begin >= before && begin < before + mine) {
-        found[0] = b;
-        found[1] = begin - before;
-        found[2] = 1;
+    int b, in_seq, begin, end, w, share, FIXED = 0;
+    auto take_place = [&](int groups) {  // false: nothing to do here
+      const int wgs = groups * SPLIT, eighth = (wgs + 8 * SPLIT - 1) / (8 * SPLIT) * SPLIT;
+      // Neighbouring pieces belong to the same sequence, and a piece's workgroups
+      // read the same tokens at the same time: put them on the same XCD (workgroups
+      // go round the eight of them), whose L2 then holds its queries and the tokens.
+      int place = blockIdx.x;
+      if (8 * eighth <= static_cast<int>(gridDim.x) && place < 8 * eighth) place = place % 8 * eighth + place / 8;
+      w = place / SPLIT;
+      share = place % SPLIT * ROWS;  // its first row of the tile
+      if (place < wgs) return true;
+      if (a.parts && tid == 0) a.joins[w] = make_int4(0, 0, -1, 0);
+      return false;
+    };
+    if (few_tiles(tiles, SPLIT)) {
+      // Each row tile alone, in equal pieces of up to `most` steps. Every wave
+      // works it out for itself, a lane a sequence.
+      const int lane = tid % 64;
+      const int len = lane < a.batch ? length_of(a, lane) : 0, steps = lane < a.batch ? steps_of(len, STEP) : 0;
+      int all = steps;
+#pragma unroll
+      for (int d = 32; d > 0; d >>= 1) all += __shfl_xor(all, d, 64);
+      const int spare = kWorkgroups / SPLIT - tiles;  // sum ceil(steps / most) <= sum steps / most + tiles
+      int most = (all * a.row_tiles + spare - 1) / spare;
+      if (most < a.min_steps) most = a.min_steps;
+      const int pieces = (steps + most - 1) / most;
+      int upto = pieces * a.row_tiles;
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) {
+        const int o = __shfl_up(upto, d, 64);
+        if (lane >= d) upto += o;
       }
-      if (a.batch > NT) {
-        base += total;
-        if (base > begin) break;
+      if (!take_place(__builtin_amdgcn_readlane(upto, 63))) return;
+      b = __popcll(__ballot(upto <= w));
+      const int of_b = __builtin_amdgcn_readlane(pieces, b), steps_b = __builtin_amdgcn_readlane(steps, b);
+      const int at = w - (__builtin_amdgcn_readlane(upto, b) - of_b * a.row_tiles), rt = at / of_b, i = at - rt * of_b;
+      const int q = steps_b / of_b, r = steps_b - q * of_b;
+      begin = 0;
+      end = q + (i < r);
+      in_seq = rt * steps_b + i * q + (i < r ? i : r);
+      // the second piece's workgroup notes which tile it is and the last piece's workgroup
+      if (a.parts && tid == 0 && share == 0)
+        a.joins[w] = i == 1 ? make_int4(b, rt, 1, w + of_b - 2) : make_int4(0, 0, -1, 0);
+    } else {
+      int sum = 0, steps_all;
+      for (int i = tid; i < a.batch; i += NT) sum += steps_of(length_of(a, i), STEP);
+      int before = block_scan(sum, wave_total, steps_all);
+      steps_all = __builtin_amdgcn_readfirstlane(steps_all);
+      const int wanted = (steps_all * a.row_tiles + a.min_steps - 1) / a.min_steps;
+      int groups = wanted > tiles ? wanted : tiles;
+      if (groups > a.groups) groups = a.groups;
+      FIXED = kFixed<MR, SPLIT>;
+      const Division div(a.row_tiles * (steps_all + a.batch * FIXED), groups);
+      if (!take_place(groups)) return;
+      begin = div.first(w);
+      end = div.first(w + 1);
+      int base = 0;
+      for (int b0 = 0; b0 < a.batch; b0 += NT) {
+        const int i = b0 + tid;
+        const int mine = i < a.batch ? (steps_of(length_of(a, i), STEP) + FIXED) * a.row_tiles : 0;
+        int total;
+        if (a.batch <= NT) before = (before + tid * FIXED) * a.row_tiles;  // the first scan's answer, where it had one sequence a thread
+        else before = base + block_scan(mine, wave_total, total);
+        if (mine && begin >= before && begin < before + mine) {
+          found[0] = i;
+          found[1] = begin - before;
+        }
+        if (a.batch > NT) {
+          base += total;
+          if (base > begin) break;
+        }
       }
-    }
-    __syncthreads();
-    int b = found[0], in_seq = found[1];
-    if (a.parts && tid == 0 && share == 0) {
-      // Where pieces meet: the first workgroup that starts inside a (sequence,
-      // row tile) notes which it is and which workgroup holds the last piece;
-      // the one before it holds the first.
-      const int tile = steps_of(length_of(a, b), STEP) + FIXED;
-      const int in_tile = in_seq % tile, real = begin - in_tile + FIXED;  // its first step's unit
-      a.joins[w] = begin > real && div.first(w - 1) <= real
-                       ? make_int4(b, in_seq / tile, 1, div.group_of(real + tile - FIXED - 1))
-                       : make_int4(0, 0, -1, 0);
+      __syncthreads();
+      // in scalar registers, as all that steers the segments: branches on them are scalar branches
+      b = __builtin_amdgcn_readfirstlane(found[0]);
+      in_seq = __builtin_amdgcn_readfirstlane(found[1]);
+      if (a.parts && tid == 0 && share == 0) {
+        // Where pieces meet: the first workgroup that starts inside a (sequence,
+        // row tile) notes which it is and which workgroup holds the last piece;
+        // the one before it holds the first.
+        const int tile = steps_of(length_of(a, b), STEP) + FIXED;
+        const int in_tile = in_seq % tile, real = begin - in_tile + FIXED;  // its first step's unit
+        a.joins[w] = begin > real && div.first(w - 1) <= real
+                         ? make_int4(b, in_seq / tile, 1, div.group_of(real + tile - FIXED - 1))
+                         : make_int4(0, 0, -1, 0);
+      }
     }
 
     for (int u = begin; u < end;) {

@@ -15,8 +15,6 @@ extern template int launch<kBF16, 256, 32>(const Args&, Shape, bool, hipStream_t
 extern template int launch<kF16, 512, 64>(const Args&, Shape, bool, hipStream_t);
 extern template int launch<kF16, 256, 32>(const Args&, Shape, bool, hipStream_t);
 
-constexpr int64_t kGroups = 256;  // one workgroup (four waves, most of the LDS) a CU
-
 struct Layout {
   Shape shape;
   int64_t row_tiles, groups, min_steps;
@@ -32,10 +30,12 @@ Layout lay_out(int64_t batch, int64_t rows, int64_t latent_dim, int64_t capacity
   const int64_t tile = d.shape.tile_rows(), step = d.shape.step();
   d.row_tiles = (rows + tile - 1) / tile;
   const int64_t steps = capacity > step ? (capacity + step - 1) / step : 1;
-  d.min_steps = 128 / step;
-  const int64_t tiles = batch * d.row_tiles, wanted = (tiles * steps + d.min_steps - 1) / d.min_steps;
-  d.groups = wanted > tiles ? wanted : tiles;
-  if (d.groups > kGroups / d.shape.split) d.groups = kGroups / d.shape.split;
+  d.min_steps = step == 128 ? 1 : 2;
+  const int64_t tiles = batch * d.row_tiles, cap = kWorkgroups / d.shape.split;
+  d.groups = few_tiles(tiles, d.shape.split) ? tiles * ((steps + d.min_steps - 1) / d.min_steps)
+                                             : (tiles * steps + d.min_steps - 1) / d.min_steps;
+  if (d.groups < tiles) d.groups = tiles;
+  if (d.groups > cap) d.groups = cap;
   d.split = steps > 1 && d.groups > 1;
   d.join_bytes = (d.groups * 16 + 255) / 256 * 256;
   d.ml_bytes = 2 * d.groups * tile * 8;

@@ -63,6 +63,13 @@ inline Shape shape_for(int64_t batch, int64_t rows) {
   return batch * ((rows + 127) / 128) <= 192 ? Shape{32, 2, 2} : Shape{32, 4, 1};
 }
 
+constexpr int kWorkgroups = 256;  // one (four waves, most of the LDS) a CU
+
+// Whether each row tile is cut by itself: a workgroup then never has parts of
+// two (it would work on them one after the other), and at most an eighth of the
+// workgroups is lost to tiles that do not divide evenly.
+__host__ __device__ inline bool few_tiles(int64_t tiles, int split) { return tiles * 8 <= kWorkgroups / split; }
+
 // launches decode_kernel and, where a.parts is set, combine_kernel
 template <int DT, int DL, int DR>
 int launch(const Args& a, Shape shape, bool fp8, hipStream_t st);
