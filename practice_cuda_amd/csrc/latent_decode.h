@@ -12,6 +12,16 @@
 // codes enter the products as they are (16 bits hold them exactly); the scales
 // multiply fp32 values: the four groups' partial scores, and the weights p
 // ahead of their rounding to 16 bits, once for each group of value columns.
+//
+// What bounds it. With up to 16 rows the cache's bytes: 48 sequences of 32768
+// tokens, 16 heads, bf16: 1.81 GB in 329 us, 5.5 TB/s. With 128 rows the
+// products and the operands that they read from LDS, level with each other: 256
+// sequences of 8192 tokens 974 TFLOP/s in whole tiles. Where sequences are cut
+// into pieces, what a piece costs beside its steps: queries in, the first
+// tokens' way, partial sums out and in again. 48 sequences of 1 to 5003 tokens,
+// 128 heads: 69 us (34 of them in steps, 13 of output) and the joins 9; 19 of up
+// to 6007 tokens with 3 new ones each over an fp8 cache: 91 us, the steps' 63
+// bound by widening the codes.
 #pragma once
 
 #include "attn_common.h"

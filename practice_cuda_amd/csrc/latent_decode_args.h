@@ -33,8 +33,8 @@ struct Args {
 
 // What a piece costs whatever its length (queries in, output out, latencies),
 // in steps of its kernel. With two workgroups a tile: 8 takes 75.2 us for 48
-// sequences of up to 5003 tokens and 128 rows and 93.6 for 40 of up to 4096 in
-// fp8 with 512 rows; 4 takes 90 and 100, 12 takes 82 and 107.
+// sequences of up to 5003 tokens and 128 rows and 93.6 for 19 of up to 6007 and
+// 384 rows in fp8; 4 takes 90 and 100, 12 takes 82 and 107.
 template <int MR, int SPLIT>
 constexpr int kFixed = MR == 32 ? (SPLIT == 2 ? 8 : 10) : 2;
 

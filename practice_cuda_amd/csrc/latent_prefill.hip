@@ -9,6 +9,14 @@
 // One workgroup holds NR x 128 query rows of one head, NR x 32 a wave, and
 // walks over the keys they see in steps of 32 with a running maximum and sum.
 // With NR = 2 every operand read from LDS serves two matrix products.
+//
+// Bound by the matrix products: 2 (DN + DR + DV) operations for each seen pair
+// and head, beside an exponential and a rounding to 16 bits a pair, which the
+// vector units do while the products run. 8192 tokens, 32 heads, causal, bf16:
+// 688 GFLOP in 671 us, 1.03 PFLOP/s, where an 8192^3 product of the library
+// reaches 1.25; 6 prompts of up to 1111 tokens behind up to 700 cached ones, 128
+// heads: 310 GFLOP in 475 us (their ends fill tiles in part). Under this load
+// the clock falls to about 1.6 GHz, so what remains is power.
 #include <hip/hip_runtime.h>
 
 #include <atomic>
@@ -550,7 +558,9 @@ int launch_rows(Args a, hipStream_t st) {
 
 template <int DT, int DN, int DR, int DV>
 int launch(const Args& a, hipStream_t st) {
-  // 128-row tiles where 256-row ones would leave CUs idle
+  // 128-row tiles where 256-row ones would leave CUs idle. Rows x heads, causal, bf16, us with 128 and 256 rows:
+  // 2048 x 16 48 / 74, 512 x 128 35 / 55, 4096 x 16 103 / 134; 768 x 128 72 / 65, 8192 x 16 364 / 330, 16384 x 16
+  // 1379 / 1213; 16 sequences of 512 69 / 64
   return a.total_q * a.heads <= 256 * 256 ? launch_rows<DT, DN, DR, DV, 1>(a, st) : launch_rows<DT, DN, DR, DV, 2>(a, st);
 }
 

@@ -11,6 +11,11 @@
 // sum of squares over the row, the maxima over 16-lane groups), so every input
 // is read once. Lane i of the team takes the 8-element chunks i, i + TEAM, ..;
 // 16 neighbouring lanes then hold one quantization group.
+//
+// Bound by memory: 4096 x 7168 bf16 with a residual, 206 MB, takes 50.2 us, 4.1
+// TB/s (a copy of such size 4.9 on the same machine); by the launch where rows
+// are few: 56 tokens of 512 + 64 into an fp8 cache 9.3 us a call, most of it
+// the host's.
 #include <hip/hip_runtime.h>
 
 #include <cstdint>

@@ -291,7 +291,7 @@ def hip_latent_prefill(
     chunks. Rows that see no key, and queries behind the last sequence, give
     zeros and a log-sum of -inf. softmax_scale: default (key + rotary) ** -0.5.
     A NaN or infinity in a value reaches the queries that see it and may reach
-    up to 63 earlier ones of its sequence.
+    up to 31 earlier ones of its sequence.
 
     Returns out [Tq, H, value] in q's dtype and, with return_lse, float32
     [Tq, H]: the natural logarithm of the sum of exponentials."""
