@@ -34,6 +34,8 @@ using namespace attn;
 
 constexpr int NT = 256;
 constexpr int TOK = 32;  // tokens of a wave's step
+// 16 bytes of an output row, which is 8-byte aligned
+typedef uint32_t u32x4_out __attribute__((ext_vector_type(4), aligned(8)));
 
 // How far (log2) a score may pass the reference point of its row's weights
 // before the reference moves and the wave's sums are rescaled. Weights and sums
@@ -127,12 +129,13 @@ struct Kernel {
   static_assert(!PIPE || NB == 4, "the overlapped loop holds two tiles while two more are on their way");
   static constexpr int PAGES = 256;  // page numbers kept in LDS
   static constexpr int RING = WT * NB * TILE;
-  // epilogue, in the ring's place: the rows of EW waves at a time, those that
-  // share rows among them. Whole rows,
-  // because half rows of all of them would keep half of the memory channels idle.
-  static constexpr int EW = MR == 32 && DL > 256 ? 2 : 4, EWR = EW / WT;
-  static constexpr int PITCH = DL + 4;
-  static constexpr int EPI = EW * MR * PITCH * 4 + 4 * MR * 8 + ROWS * 8;
+  // epilogue, in the ring's place: what the waves of a row hand each other, and
+  // whole rows on their way out
+  static constexpr int OWN = OB / WT, QN = M::REGS / 4;  // blocks that a wave brings to their end; quads of a block
+  static constexpr int PACK = OWN * QN * 64 * 16;        // what it gets from each of the others
+  static constexpr int OUT_PITCH = OWN * MR * 2 + 16, STAGE = WT > 1 ? (WT - 1) * PACK : MR * OUT_PITCH;
+  static_assert(STAGE >= MR * OUT_PITCH, "a wave's rows leave through what it was handed");
+  static constexpr int EPI = 4 * STAGE + 4 * MR * 8 + 4 * MR * 8;
   // prologue, there too: each wave's query rows, [block][row][128 bytes]
   static constexpr int QBLOCKS = DL / 64, QBLOCK = MR * 128;
   static constexpr int QUERIES = (QBLOCKS + 1) * QBLOCK;
@@ -805,17 +808,18 @@ struct Kernel {
     }
     l = row_sum<MR>(l);
 
-    // ---- epilogue: the waves' rows meet in LDS and leave as whole rows
+    // ---- epilogue. The WT waves of a row split its columns: each hands the
+    // others their blocks through LDS and adds up its own.
     const bool whole = n == steps;
-    float* ep = reinterpret_cast<float*>(lds);
-    float2* ml = reinterpret_cast<float2*>(lds + EW * MR * PITCH * 4);  // of each wave's rows; then factors and sums
-    int64_t* place = reinterpret_cast<int64_t*>(ml + 4 * MR);          // where a row of the tile goes; -1: nowhere
+    float2* ml = reinterpret_cast<float2*>(lds + 4 * STAGE);                     // of each wave's rows
+    int64_t* place = reinterpret_cast<int64_t*>(lds + 4 * STAGE + 4 * MR * 8) + wave * MR;  // where its rows go; -1: nowhere
+    float big = m, total = l, factor = 1.0f;  // of this lane's row
     __syncthreads();
-    if (lane < MR) ml[wave * MR + ln] = make_float2(m, l);
-    __syncthreads();
-    float factor = 1.0f;  // of this lane's row
-    {
-      float big = kNoMax, total = 0.0f;
+    if constexpr (WT > 1) {
+      if (lane < MR) ml[wave * MR + ln] = make_float2(m, l);
+      __syncthreads();
+      big = kNoMax;
+      total = 0.0f;
 #pragma unroll
       for (int t = 0; t < WT; ++t) big = fmaxf(big, ml[(t * WR + wr) * MR + ln].x);
 #pragma unroll
@@ -824,52 +828,71 @@ struct Kernel {
         total += __builtin_amdgcn_exp2f(s.x - big) * s.y;
       }
       factor = __builtin_amdgcn_exp2f(m - big);
-      if (whole) factor *= total > 0.0f ? 1.0f / total : total == 0.0f ? 0.0f : NAN;
-      if constexpr (FP8) factor *= 1.0f / kScaleUp<DT>;
-      if (wt == 0 && lane < MR) {
-        const int64_t at = static_cast<int64_t>(slot) * TILE_ROWS + share + wr * MR + ln;
-        if (whole) {
-          place[wr * MR + ln] = live ? b * a.ob + tok_new * a.os + head * a.oh : -1;
-          if (live && a.lse)
-            a.lse[b * a.lb + tok_new * a.ls + head * a.lh] = total == 0.0f ? -INFINITY : (big + log2f(total)) * kLn2;
-        } else {
-          place[wr * MR + ln] = live ? at * DL : -1;
-          a.part_ml[at] = make_float2(big, total);
-        }
+    }
+    if (whole) factor *= total > 0.0f ? 1.0f / total : total == 0.0f ? 0.0f : NAN;
+    if constexpr (FP8) factor *= 1.0f / kScaleUp<DT>;
+    const int64_t at = static_cast<int64_t>(slot) * TILE_ROWS + share + wr * MR;  // of its first row among the partial sums
+    if (lane < MR) {
+      place[ln] = live ? b * a.ob + tok_new * a.os + head * a.oh : -1;
+      if (wt == 0) {
+        if (!whole) a.part_ml[at + ln] = make_float2(big, total);
+        else if (live && a.lse)
+          a.lse[b * a.lb + tok_new * a.ls + head * a.lh] = total == 0.0f ? -INFINITY : (big + log2f(total)) * kLn2;
       }
     }
+    auto quad = [&](int j, int q) {
+      return make_float4(o[j][4 * q] * factor, o[j][4 * q + 1] * factor, o[j][4 * q + 2] * factor, o[j][4 * q + 3] * factor);
+    };
+    float4 own[WT > 1 ? OWN * QN : 1];
+    if constexpr (WT > 1) {
 #pragma unroll
-    for (int w0 = 0; w0 < WR; w0 += EWR) {
-      if (w0) __syncthreads();
-      if (wr >= w0 && wr < w0 + EWR) {
+      for (int w = 0; w < WT; ++w) {
+        if (wt != w) continue;
 #pragma unroll
         for (int j = 0; j < OB; ++j) {
 #pragma unroll
-          for (int q = 0; q < M::REGS / 4; ++q) {
-            float* d = ep + ((wt * EWR + wr - w0) * MR + ln) * PITCH + j * MR + q * 8 + 4 * h;
-            *reinterpret_cast<float4*>(d) = make_float4(o[j][4 * q] * factor, o[j][4 * q + 1] * factor,
-                                                        o[j][4 * q + 2] * factor, o[j][4 * q + 3] * factor);
+          for (int q = 0; q < QN; ++q) {
+            const int to = j / OWN, i = j % OWN * QN + q;
+            if (to == w) own[i] = quad(j, q);
+            else *reinterpret_cast<float4*>(lds + (wr * WT + to) * STAGE + (w < to ? w : w - 1) * PACK + (i * 64 + lane) * 16) = quad(j, q);
           }
         }
       }
       __syncthreads();
-      constexpr int PASS = EWR * MR;  // rows of this pass
-#pragma unroll 4
-      for (int i = tid; i < PASS * (DL / 4); i += NT) {
-        const int r = i / (DL / 4), d = 4 * (i % (DL / 4));
-        const int64_t to = place[w0 * MR + r];
-        float4 x = make_float4(0, 0, 0, 0);
 #pragma unroll
-        for (int t = 0; t < WT; ++t) {
-          const float4 y = *reinterpret_cast<const float4*>(ep + (t * PASS + r) * PITCH + d);
-          x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
+      for (int t = 0; t < WT - 1; ++t) {
+#pragma unroll
+        for (int i = 0; i < OWN * QN; ++i) {
+          const float4 x = *reinterpret_cast<const float4*>(lds + (wr * WT + wt) * STAGE + t * PACK + (i * 64 + lane) * 16);
+          own[i].x += x.x; own[i].y += x.y; own[i].z += x.z; own[i].w += x.w;
         }
-        if (to < 0) continue;
-        if (whole)
-          *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + to + d) =
-              make_uint2(Elem<DT>::narrow2(x.x, x.y), Elem<DT>::narrow2(x.z, x.w));
-        else
-          *reinterpret_cast<float4*>(a.parts + to + d) = x;
+      }
+    }
+    auto sum = [&](int i) {  // columns i / QN * MR + i % QN * 8 + 4 h .. of the wave's blocks
+      if constexpr (WT > 1) return own[i];
+      else return quad(i / QN, i % QN);
+    };
+    if (!whole) {
+      // as the lanes hold them, 1 KB a store: [row block][column block][quad][lane]
+      float4* to = reinterpret_cast<float4*>(a.parts + at * DL) + wt * (PACK / 16) + lane;
+#pragma unroll
+      for (int i = 0; i < OWN * QN; ++i) to[i * 64] = sum(i);
+    } else {
+      uint8_t* rows = lds + (wr * WT + wt) * STAGE;
+#pragma unroll
+      for (int i = 0; i < OWN * QN; ++i) {
+        const float4 x = sum(i);
+        *reinterpret_cast<uint2*>(rows + ln * OUT_PITCH + 2 * (i / QN * MR + i % QN * 8 + 4 * h)) =
+            make_uint2(Elem<DT>::narrow2(x.x, x.y), Elem<DT>::narrow2(x.z, x.w));
+      }
+      constexpr int CHUNKS = OWN * MR / 8;  // 16-byte chunks of a row
+#pragma unroll 4
+      for (int i = lane; i < MR * CHUNKS; i += 64) {
+        const int r = i / CHUNKS, c = i % CHUNKS;
+        const uint4 x = *reinterpret_cast<const uint4*>(rows + r * OUT_PITCH + 16 * c);
+        const u32x4_out y = {x.x, x.y, x.z, x.w};
+        if (place[r] >= 0)
+          *reinterpret_cast<u32x4_out*>(static_cast<uint16_t*>(a.out) + place[r] + wt * (OWN * MR) + 8 * c) = y;
       }
     }
     __syncthreads();
@@ -885,26 +908,30 @@ __global__ __launch_bounds__(NT, 1) void decode_kernel(Args a) {
 
 // Joins the pieces of the (sequence, row tile)s that more than one workgroup
 // worked on: o = sum_i 2^(m_i - m) o_i / sum_i 2^(m_i - m) l_i. Every workgroup
-// lists the joins from the main kernel's notes. Few pieces: a wave takes a row,
-// all pieces' loads at once. Many (a long context split over the whole device):
-// a workgroup takes a row's 128 columns, and eight groups of lanes share the
-// pieces.
+// lists the joins from the main kernel's notes. Partial sums lie as that
+// kernel's lanes held them, in units of 1 KB: MR rows (a lane's is lane % MR)
+// and 256 / MR columns (four of them its own). Few pieces: a wave takes two
+// units, all pieces' loads at once. Many (a long context split over the whole
+// device): a workgroup takes a unit, and its waves share the pieces.
 constexpr int kFewPieces = 8;
-constexpr int kJoinGroups = 1024;  // four workgroups a CU; twice as many take as long
+constexpr int kJoinThreads = 512, kJoinWaves = kJoinThreads / 64;
+constexpr int kJoinGroups = 512;  // two workgroups a CU
 
 struct Joins {
-  int4 join[2][NT];  // few pieces, many: {sequence, row tile, 1, last workgroup}
-  int first[2][NT];  // workgroup of the second piece
-  int count[2][NT / 64];
-  float weight[NT + 1];
-  float red[NT / 64];
-  float4 sums[8][32];
+  int4 join[2][kWorkgroups];  // few pieces, many: {sequence, row tile, 1, last workgroup}
+  int first[2][kWorkgroups];  // workgroup of the second piece
+  int count[2][kJoinWaves];
+  float red[kJoinWaves][32];
+  float4 sums[kJoinWaves][64];
+  float total[kJoinWaves][64];
 };
 
-template <int DT, int DL>
-__global__ __launch_bounds__(NT) void combine_kernel(Args a, int tile_rows) {
+template <int DT, int DL, int MR>
+__global__ __launch_bounds__(kJoinThreads) void combine_kernel(Args a, int tile_rows) {
   __shared__ Joins L;
   const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64;
+  const int ln = lane % MR, h = lane / MR;
+  constexpr int UNITS = DL * MR / 256, COLS = 256 / MR;  // units of a row block, columns of a unit
 
   // ---- the lists, in the same order in every workgroup
   const int4 mine = tid < a.groups ? a.joins[tid] : make_int4(0, 0, -1, 0);
@@ -916,7 +943,7 @@ __global__ __launch_bounds__(NT) void combine_kernel(Args a, int tile_rows) {
 #pragma unroll
   for (int k = 0; k < 2; ++k)
 #pragma unroll
-    for (int w = 0; w < NT / 64; ++w) {
+    for (int w = 0; w < kJoinWaves; ++w) {
       before[k] += w < wave ? L.count[k][w] : 0;
       total[k] += L.count[k][w];
     }
@@ -940,105 +967,105 @@ __global__ __launch_bounds__(NT) void combine_kernel(Args a, int tile_rows) {
   };
   auto inverse = [](float l) { return l > 0.0f ? 1.0f / l : l == 0.0f ? 0.0f : NAN; };
 
-  // ---- few pieces: a wave a row
-  for (int i = blockIdx.x * (NT / 64) + wave; i < total[0] * tile_rows; i += gridDim.x * (NT / 64)) {
-    const int4 j = L.join[0][i / tile_rows];
-    const int first = L.first[0][i / tile_rows], r = i % tile_rows, n = j.w - first + 2;
-    int64_t out, lse;
-    if (!address(j, r, out, lse)) continue;
-    constexpr int V = DL / 256;
-    float4 x[kFewPieces][V];
+  const int blocks = tile_rows / MR;  // row blocks of a tile
+
+  // ---- few pieces: a wave for two units
+  const int of_tile = blocks * (UNITS / 2);
+  for (int i = blockIdx.x * kJoinWaves + wave; i < total[0] * of_tile; i += gridDim.x * kJoinWaves) {
+    const int t = i / of_tile, block = i / (UNITS / 2) % blocks, u = i % (UNITS / 2) * 2;
+    const int4 j = L.join[0][t];
+    const int first = L.first[0][t], n = j.w - first + 2;
+    float4 x[kFewPieces][2];
     float2 s[kFewPieces];
 #pragma unroll
     for (int p = 0; p < kFewPieces; ++p) {
-      const int64_t at = slot_of(first, p < n ? p : 0) * tile_rows + r;
-      s[p] = a.part_ml[at];
+      const int64_t at = slot_of(first, p < n ? p : 0) * tile_rows + block * MR;
+      s[p] = a.part_ml[at + ln];
       if (p >= n) s[p] = make_float2(kNoMax, 0.0f);
       if (p < n) {
 #pragma unroll
-        for (int v = 0; v < V; ++v) x[p][v] = *reinterpret_cast<const float4*>(a.parts + at * DL + v * 256 + lane * 4);
+        for (int v = 0; v < 2; ++v) x[p][v] = reinterpret_cast<const float4*>(a.parts + at * DL)[(u + v) * 64 + lane];
       }
     }
     float m = kNoMax, l = 0.0f;
 #pragma unroll
     for (int p = 0; p < kFewPieces; ++p) m = fmaxf(m, s[p].x);
-    float4 o[V];
+    float4 o[2];
 #pragma unroll
-    for (int v = 0; v < V; ++v) o[v] = make_float4(0, 0, 0, 0);
+    for (int v = 0; v < 2; ++v) o[v] = make_float4(0, 0, 0, 0);
 #pragma unroll
     for (int p = 0; p < kFewPieces; ++p) {
       if (p >= n) break;
       const float f = __builtin_amdgcn_exp2f(s[p].x - m);
       l += f * s[p].y;
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
+      for (int v = 0; v < 2; ++v) {
         o[v].x += f * x[p][v].x; o[v].y += f * x[p][v].y; o[v].z += f * x[p][v].z; o[v].w += f * x[p][v].w;
       }
     }
+    int64_t out, lse;
+    const bool live = address(j, block * MR + ln, out, lse);
     const float inv = inverse(l);
+    uint2 y[2];
 #pragma unroll
-    for (int v = 0; v < V; ++v)
-      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + out + v * 256 + lane * 4) =
-          make_uint2(Elem<DT>::narrow2(o[v].x * inv, o[v].y * inv), Elem<DT>::narrow2(o[v].z * inv, o[v].w * inv));
-    if (lane == 0) finish(lse, m, l);
+    for (int v = 0; v < 2; ++v)
+      y[v] = make_uint2(Elem<DT>::narrow2(o[v].x * inv, o[v].y * inv), Elem<DT>::narrow2(o[v].z * inv, o[v].w * inv));
+    uint16_t* to = static_cast<uint16_t*>(a.out) + out + u * COLS;
+    if constexpr (MR == 32) {
+      // a lane's four columns of both units for eight of one
+      const auto p = __builtin_amdgcn_permlane32_swap(y[0].x, y[1].x, false, false);
+      const auto q = __builtin_amdgcn_permlane32_swap(y[0].y, y[1].y, false, false);
+      const u32x4_out z = {p[0], q[0], p[1], q[1]};
+      if (live) *reinterpret_cast<u32x4_out*>(to + 8 * h) = z;
+    } else if (live) {
+#pragma unroll
+      for (int v = 0; v < 2; ++v) *reinterpret_cast<uint2*>(to + v * COLS + 4 * h) = y[v];
+    }
+    if (live && u == 0 && h == 0) finish(lse, m, l);
   }
 
-  // ---- many: a workgroup for 128 columns of a row
-  constexpr int SLICES = DL / 128;
-  for (int i = blockIdx.x; i < total[1] * tile_rows * SLICES; i += gridDim.x) {
-    const int t = i / (tile_rows * SLICES), r = i / SLICES % tile_rows, slice = i % SLICES;
+  // ---- many: a workgroup for a unit
+  for (int i = blockIdx.x; i < total[1] * blocks * UNITS; i += gridDim.x) {
+    const int t = i / (blocks * UNITS), block = i / UNITS % blocks, u = i % UNITS;
     const int4 j = L.join[1][t];
-    const int first = L.first[1][t], n = j.w - first + 2;  // up to one more than there are threads
-    int64_t out, lse;
-    if (!address(j, r, out, lse)) continue;
-    float2 s[2];
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const int p = tid + k * NT;
-      s[k] = p < n ? a.part_ml[slot_of(first, p) * tile_rows + r] : make_float2(kNoMax, 0.0f);
-    }
-    float m = fmaxf(s[0].x, s[1].x);
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
-    if (lane == 0) L.red[wave] = m;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < NT / 64; ++w) m = fmaxf(m, L.red[w]);
-    float l = 0.0f;
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const float f = __builtin_amdgcn_exp2f(s[k].x - m);
-      l += f * s[k].y;
-      if (tid + k * NT < n) L.weight[tid + k * NT] = f;
-    }
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) l += __shfl_xor(l, d, 64);
-    __syncthreads();
-    if (lane == 0) L.red[wave] = l;
-    __syncthreads();
-    l = 0.0f;
-#pragma unroll
-    for (int w = 0; w < NT / 64; ++w) l += L.red[w];
-    const int col = slice * 128 + tid % 32 * 4;
-    float4 o = make_float4(0, 0, 0, 0);
+    const int first = L.first[1][t], n = j.w - first + 2;  // up to one more than there are workgroups
+    auto row_of = [&](int p) { return slot_of(first, p) * tile_rows + block * MR; };
+    float m = kNoMax;
 #pragma unroll 4
-    for (int p = tid / 32; p < n; p += 8) {
-      const float f = L.weight[p];
-      const float4 x = *reinterpret_cast<const float4*>(a.parts + (slot_of(first, p) * tile_rows + r) * DL + col);
+    for (int p = tid / MR; p < n; p += kJoinThreads / MR) m = fmaxf(m, a.part_ml[row_of(p) + ln].x);
+    m = row_max<MR>(m);
+    if (lane < MR) L.red[wave][ln] = m;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kJoinWaves; ++w) m = fmaxf(m, L.red[w][ln]);
+    float l = 0.0f;
+    float4 o = make_float4(0, 0, 0, 0);
+#pragma unroll 8
+    for (int p = wave; p < n; p += kJoinWaves) {
+      const int64_t at = row_of(p);
+      const float2 s = a.part_ml[at + ln];
+      const float4 x = reinterpret_cast<const float4*>(a.parts + at * DL)[u * 64 + lane];
+      const float f = __builtin_amdgcn_exp2f(s.x - m);
+      l += f * s.y;
       o.x += f * x.x; o.y += f * x.y; o.z += f * x.z; o.w += f * x.w;
     }
-    L.sums[tid / 32][tid % 32] = o;
+    L.sums[wave][lane] = o;
+    L.total[wave][lane] = l;
     __syncthreads();
-    if (tid < 32) {
+    if (wave == 0) {
 #pragma unroll
-      for (int p = 1; p < 8; ++p) {
-        const float4 x = L.sums[p][tid];
+      for (int w = 1; w < kJoinWaves; ++w) {
+        const float4 x = L.sums[w][lane];
         o.x += x.x; o.y += x.y; o.z += x.z; o.w += x.w;
+        l += L.total[w][lane];
       }
-      const float inv = inverse(l);
-      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + out + col) =
-          make_uint2(Elem<DT>::narrow2(o.x * inv, o.y * inv), Elem<DT>::narrow2(o.z * inv, o.w * inv));
-      if (tid == 0 && slice == 0) finish(lse, m, l);
+      int64_t out, lse;
+      if (address(j, block * MR + ln, out, lse)) {
+        const float inv = inverse(l);
+        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + out + u * COLS + 4 * h) =
+            make_uint2(Elem<DT>::narrow2(o.x * inv, o.y * inv), Elem<DT>::narrow2(o.z * inv, o.w * inv));
+        if (u == 0 && h == 0) finish(lse, m, l);
+      }
     }
     __syncthreads();
   }

@@ -31,8 +31,9 @@ int launch(const Args& a, Shape shape, bool fp8, hipStream_t st) {
   if (rc != PCAMD_OK || !a.parts) return rc;
   // as many workgroups as the joins can keep busy: one at most a boundary between pieces
   const int64_t tiles = a.batch * a.row_tiles, joins = tiles < a.groups - 1 ? tiles : a.groups - 1;
-  const int64_t most = joins * shape.tile_rows() * (DL / 128);
-  combine_kernel<DT, DL><<<static_cast<uint32_t>(most < kJoinGroups ? most : kJoinGroups), NT, 0, st>>>(a, shape.tile_rows());
+  const int64_t units = joins * shape.tile_rows() * DL / 256;  // of 1 KB
+  const auto kern = shape.mr == 32 ? combine_kernel<DT, DL, 32> : combine_kernel<DT, DL, 16>;
+  kern<<<static_cast<uint32_t>(units < kJoinGroups ? units : kJoinGroups), kJoinThreads, 0, st>>>(a, shape.tile_rows());
   return check_launch("combine_kernel");
 }
 
