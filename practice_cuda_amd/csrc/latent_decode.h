@@ -19,9 +19,9 @@
 // sequences of 8192 tokens 974 TFLOP/s in whole tiles. Where sequences are cut
 // into pieces, what a piece costs beside its steps: queries in, the first
 // tokens' way, partial sums out and in again. 48 sequences of 1 to 5003 tokens,
-// 128 heads: 69 us (34 of them in steps, 13 of output) and the joins 9; 19 of up
-// to 6007 tokens with 3 new ones each over an fp8 cache: 91 us, the steps' 63
-// bound by widening the codes.
+// 128 heads: 63 us (34 of them in steps) and the joins 10; 19 of up to 6007
+// tokens with 3 new ones each over an fp8 cache: 85 us, the steps' 60 bound by
+// widening the codes.
 #pragma once
 
 #include "attn_common.h"

@@ -31,12 +31,16 @@ struct Args {
   }
 };
 
+constexpr int kWorkgroups = 256;  // one (four waves, most of the LDS) a CU
+
 // What a piece costs whatever its length (queries in, output out, latencies),
-// in steps of its kernel. With two workgroups a tile: 8 takes 75.2 us for 48
-// sequences of up to 5003 tokens and 128 rows and 93.6 for 19 of up to 6007 and
-// 384 rows in fp8; 4 takes 90 and 100, 12 takes 82 and 107.
+// in steps of its kernel. With two workgroups a tile: 8 takes 72.4 us for 48
+// sequences of up to 5003 tokens and 128 rows and 92.2 for 19 of up to 6007 and
+// 384 rows in fp8; 4 takes 84.8 and 100.5, 10 takes 74.9 and 93.8. Waves of 16
+// rows: 3 takes 52.2 and 33.7 us for 48 sequences of 4000 tokens and 16 rows and
+// of 1000 and 64; 1 takes 53.9 and 37.2.
 template <int MR, int SPLIT>
-constexpr int kFixed = MR == 32 ? (SPLIT == 2 ? 8 : 10) : 2;
+constexpr int kFixed = MR == 32 ? (SPLIT == 2 ? 8 : 10) : 3;
 
 // Rows of a tile and tokens of a step. Up to 16 (32, 64) rows a sequence fill
 // one (two, four) waves of 16 rows, and the other waves of a workgroup take
@@ -46,11 +50,11 @@ constexpr int kFixed = MR == 32 ? (SPLIT == 2 ? 8 : 10) : 2;
 // a piece reads of queries and writes of partial sums, but copy the cache twice
 // to LDS (the second time from the XCD's L2) and cannot overlap a tile's
 // softmax with the next one's scores: they win where sequences are cut into
-// pieces. 128 heads over a bf16 cache, us, two workgroups against one: 16
-// sequences of 4096 tokens 49 / 72, 48 of 2048 63 / 79, 128 of 4096 192 / 205,
-// 192 of 1024 and of 4096 113 / 125 and 308 / 298, 256 of 300 and of 8192
-// 66 / 58 and 686 / 615. fp8: 16 of 4096 55 / 71, 192 of 4096 334 / 331, 256 of
-// 2048 233 / 219.
+// pieces, up to half as many tiles as CUs. 128 heads over a bf16 cache, us, two
+// workgroups against one: 16 sequences of 4096 tokens 45 / 64, 48 of 2048 56 /
+// 64, 128 of 4096 203 / 199, 160 of 1024 and of 4096 91 / 98 and 270 / 253, 256
+// of 300 and of 8192 63 / 50 and 690 / 609. fp8: 16 of 4096 52 / 65, 128 of 4096
+// 209 / 220, 192 of 4096 321 / 315, 256 of 300 71 / 52.
 struct Shape {
   int mr, wr, split;  // rows of a wave, waves over rows, workgroups over rows
   int tile_rows() const { return mr * wr * split; }
@@ -60,10 +64,8 @@ inline Shape shape_for(int64_t batch, int64_t rows) {
   if (rows <= 16) return {16, 1, 1};
   if (rows <= 32) return {16, 2, 1};
   if (rows <= 64) return {16, 4, 1};
-  return batch * ((rows + 127) / 128) <= 192 ? Shape{32, 2, 2} : Shape{32, 4, 1};
+  return batch * ((rows + 127) / 128) <= kWorkgroups / 2 ? Shape{32, 2, 2} : Shape{32, 4, 1};
 }
-
-constexpr int kWorkgroups = 256;  // one (four waves, most of the LDS) a CU
 
 // Whether each row tile is cut by itself: a workgroup then never has parts of
 // two (it would work on them one after the other), and at most an eighth of the

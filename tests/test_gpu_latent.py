@@ -167,13 +167,13 @@ def test_decode_many_sequences(dev, heads):
 @pytest.mark.parametrize("dtype,dl,dr,page", [(BF16, 512, 64, 16), (FP16, 512, 64, 1), (BF16, 256, 32, 1),
                                               (FP16, 256, 32, 48)])
 def test_decode_many_sequences_of_many_rows(dev, dtype, dl, dr, page, fp8):
-    # from 193 tiles of 128 rows on one workgroup takes a tile; page 1: more pages than are kept at hand
+    # many tiles of 128 rows: one workgroup takes a tile; page 1: more pages than are kept at hand
     lens = [0, 1] + [97 * i % 300 for i in range(195)] + [601, 333, 64]
     decode_case(dev, lens, 1, 128, page, dtype, fp8, dl, dr, seed=dl + page, q_std=4.0 if page == 1 else 1.0)
 
 
 @pytest.mark.parametrize("fp8", [False, True])
-@pytest.mark.parametrize("batch,new,heads", [(3, 1, 65), (3, 2, 65), (192, 1, 66), (97, 2, 100), (1, 3, 200)])
+@pytest.mark.parametrize("batch,new,heads", [(3, 1, 65), (3, 2, 65), (128, 1, 66), (129, 1, 66), (97, 2, 100), (1, 3, 200)])
 def test_decode_rows_of_two_workgroups(dev, batch, new, heads, fp8):
     # the last tile's second workgroup has one row, a few rows, none
     decode_case(dev, [(53 * i + 70) % 260 for i in range(batch)], new, heads, 32, fp8=fp8, seed=batch)
