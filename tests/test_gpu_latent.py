@@ -413,6 +413,67 @@ def test_prefill_long(dev):
     prefill_case(dev, [(2500, 4100)], 2, seed=5)
 
 
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("widths", [(128, 64, 128), (64, 32, 64)])
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_prefill_many_rows(dev, dtype, widths, causal):
+    # past 65536 rows and heads tiles have 256 rows: whole ones, ends of up to 128 and of more, keys before and missing
+    pairs = [(257, 300), (129, 400), (128, 128), (256, 256), (1, 70), (30, 0), (0, 7), (385, 385), (20, 10)]
+    prefill_case(dev, pairs, 56, dtype=dtype, widths=widths, causal=causal, seed=7, spare=3, strided=True)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_prefill_many_rows_sharp_scores(dev, dtype):
+    prefill_case(dev, [(900, 1000)], 74, dtype=dtype, q_std=8.0, scale=0.5, seed=8)
+
+
+@pytest.mark.parametrize("n", [62, 63, 64, 65])
+@pytest.mark.parametrize("heads", [1, 64])
+def test_prefill_sequences_of_a_wave(dev, n, heads):
+    # up to 63 sequences a wave finds its tile alone; 64 heads: tiles of 256 rows
+    prefill_case(dev, [((37 * i) % 35 + (0 if heads == 1 else 2), (37 * i) % 35 + i % 6) for i in range(n)], heads,
+                 seed=n)
+
+
+def test_scales_of_zero_and_below(dev):
+    prefill_case(dev, [(100, 130), (3, 3)], 2, scale=0.0, seed=1)
+    decode_case(dev, [300, 1, 0], 2, 5, 16, scale=0.0, seed=1)
+    decode_case(dev, [300, 1, 0], 1, 100, 16, fp8=True, scale=0.0, seed=1)
+    g = torch.Generator(device=dev).manual_seed(3)
+    q, k, v, kr = (torch.randn(s, generator=g, device=dev).bfloat16()
+                   for s in ((90, 3, 192), (90, 3, 128), (90, 3, 128), (90, 64)))
+    cu = torch.tensor([0, 90], dtype=torch.int32, device=dev)
+    a, b = (pca.latent_prefill(x, k, kr, v, cu, cu, softmax_scale=s) for x, s in ((q, -0.07), (-q, 0.07)))
+    assert torch.equal(a, b)
+    cache = pca.LatentCache.empty(4, 64, device=dev)
+    cache.latent.normal_(generator=g)
+    cache.rope.normal_(generator=g)
+    table, lens = torch.arange(4, dtype=torch.int32, device=dev)[None], torch.tensor([222], dtype=torch.int32, device=dev)
+    for heads in (16, 128):
+        ql, qr = (torch.randn((1, 1, heads, n), generator=g, device=dev).bfloat16() for n in (512, 64))
+        a = pca.latent_decode(ql, qr, cache, table, lens, softmax_scale=-0.07)
+        assert torch.equal(a, pca.latent_decode(-ql, -qr, cache, table, lens, softmax_scale=0.07))
+
+
+def test_rows_off_their_alignment_are_refused(dev):
+    cu = torch.tensor([0, 8], dtype=torch.int32, device=dev)
+    q = torch.zeros((8, 2, 196), device=dev).bfloat16()[..., 4:]
+    k, kr = torch.zeros((8, 2, 128), device=dev).bfloat16(), torch.zeros((8, 64), device=dev).bfloat16()
+    with pytest.raises(ValueError, match="q"):
+        pca.latent_prefill(q, k, kr, k, cu, cu)
+    q = q.contiguous()
+    with pytest.raises(ValueError, match="v"):
+        pca.latent_prefill(q, k, kr, torch.zeros((8, 2, 132), device=dev).bfloat16()[..., :128], cu, cu)
+    cache = pca.LatentCache.empty(2, 16, device=dev)
+    table, lens = torch.zeros((1, 2), dtype=torch.int32, device=dev), torch.ones(1, dtype=torch.int32, device=dev)
+    ql, qr = torch.zeros((1, 1, 2, 516), device=dev).bfloat16(), torch.zeros((1, 1, 2, 64), device=dev).bfloat16()
+    with pytest.raises(ValueError, match="q_latent"):
+        pca.latent_decode(ql[..., 4:], qr, cache, table, lens, softmax_scale=1.0)
+    odd = pca.LatentCache(torch.zeros((2, 16, 516), device=dev).bfloat16()[..., :512], cache.rope)
+    with pytest.raises(ValueError, match="latent"):
+        pca.latent_decode(ql[..., :512].contiguous(), qr, odd, table, lens, softmax_scale=1.0)
+
+
 def test_prefill_nothing(dev):
     q = torch.ones((5, 2, 192), device=dev).bfloat16()
     k = torch.ones((0, 2, 128), device=dev).bfloat16()
