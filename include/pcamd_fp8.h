@@ -358,7 +358,9 @@ int pcamd_latent_append(const void *latent, const void *rope, int dtype,
  * head); token t of sequence b is place t % page_size of page table[b, t /
  * page_size]; lens[batch] counts a sequence's tokens. Lengths are cut to
  * max_pages * page_size and page numbers to the pool. latent_dim and rope_dim
- * are 512 and 64, or 256 and 32. The workspace (16-byte aligned, contents
+ * are 512 and 64, or 256 and 32. Rows of queries and cache are 16-byte aligned,
+ * of out 8-byte; a cache stride may be up to 2^31 - 1 elements (offsets are 64
+ * bits wide). The workspace (16-byte aligned, contents
  * ignored and overwritten) has at least pcamd_latent_decode_workspace() bytes;
  * a negative result of that call is a status.
  */
@@ -388,7 +390,9 @@ int pcamd_latent_decode(const void *q_latent, const void *q_rope, int dtype,
  * the first nk - nq + i + 1 keys of nk. out [total_q, heads, v_dim], lse
  * [total_q, heads] (may be NULL); queries that see no key, and those behind
  * the last sequence, give zeros and -inf. nope_dim, rope_dim and v_dim are
- * 128, 64 and 128, or 64, 32 and 64.
+ * 128, 64 and 128, or 64, 32 and 64. Rows of q, k_nope, k_rope and v are 16-byte
+ * aligned, of out 8-byte; up to 2^30 tokens, and up to 2^30 elements from one
+ * key's (value's) token to the next.
  */
 int pcamd_latent_prefill(const void *q, const void *k_nope, const void *k_rope,
                          const void *v, int dtype, int64_t total_q,

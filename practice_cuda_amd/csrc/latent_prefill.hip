@@ -13,9 +13,9 @@
 // Bound by the matrix products: 2 (DN + DR + DV) operations for each seen pair
 // and head, beside an exponential and a rounding to 16 bits a pair, which the
 // vector units do while the products run. 8192 tokens, 32 heads, causal, bf16:
-// 688 GFLOP in 671 us, 1.03 PFLOP/s, where an 8192^3 product of the library
+// 688 GFLOP in 647 us, 1.06 PFLOP/s, where an 8192^3 product of the library
 // reaches 1.25; 6 prompts of up to 1111 tokens behind up to 700 cached ones, 128
-// heads: 310 GFLOP in 475 us (their ends fill tiles in part). Under this load
+// heads: 310 GFLOP in 467 us (their ends fill tiles in part). Under this load
 // the clock falls to about 1.6 GHz, so what remains is power.
 #include <hip/hip_runtime.h>
 
