@@ -8,15 +8,18 @@
 //
 // One workgroup holds NR x 128 query rows of one head, NR x 32 a wave, and
 // walks over the keys they see in steps of 32 with a running maximum and sum.
-// With NR = 2 every operand read from LDS serves two matrix products.
+// With NR = 2 every operand read from LDS serves two matrix products; with NR =
+// 1 two workgroups share a CU, and one's queries, first tiles and output pass
+// beside the other's products.
 //
 // Bound by the matrix products: 2 (DN + DR + DV) operations for each seen pair
 // and head, beside an exponential and a rounding to 16 bits a pair, which the
 // vector units do while the products run. 8192 tokens, 32 heads, causal, bf16:
-// 688 GFLOP in 647 us, 1.06 PFLOP/s, where an 8192^3 product of the library
+// 688 GFLOP in 646 us, 1.06 PFLOP/s, where an 8192^3 product of the library
 // reaches 1.25; 6 prompts of up to 1111 tokens behind up to 700 cached ones, 128
-// heads: 310 GFLOP in 467 us (their ends fill tiles in part). Under this load
-// the clock falls to about 1.6 GHz, so what remains is power.
+// heads: 310 GFLOP in 411 us (their ends fill tiles in part; a workgroup a CU
+// took 467). Under this load the clock falls to about 1.6 GHz, so what remains
+// is power.
 #include <hip/hip_runtime.h>
 
 #include <atomic>
@@ -84,15 +87,19 @@ struct Kernel {
   // its rotary part (one block, half filled where it is 64 bytes), the value.
   static constexpr int KB = DN / 64, VB = DV / 64, CR = DR / 8;
   static constexpr int BLOCK = BN * 128, VALUES = (KB + 1) * BLOCK, TILE = (KB + 1 + VB) * BLOCK;
-  static constexpr int NB = 6;  // tiles: the one in use, the next, and four on their way
+  // Tiles: the one in use, the next, and others on their way. With 128 rows a
+  // workgroup has half of the registers and takes half of the LDS.
+  static constexpr int HALF = 163840 / 2, FIT = HALF / TILE;
+  static constexpr int NB = NR == 1 && FIT < 6 ? FIT : 6;
   // In the ring's place: queries [block][row][128 bytes] first, behind the tiles
   // that are copied meanwhile; output rows last
   static constexpr int QROWS = NR * 32, QBLOCK = QROWS * 128, QUERIES = (KB + 1) * QBLOCK;
-  static constexpr int EARLY = 2, QAT = EARLY * TILE;
+  static constexpr int EARLY = NB < 6 ? 1 : 2, QAT = EARLY * TILE;
   static constexpr int OPITCH = DV * 2 + 16, OUT = QROWS * OPITCH;
   static constexpr int max3(int a, int b, int c) { return a > b ? (a > c ? a : c) : (b > c ? b : c); }
   static constexpr int BODY = max3(NB * TILE, QAT + 4 * QUERIES, 4 * OUT);
-  static constexpr int LDS = BODY + 64;
+  static constexpr int LDS = BODY;
+  static_assert(NR > 1 || LDS <= HALF, "two workgroups share a CU's LDS");
   static constexpr int COPIES = KB + 1 + VB;  // of a wave for a tile: 8 keys x 128 bytes each
 
   // a wave's share of a tile's copies: 8 of its keys
@@ -133,14 +140,15 @@ struct Kernel {
   };
 
   static PCAMD_DEV void run(const Args& a, uint8_t* lds) {
-    int* wave_total = reinterpret_cast<int*>(lds + BODY);
+    int* wave_total = reinterpret_cast<int*>(lds);
     int* found = wave_total + NT / 64;
     const int tid = threadIdx.x, lane = tid % 64, wave = __builtin_amdgcn_readfirstlane(tid / 64);
     // Workgroups go round the eight XCDs: each gets a run of neighbouring heads,
     // one head's tiles after the other's, so that its L2 holds the keys in use
     // and they lie in all of its channels.
     const int per = gridDim.x / 8, item = blockIdx.x % 8 * per + blockIdx.x / 8;
-    const int head = item / a.max_tiles, want = item - head * a.max_tiles;
+    const int head = item / a.max_tiles;
+    int want = item - head * a.max_tiles;
     if (head >= a.heads) return;
 
     // ---- the tile's sequence, found in a running count of tiles over the
@@ -157,6 +165,10 @@ struct Kernel {
         const int o = __shfl_up(inc, d, 64);
         if (lane >= d) inc += o;
       }
+      // Every second head, counted from the last, the other way round: workgroups
+      // that share a CU then have long rows and short ones.
+      const int total = __builtin_amdgcn_readlane(inc, 63);
+      if (((a.heads - 1 - head) & 1) && want < total) want = total - 1 - want;
       const uint64_t here = __ballot(want >= inc - mine && want < inc);
       if (!here) return;
       const int from = __builtin_ctzll(here);
@@ -196,8 +208,9 @@ struct Kernel {
         if (found[0] >= 0) break;
       }
       if (found[0] < 0) return;
-      t = sequence(a, found[0]);
-      row0 = found[1] * BM;
+      t = sequence(a, __builtin_amdgcn_readfirstlane(found[0]));
+      row0 = __builtin_amdgcn_readfirstlane(found[1]) * BM;
+      __syncthreads();  // the queries take this place
     }
     // a tile of at most 128 rows, the rest of a sequence, goes to all four waves too
     if (NR == 2 && t.qn - row0 <= 128) Kernel<DT, DN, DR, DV, 1>::rows(a, lds, t, row0, head);
@@ -302,7 +315,7 @@ struct Kernel {
       const uint2 z = read_tr4(lds + ((tile + lane_v) ^ (x ^ 16)) + at + 8 * 128);
       return make_uint4(y.x, y.y, z.x, z.y);
     };
-    constexpr int DA = KS < 8 ? KS : 8;                      // key operands read ahead
+    constexpr int DA = KS < (NR == 1 ? 6 : 8) ? KS : (NR == 1 ? 6 : 8);                      // key operands read ahead
     constexpr int NP = 2 * OB, DVA = NP < 6 ? NP : 6;        // value operands (contraction step n / OB, block n % OB), ahead
     uint4 val[DVA];
     f32x16 c[NR];
@@ -535,7 +548,7 @@ struct Kernel {
 };
 
 template <int DT, int DN, int DR, int DV, int NR>
-__global__ __launch_bounds__(NT, 1) void prefill_kernel(Args a) {
+__global__ __launch_bounds__(NT, NR == 1 ? 2 : 1) void prefill_kernel(Args a) {
   // all of the kernel's LDS, so that it starts at address 0: copies and tile addresses count on it
   extern __shared__ __align__(16) uint8_t lds[];
   Kernel<DT, DN, DR, DV, NR>::run(a, lds);
@@ -558,10 +571,11 @@ int launch_rows(Args a, hipStream_t st) {
 
 template <int DT, int DN, int DR, int DV>
 int launch(const Args& a, hipStream_t st) {
-  // 128-row tiles where 256-row ones would leave CUs idle. Rows x heads, causal, bf16, us with 128 and 256 rows:
-  // 2048 x 16 48 / 74, 512 x 128 35 / 55, 4096 x 16 103 / 134; 768 x 128 72 / 65, 8192 x 16 364 / 330, 16384 x 16
-  // 1379 / 1213; 16 sequences of 512 69 / 64
-  return a.total_q * a.heads <= 256 * 256 ? launch_rows<DT, DN, DR, DV, 1>(a, st) : launch_rows<DT, DN, DR, DV, 2>(a, st);
+  // 256-row tiles for prompts that are long on average. Tokens x heads, causal, bf16, us with 128 and 256 rows: 4096 x 16
+  // 103 / 133, 8192 x 16 337 / 335, 8192 x 32 653 / 644, 16384 x 16 1278 / 1229, 32768 x 16 5177 / 4734; 4096 x 128 731 /
+  // 732, 4 sequences of 10 to 4000 tokens, 32 heads 251 / 271, 16 of 512, 16 heads 49 / 64, 40 of 300, 128 heads 470 / 807
+  const bool many = a.total_q >= int64_t{8192} * a.sequences && a.total_q * a.heads >= 8192 * 16;
+  return many ? launch_rows<DT, DN, DR, DV, 2>(a, st) : launch_rows<DT, DN, DR, DV, 1>(a, st);
 }
 
 }  // namespace prefill

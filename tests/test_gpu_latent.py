@@ -427,6 +427,25 @@ def test_prefill_many_rows_sharp_scores(dev, dtype):
     prefill_case(dev, [(900, 1000)], 74, dtype=dtype, q_std=8.0, scale=0.5, seed=8)
 
 
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("widths", [(128, 64, 128), (64, 32, 64)])
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_prefill_tiles_of_256_rows(dev, dtype, widths, causal):
+    # 8192 rows a sequence and more on average, most of them behind the last sequence
+    pairs = [(257, 300), (129, 400), (128, 128), (256, 256), (1, 70), (30, 0), (0, 7), (385, 385), (900, 1100)]
+    prefill_case(dev, pairs, 2, dtype=dtype, widths=widths, causal=causal, seed=9, spare=9 * 8192, strided=True)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_prefill_tiles_of_256_rows_sharp_scores(dev, dtype):
+    prefill_case(dev, [(900, 1000)], 2, dtype=dtype, q_std=8.0, scale=0.5, seed=8, spare=65536)
+
+
+@pytest.mark.parametrize("n", [63, 64, 65])
+def test_prefill_tiles_of_256_rows_in_many_sequences(dev, n):
+    prefill_case(dev, [((37 * i) % 350, (37 * i) % 350 + i % 6) for i in range(n)], 1, seed=n, spare=n * 8192)
+
+
 @pytest.mark.parametrize("n", [62, 63, 64, 65])
 @pytest.mark.parametrize("heads", [1, 64])
 def test_prefill_sequences_of_a_wave(dev, n, heads):
