@@ -315,7 +315,7 @@ struct Kernel {
       const uint2 z = read_tr4(lds + ((tile + lane_v) ^ (x ^ 16)) + at + 8 * 128);
       return make_uint4(y.x, y.y, z.x, z.y);
     };
-    constexpr int DA = KS < (NR == 1 ? 6 : 8) ? KS : (NR == 1 ? 6 : 8);                      // key operands read ahead
+    constexpr int DA = KS < 8 ? KS : 8;                      // key operands read ahead
     constexpr int NP = 2 * OB, DVA = NP < 6 ? NP : 6;        // value operands (contraction step n / OB, block n % OB), ahead
     uint4 val[DVA];
     f32x16 c[NR];
