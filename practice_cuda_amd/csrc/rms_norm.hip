@@ -142,9 +142,11 @@ PCAMD_DEV void store_codes(uint8_t* p, int64_t valid, uint2 c) {
   }
 }
 
-PCAMD_DEV float wave_sum(float v) {
+// over groups of LANES neighbouring lanes
+template <int LANES>
+PCAMD_DEV float lanes_sum(float v) {
 #pragma unroll
-  for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d, 64);
+  for (int d = LANES / 2; d > 0; d >>= 1) v += __shfl_xor(v, d, 64);
   return v;
 }
 
@@ -202,13 +204,13 @@ __global__ __launch_bounds__(TEAM < 256 ? 256 : TEAM) void norm_quant_kernel(Nor
         for (int i = 0; i < 8; ++i) s += v[0][i] * v[0][i];
       }
     }
-    s = wave_sum(s);
+    s = lanes_sum<(TEAM < 64 ? TEAM : 64)>(s);
     if constexpr (TEAM > 64) {
       if (threadIdx.x % 64 == 0) sums[parity][threadIdx.x / 64] = s;
       __syncthreads();  // the other parity's sums may still be read: two buffers, one barrier a row
       s = 0.0f;
 #pragma unroll
-      for (int w = 0; w < TEAM / 64; ++w) s += sums[parity][w];
+      for (int w = 0; w < TEAM / 64; ++w) s += sums[parity][threadIdx.x / TEAM * (TEAM / 64) + w];
     }
     const float inv = rsqrtf(s / static_cast<float>(a.n) + a.norm_eps);
 
@@ -262,7 +264,7 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
       float s = 0.0f;
 #pragma unroll
       for (int i = 0; i < 8; ++i) s += v[i] * v[i];
-      inv = rsqrtf(wave_sum(s) / static_cast<float>(a.dl) + a.norm_eps);
+      inv = rsqrtf(lanes_sum<64>(s) / static_cast<float>(a.dl) + a.norm_eps);
       float w[8];
       load8_as(a.w_dtype, a.weight, 8 * lane, valid > 0 ? valid : 0, w);
 #pragma unroll
@@ -289,7 +291,7 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
 
 template <int DT, int FMT>
 int launch_norm(const NormArgs& a, hipStream_t st) {
-  // the smallest team that holds a row; workgroups beyond the cap take further rows
+  // workgroups beyond the cap take further rows
   auto go = [&](auto team, auto nv) {
     constexpr int TEAM = decltype(team)::value, NV = decltype(nv)::value;
     constexpr int WG = TEAM < 256 ? 256 : TEAM;
@@ -299,11 +301,22 @@ int launch_norm(const NormArgs& a, hipStream_t st) {
     return check_launch("norm_quant_kernel");
   };
   using std::integral_constant;
-  if (a.n <= 512) return go(integral_constant<int, 64>{}, integral_constant<int, 1>{});
-  if (a.n <= 2048) return go(integral_constant<int, 64>{}, integral_constant<int, 4>{});
+  // A team that a row fills, with two chunks a lane and more where it can: the loads of both are in flight at once. 29 million
+  // values (16384 rows at most), bf16 with a residual, us, the team taken and the ones beside it:
+  //   64 columns 16 x 1 5.1, 64 x 1 11.0; 129 16 x 2 7.8, 32 x 1 10.0; 300 32 x 2 16.0, 64 x 1 20.0; 1024 64 x 2 29.2, 128 x 1
+  //   30.9, 64 x 4 42.2; 1031 64 x 3 49.1, 128 x 2 54.1; 2000 128 x 2 50.0, 64 x 4 59.2; 4096 256 x 2 47.3, 512 x 1 48.3, 128 x 4
+  //   56.0; 5120 256 x 3 49.7, 512 x 2 57.0; 7168 512 x 2 51.1, 256 x 4 55.0, 1024 x 1 65.2; 10007 512 x 3 73.5, 1024 x 2 96.2;
+  //   16384 512 x 4 53.9, 1024 x 2 54.0
+  if (a.n <= 128) return go(integral_constant<int, 16>{}, integral_constant<int, 1>{});
+  if (a.n <= 256) return go(integral_constant<int, 16>{}, integral_constant<int, 2>{});
+  if (a.n <= 512) return go(integral_constant<int, 32>{}, integral_constant<int, 2>{});
+  if (a.n <= 1024) return go(integral_constant<int, 64>{}, integral_constant<int, 2>{});
+  if (a.n <= 1536) return go(integral_constant<int, 64>{}, integral_constant<int, 3>{});
+  if (a.n <= 2048) return go(integral_constant<int, 128>{}, integral_constant<int, 2>{});
   if (a.n <= 4096) return go(integral_constant<int, 256>{}, integral_constant<int, 2>{});
-  // 4096 x 7168 bf16 with a residual: 512 lanes 50.3 us, 256 lanes (4 chunks each) 54.7, 1024 (1 each) 62.6
+  if (a.n <= 6144) return go(integral_constant<int, 256>{}, integral_constant<int, 3>{});
   if (a.n <= 8192) return go(integral_constant<int, 512>{}, integral_constant<int, 2>{});
+  if (a.n <= 12288) return go(integral_constant<int, 512>{}, integral_constant<int, 3>{});
   if (a.n <= 16384) return go(integral_constant<int, 512>{}, integral_constant<int, 4>{});
   if (a.n <= 65536) return go(integral_constant<int, 1024>{}, integral_constant<int, 8>{});
   return go(integral_constant<int, 1024>{}, integral_constant<int, 0>{});

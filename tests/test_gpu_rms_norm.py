@@ -69,6 +69,22 @@ def test_rows(dev, rows, n):
     check(x, w, r)
 
 
+@pytest.mark.parametrize("n", [64, 100, 256, 257, 300, 511, 768, 1024, 1025, 1536, 1537, 3000, 5003, 6144, 6145, 8192,
+                               8193, 12288, 12289])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_row_lengths_around_the_teams(dev, n, dtype):
+    x, w, r = tensors(dev, (37, n), dtype, True, seed=n)
+    check(x, w, r)
+    check(x, w)
+
+
+@pytest.mark.parametrize("rows", [1, 2, 7, 15, 16, 17, 31, 33, 1000])
+@pytest.mark.parametrize("n", [1, 64, 128, 200, 400, 2000])
+def test_rows_of_small_teams(dev, rows, n):
+    x, w, r = tensors(dev, (rows, n), torch.bfloat16, True, seed=rows)
+    check(x, w, r)
+
+
 def test_batches_strides_and_alignment(dev):
     g = torch.Generator(device=dev).manual_seed(3)
     buf = torch.randn((4, 9, 1301), generator=g, device=dev).bfloat16()
