@@ -41,9 +41,11 @@ PCAMD_DEV void unrolled(F f) {
   unrolled(f, std::make_integer_sequence<int, N>{});
 }
 
-// Scores are kept times log2(e). The running maximum starts at a finite value
-// below every score that is told apart from -inf, so that a row that has seen
-// nothing (all scores -inf) gets weights exp2(-inf) = 0 and no NaN.
+// The running maximum (of scores times scale and log2(e) in the decode kernels,
+// of bare products q . k in the prefill kernels) starts at a finite value below
+// every score that is told apart from -inf, so that a row that has seen nothing
+// (all scores -inf) gets weights exp2(-inf) = 0 and no NaN. Times a scale above
+// 0.78 it is not finite any more: the prefill kernels keep it out of the weights.
 constexpr float kNoMax = -3.0e38f;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;

@@ -401,7 +401,9 @@ struct Kernel {
         for (int u = 0; u < NR; ++u) {
           const float to = fmaxf(m[u], top[u]), alpha = __builtin_amdgcn_exp2f((m[u] - to) * a.scale_log2);
           m[u] = to;
-          nm[u] = -to * a.scale_log2;
+          // A row that has seen nothing keeps a factor of zero: kNoMax itself times a scale_log2 above 1.13 is not
+          // finite, and its scores of -inf would become NaN.
+          nm[u] = to == kNoMax ? 0.0f : -to * a.scale_log2;
           l[u] *= alpha;
 #pragma unroll
           for (int j = 0; j < OB; ++j) {
