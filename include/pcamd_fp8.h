@@ -388,11 +388,11 @@ int pcamd_latent_decode(const void *q_latent, const void *q_rope, int dtype,
  * the queries cu_q[i] .. cu_q[i + 1] - 1 and the keys cu_k[i] .. cu_k[i + 1] -
  * 1 (offsets beyond the tensors are cut to them). causal: query i of nq sees
  * the first nk - nq + i + 1 keys of nk. out [total_q, heads, v_dim], lse
- * [total_q, heads] (may be NULL); queries that see no key, and those behind
- * the last sequence, give zeros and -inf. nope_dim, rope_dim and v_dim are
- * 128, 64 and 128, or 64, 32 and 64. Rows of q, k_nope, k_rope and v are 16-byte
- * aligned, of out 8-byte; up to 2^30 tokens, and up to 2^30 elements from one
- * key's (value's) token to the next.
+ * [total_q, heads] (may be NULL); queries that see no key, and those ahead of
+ * the first sequence or behind the last, give zeros and -inf. nope_dim,
+ * rope_dim and v_dim are 128, 64 and 128, or 64, 32 and 64. Rows of q, k_nope,
+ * k_rope and v are 16-byte aligned, of out 8-byte; up to 2^30 tokens, and up to
+ * 2^30 elements from one key's (value's) token to the next.
  */
 int pcamd_latent_prefill(const void *q, const void *k_nope, const void *k_rope,
                          const void *v, int dtype, int64_t total_q,

@@ -52,20 +52,26 @@ struct Args {
 struct Tile {
   int64_t q0, k0;  // first token of the sequence's queries and keys (below 2^31)
   int qn, kn;
+  int ahead, gap;  // queries from `ahead` on lie `gap` tokens further on
+  PCAMD_DEV int query(int row) const { return row + (row >= ahead ? gap : 0); }  // from q0 on
 };
 
 PCAMD_DEV int64_t clamp64(int64_t v, int64_t lo, int64_t hi) { return v < lo ? lo : v > hi ? hi : v; }
 
 // Sequence i: its queries and keys, within the tensors whatever the offsets
-// say. "Sequence" n (past the last) is the tokens behind the last one, which
-// see no key and get zeros.
+// say. "Sequence" n (past the last) is the tokens ahead of the first one and
+// behind the last, which see no key and get zeros.
 PCAMD_DEV Tile sequence(const Args& a, int i) {
   Tile t;
-  t.q0 = clamp64(a.cu_q[i], 0, a.total_q);
-  const int64_t q1 = i < a.sequences ? clamp64(a.cu_q[i + 1], t.q0, a.total_q) : a.total_q;
-  t.qn = static_cast<int>(q1 - t.q0);
+  const bool own = i < a.sequences;
+  const int64_t q0 = clamp64(a.cu_q[own ? i : 0], 0, a.total_q), q1 = clamp64(a.cu_q[own ? i + 1 : i], q0, a.total_q);
+  const int n = static_cast<int>(q1 - q0);
+  t.q0 = own ? q0 : 0;
+  t.qn = own ? n : static_cast<int>(a.total_q) - n;
+  t.ahead = own ? 0 : static_cast<int>(q0);
+  t.gap = own ? 0 : n;
   t.k0 = t.kn = 0;
-  if (i < a.sequences) {
+  if (own) {
     t.k0 = clamp64(a.cu_k[i], 0, a.total_k);
     t.kn = static_cast<int>(clamp64(a.cu_k[i + 1], t.k0, a.total_k) - t.k0);
   }
@@ -177,6 +183,8 @@ struct Kernel {
       t.k0 = of(static_cast<int>(own.k0));
       t.qn = of(own.qn);
       t.kn = of(own.kn);
+      t.ahead = of(own.ahead);
+      t.gap = of(own.gap);
       row0 = (of(inc) - 1 - want) * BM;
     } else {
       if (tid == 0) found[0] = -1;
@@ -527,7 +535,7 @@ struct Kernel {
       const float sum = row_sum<32>(l[u]);
       const float inv = sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : NAN;
       if (a.lse && h == 0 && row[u] < t.qn)
-        a.lse[(t.q0 + row[u]) * a.slt + head * a.slh] =
+        a.lse[(t.q0 + t.query(row[u])) * a.slt + head * a.slh] =
             sum == 0.0f ? -INFINITY : (m[u] * a.scale_log2 + log2f(sum)) * kLn2;
 #pragma unroll
       for (int j = 0; j < OB; ++j)
@@ -544,7 +552,7 @@ struct Kernel {
     for (int i = lane; i < QROWS * PER; i += 64) {
       const int r = i / PER, d = i % PER, to = row0 + wave * QROWS + r;
       const uint2 x = *reinterpret_cast<const uint2*>(lds + wave * OUT + r * OPITCH + 8 * d);
-      if (to < t.qn) *reinterpret_cast<uint2*>(out + to * a.sot + 4 * d) = x;
+      if (to < t.qn) *reinterpret_cast<uint2*>(out + t.query(to) * a.sot + 4 * d) = x;
     }
   }
 };

@@ -288,10 +288,10 @@ def hip_latent_prefill(
     cu_q, cu_k: int32 [n + 1], the sequences' first tokens and the end of the
     last one. causal: query i of a sequence with nq queries and nk keys sees
     its first nk - nq + i + 1 keys, so a chunk may follow keys of earlier
-    chunks. Rows that see no key, and queries behind the last sequence, give
-    zeros and a log-sum of -inf. softmax_scale: default (key + rotary) ** -0.5.
-    A NaN or infinity in a value reaches the queries that see it and may reach
-    up to 31 earlier ones of its sequence.
+    chunks. Rows that see no key, and queries ahead of the first sequence or
+    behind the last, give zeros and a log-sum of -inf. softmax_scale: default
+    (key + rotary) ** -0.5. A NaN or infinity in a value reaches the queries
+    that see it and may reach up to 31 earlier ones of its sequence.
 
     Returns out [Tq, H, value] in q's dtype and, with return_lse, float32
     [Tq, H]: the natural logarithm of the sum of exponentials."""
