@@ -197,11 +197,11 @@ PCAMD_DEV uint2 read_tr8(const uint8_t* p) {
   return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_ptr)(p)));
 }
 
-// two of four fp8 codes as 16-bit elements (exact: a scale of one)
+// two of four fp8 codes as 16-bit elements, times a power of two (exact where it is one)
 template <int DT, bool HI>
-PCAMD_DEV uint32_t widen2(uint32_t c) {
-  if constexpr (DT == kBF16) return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c, 1.0f, HI));
-  else return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(c, 1.0f, HI));
+PCAMD_DEV uint32_t widen2(uint32_t c, float unit) {
+  if constexpr (DT == kBF16) return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c, unit, HI));
+  else return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(c, unit, HI));
 }
 
 }  // namespace attn

@@ -12,6 +12,9 @@
 // codes enter the products as they are (16 bits hold them exactly); the scales
 // multiply fp32 values: the four groups' partial scores, and the weights p
 // ahead of their rounding to 16 bits, once for each group of value columns.
+// fp16 has no room for scales of any size there: a wave takes the power of two
+// out of its tile's largest scale of a group and widens the group's value codes
+// times it instead, so that the weights stay p times a scale of one to two.
 //
 // What bounds it. With up to 16 rows the cache's bytes: 48 sequences of 32768
 // tokens, 16 heads, bf16: 1.81 GB in 329 us, 5.5 TB/s. With 128 rows the
@@ -40,10 +43,15 @@ typedef uint32_t u32x4_out __attribute__((ext_vector_type(4), aligned(8)));
 // How far (log2) a score may pass the reference point of its row's weights
 // before the reference moves and the wave's sums are rescaled. Weights and sums
 // are floating point: bf16 and fp32 hold 2^40 as exactly as 1, so the first
-// tile's maximum nearly always stays the reference. fp16 ends at 2^16, and has
-// no room left where an fp8 cache's scales multiply the weights.
-template <int DT, bool FP8>
-constexpr float kSlack = DT == kF16 ? (FP8 ? 0.0f : 8.0f) : 40.0f;
+// tile's maximum nearly always stays the reference. fp16 ends at 2^16:
+// half of its room is left to an fp8 cache's scales past kTopUnit.
+template <int DT>
+constexpr float kSlack = DT == kF16 ? 8.0f : 40.0f;
+
+// fp16 over an fp8 cache: bounds of the power of two that goes from a tile's
+// scales to its value codes. Codes of up to 448 times 2^7 are finite in fp16;
+// what is lost below its smallest number, 2^-25 of a value, the output loses too.
+constexpr float kTopUnit = 128.0f, kLeastUnit = 0x1p-100f;
 
 // Registers that hold operands read ahead of their products, in operands
 template <bool FP8>
@@ -253,10 +261,12 @@ struct Kernel {
     }
   };
 
-  // 8 fp8 codes as 16-bit elements (exact)
-  static PCAMD_DEV uint4 widen8(uint2 c) {
-    return make_uint4(widen2<DT, false>(c.x), widen2<DT, true>(c.x), widen2<DT, false>(c.y), widen2<DT, true>(c.y));
+  // 8 fp8 codes as 16-bit elements, times a power of two
+  static PCAMD_DEV uint4 widen8(uint2 c, float unit = 1.0f) {
+    return make_uint4(widen2<DT, false>(c.x, unit), widen2<DT, true>(c.x, unit), widen2<DT, false>(c.y, unit),
+                      widen2<DT, true>(c.y, unit));
   }
+  static constexpr bool UNITS = FP8 && DT == kF16;  // value codes times a power of two of their tile and group
 
   // Where this lane reads in a tile. Chunks of a row lie at c ^ f(row), so
   // another chunk's place differs by an exclusive or with a constant (bits 4-6
@@ -596,6 +606,35 @@ struct Kernel {
       }
       __builtin_amdgcn_sched_barrier(0);
     };
+    // The powers of two in a tile's scales. Each lane takes one or two of them, and
+    // 16 lanes have what belongs to one group. Exponents compare as integers.
+    float unit[UNITS ? GROUPS : 1];
+    uint32_t exponent = 0;
+    auto find_unit = [&](uint32_t tile) {
+      const uint32_t* at = reinterpret_cast<const uint32_t*>(lds + tile + SCALES) + lane * (GROUPS / 2);
+      exponent = at[0] & 0x7f800000u;
+      if constexpr (GROUPS == 4) {
+        const uint32_t other = at[1] & 0x7f800000u;
+        exponent = exponent > other ? exponent : other;
+      }
+    };
+    auto set_unit = [&]() {
+      unrolled<4>([&](auto n) {  // rotations by 1, 2, 4 and 8 within 16 lanes
+        const uint32_t other = __builtin_amdgcn_update_dpp(0, exponent, 0x120 + (1 << decltype(n)::value), 0xf, 0xf, true);
+        exponent = exponent > other ? exponent : other;
+      });
+      constexpr uint32_t least = __builtin_bit_cast(uint32_t, kLeastUnit), most = __builtin_bit_cast(uint32_t, kTopUnit);
+#pragma unroll
+      for (int g = 0; g < GROUPS; ++g) {
+        uint32_t top = least;
+#pragma unroll
+        for (int i = 0; i < 4 / GROUPS; ++i) {
+          const uint32_t part = __builtin_amdgcn_readlane(exponent, 64 / GROUPS * g + 16 * i);
+          top = top > part ? top : part;
+        }
+        unit[g] = __uint_as_float(top < most ? top : most);
+      }
+    };
     float s[QUADS * 4];
     auto mask = [&](int tb) {
 #pragma unroll
@@ -608,7 +647,7 @@ struct Kernel {
       return top;
     };
     auto refer = [&](float top) {  // top: of the row
-      if (__any(top > m + kSlack<DT, FP8>)) {
+      if (__any(top > m + kSlack<DT>)) {
         const float to = fmaxf(m, top), alpha = __builtin_amdgcn_exp2f(m - to);
         m = to;
         l *= alpha;
@@ -629,11 +668,17 @@ struct Kernel {
     };
     auto weights = [&](int g, int q) {  // registers 4 q .. + 3
       float x0 = s[4 * q], x1 = s[4 * q + 1], x2 = s[4 * q + 2], x3 = s[4 * q + 3];
-      if constexpr (FP8) {
-        x0 *= fw.x * kScaleUp<DT>;
-        x1 *= fw.y * kScaleUp<DT>;
-        x2 *= fw.z * kScaleUp<DT>;
-        x3 *= fw.w * kScaleUp<DT>;
+      if constexpr (UNITS) {
+        const float per = __uint_as_float((254u << 23) - __float_as_uint(unit[g]));  // 1 / unit
+        x0 *= fw.x * per;
+        x1 *= fw.y * per;
+        x2 *= fw.z * per;
+        x3 *= fw.w * per;
+      } else if constexpr (FP8) {
+        x0 *= fw.x;
+        x1 *= fw.y;
+        x2 *= fw.z;
+        x3 *= fw.w;
       }
       p[FP8 ? g & 1 : 0][2 * q] = Elem<DT>::narrow2(x0, x1);
       p[FP8 ? g & 1 : 0][2 * q + 1] = Elem<DT>::narrow2(x2, x3);
@@ -641,7 +686,8 @@ struct Kernel {
     auto values = [&](uint32_t tile, auto beside) {  // O^T += V^T P^T
       auto operand = [&](int k) {
         const uint4 x = val[k % DV];
-        if constexpr (FP8) return widen8(make_uint2(x.x, x.y));
+        if constexpr (UNITS) return widen8(make_uint2(x.x, x.y), unit[k * GROUPS / NP]);
+        else if constexpr (FP8) return widen8(make_uint2(x.x, x.y));
         else return x;
       };
       uint4 next = operand(0);
@@ -756,6 +802,10 @@ struct Kernel {
             copies.emit_all(tile_of(i + AHEAD), wr, lane);
           }
           auto ahead = [&](int k) {
+            if constexpr (UNITS) {
+              if (k == 2) find_unit(tile);
+              if (k == 8) set_unit();
+            }
             if constexpr (MR == 16 || !FP8) {
               if (k == 1) copies.find(a, src, first_token(i + AHEAD), wr, lane);
               if (k == 6) copies.address(a, wr, lane);
@@ -830,7 +880,6 @@ struct Kernel {
       factor = __builtin_amdgcn_exp2f(m - big);
     }
     if (whole) factor *= total > 0.0f ? 1.0f / total : total == 0.0f ? 0.0f : NAN;
-    if constexpr (FP8) factor *= 1.0f / kScaleUp<DT>;
     const int64_t at = static_cast<int64_t>(slot) * TILE_ROWS + share + wr * MR;  // of its first row among the partial sums
     if (lane < MR) {
       place[ln] = live ? b * a.ob + tok_new * a.os + head * a.oh : -1;

@@ -76,10 +76,5 @@ __host__ __device__ inline bool few_tiles(int64_t tiles, int split) { return til
 template <int DT, int DL, int DR>
 int launch(const Args& a, Shape shape, bool fp8, hipStream_t st);
 
-// fp16 weights times an fp8 cache's scales (a 448th of its group's maximum)
-// would reach the subnormal numbers; bf16 has fp32's range
-template <int DT>
-constexpr float kScaleUp = DT == 2 /* PCAMD_F16 */ ? 256.0f : 1.0f;
-
 }  // namespace decode
 }  // namespace pcamd

@@ -205,6 +205,9 @@ def hip_latent_decode(
     token reaches the rows that see it and may reach the same sequence's
     earlier new tokens, which do not.
 
+    An fp8 cache's scales may have any size under bfloat16 queries, and up to
+    2^15 under float16 ones, whose attention weights are multiplied by them.
+
     Returns out [B, S, H, latent] in the queries' dtype and, with return_lse,
     float32 [B, S, H]: the natural logarithm of the sum of exponentials."""
     if q_latent.ndim != 4 or q_rope.ndim != 4 or q_latent.shape[:3] != q_rope.shape[:3]:
