@@ -357,8 +357,8 @@ int pcamd_latent_append(const void *latent, const void *rope, int dtype,
  * [batch, S, heads, rope_dim], out like q_latent (strides per batch, token and
  * head); token t of sequence b is place t % page_size of page table[b, t /
  * page_size]; lens[batch] counts a sequence's tokens. Lengths are cut to
- * max_pages * page_size and page numbers to the pool. latent_dim and rope_dim
- * are 512 and 64, or 256 and 32. Rows of queries and cache are 16-byte aligned,
+ * max_pages * page_size, at most 2^31 - 1024, and page numbers to the pool.
+ * latent_dim and rope_dim are 512 and 64, or 256 and 32. Rows of queries and cache are 16-byte aligned,
  * of out 8-byte; a cache stride may be up to 2^31 - 1 elements (offsets are 64
  * bits wide). The workspace (16-byte aligned, contents
  * ignored and overwritten) has at least pcamd_latent_decode_workspace() bytes;

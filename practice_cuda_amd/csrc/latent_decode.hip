@@ -43,6 +43,10 @@ Layout lay_out(int64_t batch, int64_t rows, int64_t latent_dim, int64_t capacity
   return d;
 }
 
+// A sequence's tokens: the kernels count them in 32 bits, and name tokens past the last one by up to a workgroup's
+// tiles on their way (four steps of 128 tokens) ahead of cutting them to it.
+constexpr int64_t kMaxTokens = (int64_t{1} << 31) - 1024;
+
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 int check_sizes(int64_t batch, int64_t new_tokens, int64_t heads, int64_t latent_dim, int64_t page_size,
@@ -53,7 +57,7 @@ int check_sizes(int64_t batch, int64_t new_tokens, int64_t heads, int64_t latent
   if (latent_dim != 512 && latent_dim != 256)
     return set_error(PCAMD_ERR_UNSUPPORTED, "latent width must be 512 or 256, got %lld", (long long)latent_dim);
   if (batch > (1 << 20) || new_tokens > (1 << 20) || heads > (1 << 20) || new_tokens * heads > (1 << 24) ||
-      max_pages > INT32_MAX / page_size ||
+      max_pages > kMaxTokens / page_size ||
       batch * ((new_tokens * heads + 15) / 16) * ((page_size * max_pages) / 32 + 32) > INT32_MAX)
     return set_error(PCAMD_ERR_UNSUPPORTED, "latent decode: too many rows or tokens a sequence");
   return PCAMD_OK;
