@@ -69,17 +69,50 @@ class LatentAttention(nn.Module):
         self.w_out = weight(1, hidden, heads * head_dim)
         freq = rope_base ** (-torch.arange(0, rope_dim, 2, device=device).float() / rope_dim)
         self.register_buffer("freq", freq, persistent=False)
-        self._fp8 = None
+        self._fp8 = self._made_from = None
 
     def quantize(self) -> "LatentAttention":
-        """The weights' fp8 forms, once: call again after changing a weight."""
+        """The weights' fp8 forms. The layer's calls make them where they are missing, or older than a weight that was
+        loaded, replaced, moved or changed in place since. Edits that torch does not count (through ``.data``, or of
+        weights made in inference mode) need a call of this. New codes take the old ones' places, so a captured graph
+        reads them."""
         both = torch.cat([self.w_key, self.w_value], 1).reshape(1, -1, self.latent_dim)
-        self._fp8 = {
+        codes = {
             "query": _quant(self.w_query, 128), "latent": _quant(self.w_latent, 128),
             "key_value": _quant(both, 128),  # [1, H * 2 head, latent], head after head
             "absorb": _quant(self.w_key.transpose(1, 2).contiguous(), 128),  # [H, latent, head]
             "value": _quant(self.w_value, 128), "out": _quant(self.w_out, 128),
         }
+        old = self._fp8
+        if old is None or any(old[n].tensor.shape != c.tensor.shape or old[n].tensor.device != c.tensor.device
+                              for n, c in codes.items()):
+            self._fp8 = codes
+        else:
+            with torch.inference_mode():  # the old ones may be inference tensors
+                for name, new in codes.items():
+                    old[name].tensor.copy_(new.tensor)
+                    old[name].dequant_scale.copy_(new.dequant_scale)
+        self._made_from = self._weights()
+        return self
+
+    def _weights(self) -> list:
+        """The weights that have codes, each with its count of changes in place (inference tensors have none)."""
+        return [(w, 0 if w.is_inference() else w._version)
+                for w in (self.w_query, self.w_latent, self.w_key, self.w_value, self.w_out)]
+
+    def _current(self) -> bool:
+        return self._fp8 is not None and all(
+            w is old and count == before for (w, count), (old, before) in zip(self._weights(), self._made_from))
+
+    def _apply(self, fn, recurse=True):
+        """Moves and type changes put other data behind the same parameters."""
+        def places():
+            return [(w.data_ptr(), w.dtype, w.device) for w, _ in self._weights()]
+
+        before = places()
+        super()._apply(fn, recurse)
+        if places() != before:
+            self._fp8 = self._made_from = None
         return self
 
     def _rotate(self, x: torch.Tensor, positions: torch.Tensor) -> torch.Tensor:
@@ -92,7 +125,7 @@ class LatentAttention(nn.Module):
 
     def _project(self, x, residual, cache, slots, positions):
         """(queries [T, H, head + rope], latents, rotary keys, residual); the tokens are in the cache."""
-        if self._fp8 is None:
+        if not self._current():
             self.quantize()
         normed, residual = hip_rms_norm_quant(x[None], self.norm, residual=residual[None], norm_eps=self.norm_eps)
         q = _product(normed, self._fp8["query"])[0].view(-1, self.heads, self.head_dim + self.rope_dim)
