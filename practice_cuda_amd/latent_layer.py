@@ -109,8 +109,10 @@ class LatentAttention(nn.Module):
         def places():
             return [(w.data_ptr(), w.dtype, w.device) for w, _ in self._weights()]
 
-        before = places()
+        before, freq = places(), self.freq
         super()._apply(fn, recurse)
+        if self.freq.dtype != freq.dtype:  # 16 bits of a frequency are not enough at any distance
+            self.freq = freq.to(self.freq.device)
         if places() != before:
             self._fp8 = self._made_from = None
         return self
