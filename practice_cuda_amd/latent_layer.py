@@ -44,8 +44,9 @@ class LatentAttention(nn.Module):
     """hidden -> heads x (head_dim + rope_dim) queries, one latent_dim + rope_dim vector a token.
 
     Widths as the attention kernels take them: latent 512, rotary 64, head 128,
-    or 256, 32 and 64. Inputs are bfloat16 [tokens, hidden]; both calls return
-    (the layer's output, the residual to add to it)."""
+    or 256, 32 and 64. Inputs are bfloat16 [tokens, hidden]; residual may be
+    None (a stack's first layer). Both calls return (the layer's output, the
+    residual to add to it)."""
 
     def __init__(self, hidden: int, heads: int, *, latent_dim: int = 512, rope_dim: int = 64, head_dim: int = 128,
                  norm_eps: float = 1e-6, rope_base: float = 10000.0, device=None) -> None:
@@ -129,13 +130,14 @@ class LatentAttention(nn.Module):
         """(queries [T, H, head + rope], latents, rotary keys, residual); the tokens are in the cache."""
         if not self._current():
             self.quantize()
-        normed, residual = hip_rms_norm_quant(x[None], self.norm, residual=residual[None], norm_eps=self.norm_eps)
+        normed, total = hip_rms_norm_quant(x[None], self.norm, residual=None if residual is None else residual[None],
+                                           norm_eps=self.norm_eps)
         q = _product(normed, self._fp8["query"])[0].view(-1, self.heads, self.head_dim + self.rope_dim)
         both = _product(normed, self._fp8["latent"])[0]
         latent, rope = both[:, :self.latent_dim], self._rotate(both[:, self.latent_dim:], positions)
         q[..., self.head_dim:] = self._rotate(q[..., self.head_dim:], positions)
         hip_latent_append(cache, latent, rope, slots, weight=self.latent_norm, norm_eps=self.norm_eps)
-        return q, latent, rope, residual[0]
+        return q, latent, rope, x if total is None else total[0]
 
     def _output(self, o: torch.Tensor) -> torch.Tensor:  # [T, H, head]
         return _product(_quant(o.reshape(1, o.shape[0], -1)), self._fp8["out"])[0]
