@@ -121,7 +121,7 @@ class LatentAttention(nn.Module):
     def _rotate(self, x: torch.Tensor, positions: torch.Tensor) -> torch.Tensor:
         """Rotary positions over the halves of the last dimension; x [T, .., rope]."""
         angle = positions.float()[:, None] * self.freq
-        shape = (x.shape[0],) + (1,) * (x.ndim - 2) + (-1,)
+        shape = (x.shape[0],) + (1,) * (x.ndim - 2) + (x.shape[-1] // 2,)
         cos, sin = angle.cos().view(shape), angle.sin().view(shape)
         a, b = x.float().chunk(2, -1)
         return torch.cat([a * cos - b * sin, a * sin + b * cos], -1).to(x.dtype)
@@ -132,7 +132,7 @@ class LatentAttention(nn.Module):
             self.quantize()
         normed, total = hip_rms_norm_quant(x[None], self.norm, residual=None if residual is None else residual[None],
                                            norm_eps=self.norm_eps)
-        q = _product(normed, self._fp8["query"])[0].view(-1, self.heads, self.head_dim + self.rope_dim)
+        q = _product(normed, self._fp8["query"])[0].view(x.shape[0], self.heads, self.head_dim + self.rope_dim)
         both = _product(normed, self._fp8["latent"])[0]
         latent, rope = both[:, :self.latent_dim], self._rotate(both[:, self.latent_dim:], positions)
         q[..., self.head_dim:] = self._rotate(q[..., self.head_dim:], positions)
@@ -140,28 +140,30 @@ class LatentAttention(nn.Module):
         return q, latent, rope, x if total is None else total[0]
 
     def _output(self, o: torch.Tensor) -> torch.Tensor:  # [T, H, head]
-        return _product(_quant(o.reshape(1, o.shape[0], -1)), self._fp8["out"])[0]
+        return _product(_quant(o.reshape(1, o.shape[0], self.heads * self.head_dim)), self._fp8["out"])[0]
 
     def prefill(self, x, residual, cache: LatentCache, slots, positions, cu_seqlens):
         """Whole prompts, packed: sequence i holds tokens cu_seqlens[i] .. cu_seqlens[i + 1] - 1 (int32)."""
         q, latent, rope, residual = self._project(x, residual, cache, slots, positions)
         c, _ = hip_rms_norm_quant(latent[None], self.latent_norm, norm_eps=self.norm_eps)
-        both = _product(c, self._fp8["key_value"])[0].view(-1, self.heads, 2 * self.head_dim)
+        both = _product(c, self._fp8["key_value"])[0].view(x.shape[0], self.heads, 2 * self.head_dim)
         o = hip_latent_prefill(q, both[..., :self.head_dim], rope, both[..., self.head_dim:], cu_seqlens, cu_seqlens,
                                softmax_scale=self.softmax_scale)
         return self._output(o), residual
 
     def decode(self, x, residual, cache: LatentCache, slots, positions, block_table, seq_lens):
         """New tokens, [B * S, hidden] for B = seq_lens.numel() sequences of S each; seq_lens counts them."""
-        batch, heads = seq_lens.shape[0], self.heads
+        tokens, batch, heads = x.shape[0], seq_lens.shape[0], self.heads
+        new = tokens // batch if batch else 0
+        if new * batch != tokens:
+            raise ValueError(f"{tokens} tokens cannot be as many for each of {batch} sequences")
         q, _, _, residual = self._project(x, residual, cache, slots, positions)
-        tokens = q.shape[0]
         nope = _quant(q[..., :self.head_dim].transpose(0, 1).contiguous())  # [H, T, head]
         q_latent = _product(nope, self._fp8["absorb"])                      # [H, T, latent]
-        shape = (heads, batch, tokens // batch, self.latent_dim)
+        shape = (heads, batch, new, self.latent_dim)
         o = torch.empty_like(q_latent)
         hip_latent_decode(q_latent.view(shape).permute(1, 2, 0, 3),
-                          q[..., self.head_dim:].view(batch, tokens // batch, heads, self.rope_dim), cache,
+                          q[..., self.head_dim:].view(batch, new, heads, self.rope_dim), cache,
                           block_table, seq_lens, softmax_scale=self.softmax_scale,
                           out=o.view(shape).permute(1, 2, 0, 3))
         values = _product(_quant(o), self._fp8["value"])                    # [H, T, head]

@@ -1,5 +1,5 @@
 """The latent-attention layer where there is nothing yet: the first layer of a
-stack, which has no residual."""
+stack, which has no residual, and batches of no tokens."""
 from __future__ import annotations
 
 import pytest
@@ -30,3 +30,36 @@ def test_first_layer(dev):
     out, residual = layer.decode(x[:1], None, *args)
     want, _ = layer.decode(x[:1], torch.zeros_like(x[:1]), *args)
     assert torch.equal(out, want) and torch.equal(residual, x[:1])
+
+
+@pytest.mark.parametrize("widths", [(512, 64, 128), (256, 32, 64)])
+@pytest.mark.parametrize("residual", [False, True])
+def test_empty_batch(dev, residual, widths):
+    latent, rope, head = widths
+    layer = LatentAttention(256, 4, latent_dim=latent, rope_dim=rope, head_dim=head, device=dev)
+    cache = pca.LatentCache.empty(3, 32, latent_dim=latent, rope_dim=rope, device=dev)
+    x = torch.empty((0, layer.hidden), device=dev).bfloat16()
+    none = torch.empty(0, dtype=torch.int64, device=dev)
+    table, lens = torch.empty((0, 3), dtype=torch.int32, device=dev), torch.empty(0, dtype=torch.int32, device=dev)
+    out, total = layer.decode(x, x if residual else None, cache, none, none, table, lens)
+    assert out.shape == total.shape == (0, layer.hidden)
+    for cu in ([0], [0, 0, 0]):
+        cu = torch.tensor(cu, dtype=torch.int32, device=dev)
+        out, total = layer.prefill(x, x if residual else None, cache, none, none, cu)
+        assert out.shape == total.shape == (0, layer.hidden)
+    # sequences without new tokens
+    lens, table = torch.tensor([3, 1], dtype=torch.int32, device=dev), torch.zeros((2, 3), dtype=torch.int32, device=dev)
+    out, total = layer.decode(x, x if residual else None, cache, none, none, table, lens)
+    assert out.shape == total.shape == (0, layer.hidden)
+
+
+def test_tokens_that_do_not_divide(dev):
+    layer = layer_of(dev)
+    cache = pca.LatentCache.empty(3, 32, device=dev)
+    x = torch.zeros((3, layer.hidden), device=dev).bfloat16()
+    at = torch.arange(3, device=dev)
+    lens, table = torch.tensor([3, 1], dtype=torch.int32, device=dev), torch.zeros((2, 3), dtype=torch.int32, device=dev)
+    before = cache.latent.zero_().clone()
+    with pytest.raises(ValueError, match="3 tokens"):
+        layer.decode(x, x, cache, at, at, table, lens)
+    assert torch.equal(cache.latent, before)
