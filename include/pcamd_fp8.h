@@ -334,9 +334,11 @@ int pcamd_rms_norm_quant(const void *x, int x_dtype, int64_t batch, int64_t m,
  * (bf16 or fp16) or as e4m3fn codes with one fp32 scale per 128 columns, and
  * rope[tokens, rope_dim] as it is. slots (slot_bytes 4 or 8: int32, int64)
  * holds page * page_size + place per token; a token whose slot is negative or
- * past pages * page_size is skipped. The cache arrays have a stride per page
- * (clp, crp, csp) and per token (clt, crt, cst), in elements. latent_dim is a
- * multiple of 128 up to 512, rope_dim one of 8 up to 512.
+ * past pages * page_size is skipped. Tokens of one slot are written in no order
+ * and may leave parts of each there; other slots are not touched. The cache
+ * arrays have a stride per page (clp, crp, csp) and per token (clt, crt, cst),
+ * in elements. latent_dim is a multiple of 128 up to 512, rope_dim one of 8 up
+ * to 512.
  */
 int pcamd_latent_append(const void *latent, const void *rope, int dtype,
                         int64_t tokens, int64_t latent_dim, int64_t rope_dim,

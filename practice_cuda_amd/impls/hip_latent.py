@@ -119,8 +119,10 @@ def hip_latent_append(
     latent [T, latent] and rope [T, rotary], bfloat16 or float16, contiguous
     along their last dimension (views of one projection's output, say); slots:
     int32 or int64 [T], page * page_size + place. A token whose slot is
-    negative or past the cache is left out; two tokens of one slot leave one of
-    them. weight: the root-mean-square norm's, applied to the latents in fp32
+    negative or past the cache is left out. Slots that are read later must be
+    distinct: tokens of one slot are written side by side, in no order, and may
+    leave one's codes with another's scales or rotary key (a slot that padded
+    tokens share may hold anything). weight: the root-mean-square norm's, applied to the latents in fp32
     first (None: no norm). An fp8 cache gets hip_per_block_quant's codes and
     scales of 1 x 128 groups, with eps as the amax floor."""
     if latent.ndim != 2 or rope.ndim != 2 or latent.shape[0] != rope.shape[0]:
