@@ -19,6 +19,32 @@ _FP8_DTYPES = (torch.float8_e4m3fn, torch.float8_e5m2)
 _OUT_DTYPES = (torch.bfloat16, torch.float16, torch.float32, torch.float8_e4m3fn, torch.float8_e5m2)
 
 
+class _Inference(torch.autograd.Function):
+    """The results of a call that has no gradient, as results of its inputs."""
+
+    @staticmethod
+    def forward(ctx, what, count, *tensors):
+        ctx.what = what
+        return tuple(t.detach() for t in tensors[:count])
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError(f"{ctx.what} is an inference form and has no gradient")
+
+
+def without_gradient(what: str, inputs, *outputs: Optional[torch.Tensor]):
+    """The outputs of a call without a gradient, some of whose inputs require one: going backward through them is an
+    error, as through the package's ops that have no gradient formula."""
+    kept = [t for t in outputs if t is not None]
+    new = iter(_Inference.apply(what, len(kept), *kept, *(t for t in inputs if t is not None)))
+    return tuple(None if t is None else next(new) for t in outputs)
+
+
+def refuse_recorded(what: str, written: str) -> None:
+    raise ValueError(f"{what}: an input requires a gradient, which {written} cannot carry; call it under "
+                     "torch.no_grad() or with detached inputs")
+
+
 def matrix_layout(tensor: torch.Tensor, name: str) -> str:
     """'n-major' when the last dim is contiguous, 'k-major' when the second-last is."""
     if tensor.stride(-1) == 1:

@@ -127,33 +127,37 @@ def hip_latent_append(
     scales of 1 x 128 groups, with eps as the amax floor."""
     if latent.ndim != 2 or rope.ndim != 2 or latent.shape[0] != rope.shape[0]:
         raise ValueError(f"latent and rope must be [T, width], got {tuple(latent.shape)} and {tuple(rope.shape)}")
-    if latent.dtype not in _TOKEN_DTYPES or rope.dtype != latent.dtype:
-        raise ValueError(f"latent and rope must both be bfloat16 or float16, got {latent.dtype} and {rope.dtype}")
+    dtype, device = latent.dtype, latent.device
+    if dtype not in _TOKEN_DTYPES or rope.dtype != dtype:
+        raise ValueError(f"latent and rope must both be bfloat16 or float16, got {dtype} and {rope.dtype}")
     tokens = latent.shape[0]
-    if latent.stride(1) != 1 or rope.stride(1) != 1:
+    sl, sr = latent.stride(), rope.stride()
+    if sl[1] != 1 or sr[1] != 1:
         raise ValueError("latent and rope must be contiguous along their last dimension")
     if slots.shape != (tokens,) or slots.dtype not in (torch.int32, torch.int64) or tokens > 1 and slots.stride(0) != 1:
         raise ValueError(f"slots must be contiguous int32 or int64 with shape ({tokens},), got {slots.dtype}, "
                          f"{tuple(slots.shape)}")
-    if slots.device != latent.device or rope.device != latent.device:
-        raise ValueError(f"slots and rope must be on {latent.device}, got {slots.device} and {rope.device}")
-    dl, dr, _, _, cache_args = _check_cache(cache, latent.dtype, latent.device)
+    if slots.device != device or rope.device != device:
+        raise ValueError(f"slots and rope must be on {device}, got {slots.device} and {rope.device}")
+    dl, dr, _, _, cache_args = _check_cache(cache, dtype, device)
     if latent.shape[1] != dl or rope.shape[1] != dr:
         raise ValueError(f"the cache holds widths {dl} and {dr}, got {latent.shape[1]} and {rope.shape[1]}")
     if weight is not None:
         if weight.shape != (dl,) or weight.stride(0) != 1 or weight.dtype not in C._INPUT_DTYPES:
             raise ValueError(f"weight must be contiguous float32, bfloat16 or float16 with shape ({dl},), got "
                              f"{weight.dtype}, {tuple(weight.shape)}")
-        if weight.device != latent.device:
-            raise ValueError(f"weight must be on {latent.device}, got {weight.device}")
+        if weight.device != device:
+            raise ValueError(f"weight must be on {device}, got {weight.device}")
     if eps < 0 or norm_eps < 0:
         raise ValueError(f"eps and norm_eps must not be negative, got {eps} and {norm_eps}")
     if not latent.is_cuda:
         _lib.require_gpu_tensor(latent, "latent")
+    if ((latent.requires_grad or rope.requires_grad or weight is not None and weight.requires_grad)
+            and torch.is_grad_enabled()):
+        C.refuse_recorded("latent_append", "the cache")
     rc = _lib.launch(
         _lib.lib().pcamd_latent_append, latent,
-        latent.data_ptr(), rope.data_ptr(), _lib.dtype_code(latent.dtype), tokens, dl, dr,
-        latent.stride(0), rope.stride(0), _lib.ptr(weight), 0 if weight is None else _lib.dtype_code(weight.dtype),
+        latent.data_ptr(), rope.data_ptr(), _lib.dtype_code(dtype), tokens, dl, dr, sl[0], sr[0], _lib.ptr(weight), 0 if weight is None else _lib.dtype_code(weight.dtype),
         slots.data_ptr(), slots.element_size(), *cache_args, norm_eps, eps)
     if rc == _lib.ERR_UNSUPPORTED:
         raise ValueError(_lib.lib().pcamd_last_error().decode())
@@ -211,7 +215,8 @@ def hip_latent_decode(
     2^15 under float16 ones, whose attention weights are multiplied by them.
 
     Returns out [B, S, H, latent] in the queries' dtype and, with return_lse,
-    float32 [B, S, H]: the natural logarithm of the sum of exponentials."""
+    float32 [B, S, H]: the natural logarithm of the sum of exponentials. There
+    is no gradient: going backward is an error."""
     if q_latent.ndim != 4 or q_rope.ndim != 4 or q_latent.shape[:3] != q_rope.shape[:3]:
         raise ValueError("queries must be [B, S, H, width], got "
                          f"{tuple(q_latent.shape)} and {tuple(q_rope.shape)}")
@@ -237,6 +242,9 @@ def hip_latent_decode(
             or batch > 1 and seq_lens.stride(0) != 1):
         raise ValueError(f"seq_lens must be contiguous int32 with shape ({batch},) on {device}; "
                          f"got {seq_lens.dtype}, {tuple(seq_lens.shape)}, {seq_lens.device}")
+    record = (q_latent.requires_grad or q_rope.requires_grad) and torch.is_grad_enabled()
+    if record and out is not None:
+        C.refuse_recorded("latent_decode", "out")
     out = _check_out(out, (batch, new, heads, dl), q_latent)
     rows = (("q_latent", q_latent), ("q_rope", q_rope), ("the cache's latent", cache.latent),
             ("the cache's rope", cache.rope), ("out", out))
@@ -260,6 +268,8 @@ def hip_latent_decode(
         softmax_scale, _lib.ptr(workspace), need)
     if rc != 0:
         _refused(rc, "pcamd_latent_decode", rows)
+    if record:
+        out, lse = C.without_gradient("latent_decode", (q_latent, q_rope), out, lse)
     return (out, lse) if return_lse else out
 
 
@@ -299,7 +309,8 @@ def hip_latent_prefill(
     that see it and may reach up to 31 earlier ones of its sequence.
 
     Returns out [Tq, H, value] in q's dtype and, with return_lse, float32
-    [Tq, H]: the natural logarithm of the sum of exponentials."""
+    [Tq, H]: the natural logarithm of the sum of exponentials. There is no
+    gradient: going backward is an error."""
     if q.ndim != 3 or k_nope.ndim != 3 or k_rope.ndim != 2 or v.ndim != 3:
         raise ValueError("q, k_nope and v must be [T, H, width] and k_rope [T, width]; got "
                          f"{tuple(q.shape)}, {tuple(k_nope.shape)}, {tuple(v.shape)} and {tuple(k_rope.shape)}")
@@ -327,6 +338,10 @@ def hip_latent_prefill(
                 or t.stride(0) != 1):
             raise ValueError(f"cu_q and cu_k must be contiguous int32 [n + 1] on {device}; {name} is {t.dtype}, "
                              f"{tuple(t.shape)}, {t.device}")
+    record = ((q.requires_grad or k_nope.requires_grad or k_rope.requires_grad or v.requires_grad)
+              and torch.is_grad_enabled())
+    if record and out is not None:
+        C.refuse_recorded("latent_prefill", "out")
     out = _check_out(out, (total_q, heads, dv), q)
     rows = (("q", q), ("k_nope", k_nope), ("k_rope", k_rope), ("v", v), ("out", out))
     if not q.is_cuda:
@@ -342,4 +357,6 @@ def hip_latent_prefill(
         1.0 / math.sqrt(dk) if softmax_scale is None else softmax_scale, 1 if causal else 0)
     if rc != 0:
         _refused(rc, "pcamd_latent_prefill", rows)
+    if record:
+        out, lse = C.without_gradient("latent_prefill", (q, k_nope, k_rope, v), out, lse)
     return (out, lse) if return_lse else out

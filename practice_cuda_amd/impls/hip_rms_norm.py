@@ -46,7 +46,7 @@ def hip_rms_norm_quant(
     ``residual`` or ``x`` itself); None comes back where there is no residual.
     norm_eps is added to the mean square, eps is the amax floor of the
     quantization. A group with a NaN keeps it as a NaN code; its scale is that
-    of the other values."""
+    of the other values. There is no gradient: going backward is an error."""
     C.check_quant_input(x, fp8_dtype, "rms norm quant")
     shape, strides, dtype, device = x.shape, x.stride(), x.dtype, x.device
     n = shape[-1]
@@ -63,17 +63,22 @@ def hip_rms_norm_quant(
         raise ValueError(f"weight must be on {device}, got {weight.device}")
     flat = len(shape) == 2  # rows without a batch dimension: batch stride 0
     batch, m = (1, shape[0]) if flat else shape[:2]
+    given = residual_out is not None
     if residual is None:
-        if residual_out is not None:
+        if given:
             raise ValueError("residual_out needs a residual")
         residual_args, out_args = (0, 0, 0), (0, 0, 0)
     else:
-        if residual_out is None:
+        if not given:
             residual_out = torch.empty(shape, dtype=dtype, device=device)
         residual_args = _like(residual, "residual", shape, dtype, device, flat)
         out_args = _like(residual_out, "residual_out", shape, dtype, device, flat)
     if not x.is_cuda:
         _lib.require_gpu_tensor(x, "x")
+    record = ((x.requires_grad or weight.requires_grad or residual is not None and residual.requires_grad)
+              and torch.is_grad_enabled())
+    if record and given:
+        C.refuse_recorded("rms_norm_quant", "residual_out")
     groups = -(-n // _GROUP)
     q = torch.empty(shape, dtype=fp8_dtype, device=device)
     scale = torch.empty((m, groups) if flat else (batch, m, groups), dtype=torch.float32, device=device)
@@ -84,6 +89,8 @@ def hip_rms_norm_quant(
         q.data_ptr(), _lib.dtype_code(fp8_dtype), m * n, n, scale.data_ptr(), m * groups, groups,
         *out_args, norm_eps, _lib.FP8_MAX[fp8_dtype], eps)
     _lib.check(rc, "pcamd_rms_norm_quant")
+    if record:
+        q, scale, residual_out = C.without_gradient("rms_norm_quant", (x, weight, residual), q, scale, residual_out)
     return QuantResult(q, scale, "hip_rms_norm", "block",
                        {"logical_shape": tuple(shape), "fp8_dtype": _NAMES[fp8_dtype], "block_m": 1,
                         "block_n": _GROUP}), residual_out

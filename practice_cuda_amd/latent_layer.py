@@ -23,6 +23,7 @@ import math
 import torch
 import torch.nn as nn
 
+from .impls._common import without_gradient
 from .impls.hip_latent import LatentCache, hip_latent_append, hip_latent_decode, hip_latent_prefill
 from .impls.hip_per_block import hip_per_block_quant
 from .impls.hip_rms_norm import hip_rms_norm_quant
@@ -144,6 +145,22 @@ class LatentAttention(nn.Module):
 
     def prefill(self, x, residual, cache: LatentCache, slots, positions, cu_seqlens):
         """Whole prompts, packed: sequence i holds tokens cu_seqlens[i] .. cu_seqlens[i + 1] - 1 (int32)."""
+        return self._served(self._prefill, x, residual, cache, slots, positions, cu_seqlens)
+
+    def decode(self, x, residual, cache: LatentCache, slots, positions, block_table, seq_lens):
+        """New tokens, [B * S, hidden] for B = seq_lens.numel() sequences of S each; seq_lens counts them."""
+        return self._served(self._decode, x, residual, cache, slots, positions, block_table, seq_lens)
+
+    def _served(self, form, x, residual, *args):
+        """Both forms are for inference: what requires a gradient gets the same results, and an error backward."""
+        inputs = (x, residual, self.norm, self.latent_norm, *(w for w, _ in self._weights()))
+        if not torch.is_grad_enabled() or not any(t is not None and t.requires_grad for t in inputs):
+            return form(x, residual, *args)
+        with torch.no_grad():
+            results = form(x, residual, *args)
+        return without_gradient(type(self).__name__, inputs, *results)
+
+    def _prefill(self, x, residual, cache, slots, positions, cu_seqlens):
         q, latent, rope, residual = self._project(x, residual, cache, slots, positions)
         c, _ = hip_rms_norm_quant(latent[None], self.latent_norm, norm_eps=self.norm_eps)
         both = _product(c, self._fp8["key_value"])[0].view(x.shape[0], self.heads, 2 * self.head_dim)
@@ -151,8 +168,7 @@ class LatentAttention(nn.Module):
                                softmax_scale=self.softmax_scale)
         return self._output(o), residual
 
-    def decode(self, x, residual, cache: LatentCache, slots, positions, block_table, seq_lens):
-        """New tokens, [B * S, hidden] for B = seq_lens.numel() sequences of S each; seq_lens counts them."""
+    def _decode(self, x, residual, cache, slots, positions, block_table, seq_lens):
         tokens, batch, heads = x.shape[0], seq_lens.shape[0], self.heads
         new = tokens // batch if batch else 0
         if new * batch != tokens:
