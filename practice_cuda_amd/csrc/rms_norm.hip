@@ -318,7 +318,9 @@ int launch_norm(const NormArgs& a, hipStream_t st) {
   if (a.n <= 8192) return go(integral_constant<int, 512>{}, integral_constant<int, 2>{});
   if (a.n <= 12288) return go(integral_constant<int, 512>{}, integral_constant<int, 3>{});
   if (a.n <= 16384) return go(integral_constant<int, 512>{}, integral_constant<int, 4>{});
-  if (a.n <= 65536) return go(integral_constant<int, 1024>{}, integral_constant<int, 8>{});
+  // Longer rows are read twice, the second time from the caches. 1024 lanes with eight chunks hold rows of up to 65536 columns,
+  // but not within their registers: 16390 columns, bf16, 70 us (held 178), 32768 59 (113), 65536 61 (76), one row of 16390
+  // 8.4 (19.6); fp32 102 (190), 104 (134) and, the only loss, 110 (105).
   return go(integral_constant<int, 1024>{}, integral_constant<int, 0>{});
 }
 
