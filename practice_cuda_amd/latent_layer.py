@@ -94,22 +94,27 @@ class LatentAttention(nn.Module):
                 for name, new in codes.items():
                     old[name].tensor.copy_(new.tensor)
                     old[name].dequant_scale.copy_(new.dequant_scale)
-        self._made_from = self._weights()
+        # with torch's count of their changes in place, which inference tensors do not have
+        self._made_from = [(n, w, None if w.is_inference() else w._version) for n, w in self._weights()]
         return self
 
-    def _weights(self) -> list:
-        """The weights that have codes, each with its count of changes in place (inference tensors have none)."""
-        return [(w, 0 if w.is_inference() else w._version)
-                for w in (self.w_query, self.w_latent, self.w_key, self.w_value, self.w_out)]
+    def _weights(self):
+        return [(name, getattr(self, name)) for name in ("w_query", "w_latent", "w_key", "w_value", "w_out")]
 
     def _current(self) -> bool:
-        return self._fp8 is not None and all(
-            w is old and count == before for (w, count), (old, before) in zip(self._weights(), self._made_from))
+        """Whether the codes are those of the weights as they are."""
+        if self._fp8 is None:
+            return False
+        own = self._parameters  # the module's own lookup of a parameter takes half a microsecond
+        for name, weight, count in self._made_from:
+            if own.get(name) is not weight or count is not None and weight._version != count:
+                return False
+        return True
 
     def _apply(self, fn, recurse=True):
         """Moves and type changes put other data behind the same parameters."""
         def places():
-            return [(w.data_ptr(), w.dtype, w.device) for w, _ in self._weights()]
+            return [(w.data_ptr(), w.dtype, w.device) for _, w in self._weights()]
 
         before, freq = places(), self.freq
         super()._apply(fn, recurse)
@@ -119,11 +124,14 @@ class LatentAttention(nn.Module):
             self._fp8 = self._made_from = None
         return self
 
-    def _rotate(self, x: torch.Tensor, positions: torch.Tensor) -> torch.Tensor:
-        """Rotary positions over the halves of the last dimension; x [T, .., rope]."""
+    def _angles(self, positions: torch.Tensor):
         angle = positions.float()[:, None] * self.freq
+        return angle.cos(), angle.sin()
+
+    def _rotate(self, x: torch.Tensor, positions: torch.Tensor, angles=None) -> torch.Tensor:
+        """Rotary positions over the halves of the last dimension; x [T, .., rope]; angles: those of the positions."""
         shape = (x.shape[0],) + (1,) * (x.ndim - 2) + (x.shape[-1] // 2,)
-        cos, sin = angle.cos().view(shape), angle.sin().view(shape)
+        cos, sin = (t.view(shape) for t in angles or self._angles(positions))
         a, b = x.float().chunk(2, -1)
         return torch.cat([a * cos - b * sin, a * sin + b * cos], -1).to(x.dtype)
 
@@ -135,8 +143,9 @@ class LatentAttention(nn.Module):
                                            norm_eps=self.norm_eps)
         q = _product(normed, self._fp8["query"])[0].view(x.shape[0], self.heads, self.head_dim + self.rope_dim)
         both = _product(normed, self._fp8["latent"])[0]
-        latent, rope = both[:, :self.latent_dim], self._rotate(both[:, self.latent_dim:], positions)
-        q[..., self.head_dim:] = self._rotate(q[..., self.head_dim:], positions)
+        angles = self._angles(positions)
+        latent, rope = both[:, :self.latent_dim], self._rotate(both[:, self.latent_dim:], positions, angles)
+        q[..., self.head_dim:] = self._rotate(q[..., self.head_dim:], positions, angles)
         hip_latent_append(cache, latent, rope, slots, weight=self.latent_norm, norm_eps=self.norm_eps)
         return q, latent, rope, x if total is None else total[0]
 
@@ -153,12 +162,14 @@ class LatentAttention(nn.Module):
 
     def _served(self, form, x, residual, *args):
         """Both forms are for inference: what requires a gradient gets the same results, and an error backward."""
-        inputs = (x, residual, self.norm, self.latent_norm, *(w for w, _ in self._weights()))
-        if not torch.is_grad_enabled() or not any(t is not None and t.requires_grad for t in inputs):
-            return form(x, residual, *args)
-        with torch.no_grad():
-            results = form(x, residual, *args)
-        return without_gradient(type(self).__name__, inputs, *results)
+        if torch.is_grad_enabled():
+            inputs = [x, residual, *self._parameters.values()]
+            for t in inputs:
+                if t is not None and t.requires_grad:
+                    with torch.no_grad():
+                        results = form(x, residual, *args)
+                    return without_gradient(type(self).__name__, inputs, *results)
+        return form(x, residual, *args)
 
     def _prefill(self, x, residual, cache, slots, positions, cu_seqlens):
         q, latent, rope, residual = self._project(x, residual, cache, slots, positions)
