@@ -51,10 +51,11 @@ constexpr int kFixed = MR == 32 ? (SPLIT == 2 ? 8 : 10) : 3;
 // to LDS (the second time from the XCD's L2) and cannot overlap a tile's
 // softmax with the next one's scores: they win where sequences are cut into
 // pieces, up to half as many tiles as CUs. 128 heads over a bf16 cache, us, two
-// workgroups against one: 16 sequences of 4096 tokens 45 / 64, 48 of 2048 56 /
-// 64, 128 of 4096 203 / 199, 160 of 1024 and of 4096 91 / 98 and 270 / 253, 256
-// of 300 and of 8192 63 / 50 and 690 / 609. fp8: 16 of 4096 52 / 65, 128 of 4096
-// 209 / 220, 192 of 4096 321 / 315, 256 of 300 71 / 52.
+// workgroups against one: 16 sequences of 4096 tokens 47 / 66, 48 of 2048 65 /
+// 71, 128 of 1024 and of 4096 63 / 80 and 185 / 182, 160 of 1024 and of 4096 94 /
+// 98 and 249 / 233, 256 of 300 and of 2048 64 / 50 and 200 / 168. fp8: 16 of 4096
+// 55 / 66, 48 of 2048 67 / 67, 128 of 1024 and of 4096 65 / 80 and 193 / 199, 160
+// of 1024 100 / 96, 256 of 300 70 / 49.
 struct Shape {
   int mr, wr, split;  // rows of a wave, waves over rows, workgroups over rows
   int tile_rows() const { return mr * wr * split; }

@@ -17,7 +17,7 @@
 // vector units do while the products run. 8192 tokens, 32 heads, causal, bf16:
 // 688 GFLOP in 646 us, 1.06 PFLOP/s, where an 8192^3 product of the library
 // reaches 1.25; 6 prompts of up to 1111 tokens behind up to 700 cached ones, 128
-// heads: 310 GFLOP in 411 us (their ends fill tiles in part; a workgroup a CU
+// heads: 310 GFLOP in 413 us (their ends fill tiles in part; a workgroup a CU
 // took 467). Under this load the clock falls to about 1.6 GHz, so what remains
 // is power.
 #include <hip/hip_runtime.h>
@@ -582,8 +582,9 @@ int launch_rows(Args a, hipStream_t st) {
 template <int DT, int DN, int DR, int DV>
 int launch(const Args& a, hipStream_t st) {
   // 256-row tiles for prompts that are long on average. Tokens x heads, causal, bf16, us with 128 and 256 rows: 4096 x 16
-  // 103 / 133, 8192 x 16 337 / 335, 8192 x 32 653 / 644, 16384 x 16 1278 / 1229, 32768 x 16 5177 / 4734; 4096 x 128 731 /
-  // 732, 4 sequences of 10 to 4000 tokens, 32 heads 251 / 271, 16 of 512, 16 heads 49 / 64, 40 of 300, 128 heads 470 / 807
+  // 108 / 135, 4096 x 32 206 / 206, 8192 x 16 321 / 316, 8192 x 32 643 / 632, 16384 x 16 1265 / 1216, 32768 x 16 5174 / 4929;
+  // 4096 x 128 704 / 737, 2 sequences of 7000, 32 heads 979 / 992 and of 8192, 16 heads 689 / 703, 4 of 10 to 4000, 32 heads
+  // 294 / 333, 16 of 512, 16 heads 52 / 66, 40 of 300, 128 heads 465 / 830
   const bool many = a.total_q >= int64_t{8192} * a.sequences && a.total_q * a.heads >= 8192 * 16;
   return many ? launch_rows<DT, DN, DR, DV, 2>(a, st) : launch_rows<DT, DN, DR, DV, 1>(a, st);
 }

@@ -7,14 +7,15 @@
 //   per group of 128 columns: qs = fp8_max / max(max|y|, eps),
 //   codes = fp8(clamp(y * qs)), scale = 1 / qs
 //
-// One team of lanes holds a row in registers between the two reductions (the
-// sum of squares over the row, the maxima over 16-lane groups), so every input
-// is read once. Lane i of the team takes the 8-element chunks i, i + TEAM, ..;
+// One team of lanes holds a row of up to 16384 values in registers between the
+// two reductions (the sum of squares over the row, the maxima over 16-lane
+// groups), so every input is read once. Lane i of the team takes the 8-element chunks i, i + TEAM, ..;
 // 16 neighbouring lanes then hold one quantization group.
 //
 // Bound by memory: 4096 x 7168 bf16 with a residual, 206 MB, takes 50.2 us, 4.1
-// TB/s (a copy of such size 4.9 on the same machine); by the launch where rows
-// are few: 56 tokens of 512 + 64 into an fp8 cache 9.3 us a call, most of it
+// TB/s (a large copy 5.9 to 6.4). Rows that are not 16-byte aligned take longer: 29
+// million values in rows of 5003 columns 58 us, of 5120 45. By the launch where
+// rows are few: 56 tokens of 512 + 64 into an fp8 cache 9 us a call, most of it
 // the host's.
 #include <hip/hip_runtime.h>
 
@@ -110,9 +111,11 @@ PCAMD_DEV float amax8(const float (&y)[8]) {
 }
 
 // Scales of a group of y = t * inv, t = r * w: as block_scales of y, with inv
-// left out of the codes' factor where y's largest value sets it, so that codes
-// come of two roundings less. (inf * 0, of a row with an infinity, takes the
-// floor: its other values are zeros.)
+// left out of the codes' factor where y's largest value sets it: codes come of
+// r * w, one division and their product, without the roundings of inv and of y.
+// Which side of a boundary between two codes a value falls on still differs from
+// one order of operations to another. (inf * 0, of a row with an infinity, takes
+// the floor: its other values are zeros.)
 PCAMD_DEV Scales normed_scales(float amax_t, float inv, float fp8_max, float eps) {
   const bool above = amax_t * inv >= eps;
   const float qs = fp8_max / (above ? amax_t : eps);

@@ -157,8 +157,8 @@ def hip_latent_append(
         C.refuse_recorded("latent_append", "the cache")
     rc = _lib.launch(
         _lib.lib().pcamd_latent_append, latent,
-        latent.data_ptr(), rope.data_ptr(), _lib.dtype_code(dtype), tokens, dl, dr, sl[0], sr[0], _lib.ptr(weight), 0 if weight is None else _lib.dtype_code(weight.dtype),
-        slots.data_ptr(), slots.element_size(), *cache_args, norm_eps, eps)
+        latent.data_ptr(), rope.data_ptr(), _lib.dtype_code(dtype), tokens, dl, dr, sl[0], sr[0],
+        _lib.ptr(weight), 0 if weight is None else _lib.dtype_code(weight.dtype), slots.data_ptr(), slots.element_size(), *cache_args, norm_eps, eps)
     if rc == _lib.ERR_UNSUPPORTED:
         raise ValueError(_lib.lib().pcamd_last_error().decode())
     _lib.check(rc, "pcamd_latent_append")

@@ -417,7 +417,7 @@ def test_prefill_long(dev):
 @pytest.mark.parametrize("widths", [(128, 64, 128), (64, 32, 64)])
 @pytest.mark.parametrize("dtype", [BF16, FP16])
 def test_prefill_many_rows(dev, dtype, widths, causal):
-    # past 65536 rows and heads tiles have 256 rows: whole ones, ends of up to 128 and of more, keys before and missing
+    # ends of up to 128 rows and of more, keys before and missing, in tiles of 128 rows (256: from 8192 rows a sequence)
     pairs = [(257, 300), (129, 400), (128, 128), (256, 256), (1, 70), (30, 0), (0, 7), (385, 385), (20, 10)]
     prefill_case(dev, pairs, 56, dtype=dtype, widths=widths, causal=causal, seed=7, spare=3, strided=True)
 
@@ -449,7 +449,7 @@ def test_prefill_tiles_of_256_rows_in_many_sequences(dev, n):
 @pytest.mark.parametrize("n", [62, 63, 64, 65])
 @pytest.mark.parametrize("heads", [1, 64])
 def test_prefill_sequences_of_a_wave(dev, n, heads):
-    # up to 63 sequences a wave finds its tile alone; 64 heads: tiles of 256 rows
+    # up to 63 sequences a wave finds its tile alone
     prefill_case(dev, [((37 * i) % 35 + (0 if heads == 1 else 2), (37 * i) % 35 + i % 6) for i in range(n)], heads,
                  seed=n)
 
