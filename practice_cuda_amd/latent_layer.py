@@ -77,26 +77,33 @@ class LatentAttention(nn.Module):
         """The weights' fp8 forms. The layer's calls make them where they are missing, or older than a weight that was
         loaded, replaced, moved or changed in place since. Edits that torch does not count (through ``.data``, or of
         weights made in inference mode) need a call of this. New codes take the old ones' places, so a captured graph
-        reads them."""
-        both = torch.cat([self.w_key, self.w_value], 1).reshape(1, -1, self.latent_dim)
-        codes = {
-            "query": _quant(self.w_query, 128), "latent": _quant(self.w_latent, 128),
-            "key_value": _quant(both, 128),  # [1, H * 2 head, latent], head after head
-            "absorb": _quant(self.w_key.transpose(1, 2).contiguous(), 128),  # [H, latent, head]
-            "value": _quant(self.w_value, 128), "out": _quant(self.w_out, 128),
-        }
-        old = self._fp8
+        reads them; they are there when this returns, for any stream."""
+        codes, old = self._codes(), self._fp8
+        capturing = torch.cuda.is_current_stream_capturing()
         if old is None or any(old[n].tensor.shape != c.tensor.shape or old[n].tensor.device != c.tensor.device
                               for n, c in codes.items()):
+            if capturing:
+                raise RuntimeError("quantize() in a captured graph renews codes: make them before the capture")
             self._fp8 = codes
         else:
             with torch.inference_mode():  # the old ones may be inference tensors
                 for name, new in codes.items():
                     old[name].tensor.copy_(new.tensor)
                     old[name].dequant_scale.copy_(new.dequant_scale)
-        # with torch's count of their changes in place, which inference tensors do not have
-        self._made_from = [(n, w, None if w.is_inference() else w._version) for n, w in self._weights()]
+        if not capturing:
+            # with torch's count of their changes in place, which inference tensors do not have
+            self._made_from = [(n, w, None if w.is_inference() else w._version) for n, w in self._weights()]
+            torch.cuda.current_stream(self.w_out.device).synchronize()
         return self
+
+    def _codes(self) -> dict:
+        both = torch.cat([self.w_key, self.w_value], 1).reshape(1, -1, self.latent_dim)
+        return {
+            "query": _quant(self.w_query, 128), "latent": _quant(self.w_latent, 128),
+            "key_value": _quant(both, 128),  # [1, H * 2 head, latent], head after head
+            "absorb": _quant(self.w_key.transpose(1, 2).contiguous(), 128),  # [H, latent, head]
+            "value": _quant(self.w_value, 128), "out": _quant(self.w_out, 128),
+        }
 
     def _weights(self):
         return [(name, getattr(self, name)) for name in ("w_query", "w_latent", "w_key", "w_value", "w_out")]
@@ -137,8 +144,6 @@ class LatentAttention(nn.Module):
 
     def _project(self, x, residual, cache, slots, positions):
         """(queries [T, H, head + rope], latents, rotary keys, residual); the tokens are in the cache."""
-        if not self._current():
-            self.quantize()
         normed, total = hip_rms_norm_quant(x[None], self.norm, residual=None if residual is None else residual[None],
                                            norm_eps=self.norm_eps)
         q = _product(normed, self._fp8["query"])[0].view(x.shape[0], self.heads, self.head_dim + self.rope_dim)
@@ -167,9 +172,22 @@ class LatentAttention(nn.Module):
             for t in inputs:
                 if t is not None and t.requires_grad:
                     with torch.no_grad():
-                        results = form(x, residual, *args)
+                        results = self._with_codes(form, x, residual, *args)
                     return without_gradient(type(self).__name__, inputs, *results)
-        return form(x, residual, *args)
+        return self._with_codes(form, x, residual, *args)
+
+    def _with_codes(self, form, *args):
+        if self._current():
+            return form(*args)
+        if not torch.cuda.is_current_stream_capturing():
+            self.quantize()
+            return form(*args)
+        # A captured call is recorded and not run: its codes are the graph's own, made at every replay.
+        held, self._fp8 = self._fp8, self._codes()
+        try:
+            return form(*args)
+        finally:
+            self._fp8 = held
 
     def _prefill(self, x, residual, cache, slots, positions, cu_seqlens):
         q, latent, rope, residual = self._project(x, residual, cache, slots, positions)
