@@ -43,10 +43,11 @@
 extern "C" {
 #endif
 
-#define PCAMD_ABI_VERSION 6 /* 2: pcamd_bmm_scaled_mixed; 3: pcamd_quant_block_ex, pcamd_quant_block_dual_ex;
+#define PCAMD_ABI_VERSION 7 /* 2: pcamd_bmm_scaled_mixed; 3: pcamd_quant_block_ex, pcamd_quant_block_dual_ex;
                               4: PCAMD_F64 scale arithmetic of pcamd_quant_tensor;
                               5: pcamd_quant_channel_ws, pcamd_quant_tensor_ws;
-                              6: pcamd_rms_norm_quant and the pcamd_latent_ functions */
+                              6: pcamd_rms_norm_quant and the pcamd_latent_ functions;
+                              7: the int8 functions and the pcamd_expert_ ones */
 
 /* status codes */
 #define PCAMD_OK 0
@@ -73,6 +74,7 @@ extern "C" {
 /* BMM epilogue activations */
 #define PCAMD_ACT_NONE 0
 #define PCAMD_ACT_GELU 1 /* exact: 0.5 x (1 + erf(x / sqrt 2)) */
+#define PCAMD_ACT_SWIGLU 2 /* int8 products only: silu(gate) * other, over halves of b's rows */
 
 int pcamd_abi_version(void);
 const char *pcamd_last_error(void);
@@ -406,6 +408,97 @@ int pcamd_latent_prefill(const void *q, const void *k_nope, const void *k_rope,
                          int64_t sot, int64_t soh, float *lse, int64_t slt,
                          int64_t slh, float softmax_scale, int causal,
                          void *stream);
+
+/*
+ * Int8 codes of x[batch, m, n] (fp32, bf16 or fp16, contiguous along n, any
+ * row strides and alignment) with one scale a row: top = max(max|x|, eps),
+ * scale[b, i] = top / 127 (fp32 division), y = rint(127 x / top) of the real
+ * quotient, ties to even. A row with a NaN or an infinity gets the scale NaN
+ * and codes of zero. Rows of y are 16-byte aligned and written up to the next
+ * multiple of 16 bytes, with zeros behind n. Available from PCAMD_ABI_VERSION
+ * 7, as the functions below. No counterpart in the reference, whose quantizers
+ * are fp8 (fp8_training/fp8_bench/impls/triton_per_channel.py:90-219).
+ */
+int pcamd_quant_int8(const void *x, int x_dtype, int64_t batch, int64_t m,
+                     int64_t n, int64_t sxb, int64_t sxm, void *y, int64_t syb,
+                     int64_t sym, float *scale, int64_t ssb, int64_t ssm,
+                     float eps, void *stream);
+
+/*
+ * c[b, i, j] = act(sum_k a[b, i, k] b[b, j, k] * (sa[b, i] * sb[b, j]) +
+ * bias[b, i, j]) for int8 a[batch, m, k] and b[batch, n, k], both contiguous
+ * along k with 16-byte aligned rows; c is fp32, bf16 or fp16, contiguous along
+ * its columns. Sums are exact (int32), k goes up to 131071. PCAMD_ACT_SWIGLU:
+ * b has 2 n rows (and sb and bias as many columns), c[.., j] = silu(column j)
+ * * column n + j. Bytes of a row up to the next multiple of 16 may be read and
+ * do not count.
+ */
+int pcamd_bmm_int8(const void *a, const void *b, int64_t batch, int64_t m,
+                   int64_t n, int64_t k, int64_t sab, int64_t sam, int64_t sbb,
+                   int64_t sbn, void *c, int c_dtype, int64_t scb, int64_t scm,
+                   const void *bias, int bias_dtype, int64_t sbiasb,
+                   int64_t sbiasm, int64_t sbiasn, const float *sa,
+                   int64_t ssab, int64_t ssam, const float *sb, int64_t ssbb,
+                   int64_t ssbn, int activation, void *stream);
+
+/*
+ * Pairs (token, choice) sorted by expert, stable: ids[pairs] (id_bytes 4 or 8:
+ * int32, int64), order[place] = pair, place[pair] = its place, starts[experts
+ * + 1] the first place of each expert and the end of the last. Pairs whose id
+ * is negative or not below experts come last, in their own order, and have
+ * place -1 - place. Up to 1024 experts and 2^31 - 1 pairs. The workspace has
+ * at least pcamd_expert_sort_workspace() bytes; a negative result of that call
+ * is a status.
+ */
+int64_t pcamd_expert_sort_workspace(int64_t pairs, int64_t experts);
+int pcamd_expert_sort(const void *ids, int id_bytes, int64_t pairs,
+                      int64_t experts, int32_t *order, int32_t *place,
+                      int32_t *starts, void *workspace, int64_t workspace_bytes,
+                      void *stream);
+
+/*
+ * Rows to the order of experts and back (place[tokens, choices] as above;
+ * fp32, bf16 or fp16, contiguous along width, up to 128 choices):
+ *   dispatch: out[place] = x[token], zeros at the places of pairs without one;
+ *   combine: out[t] = sum_j weights[t, j] rows[place[t, j]] in fp32, choices
+ *     ascending, pairs without an expert left out; weights [tokens, choices]
+ *     contiguous (w_dtype), or NULL for ones (the gradient of dispatch);
+ *   combine_backward: grad_rows[place] = weights[t, j] grad[t] (zeros for
+ *     pairs without an expert) and grad_weights[t, j] = rows[place] . grad[t]
+ *     (fp32; 0 for those); either may be NULL.
+ */
+int pcamd_expert_dispatch(const void *x, int dtype, int64_t tokens,
+                          int64_t choices, int64_t width, int64_t sxt,
+                          const int32_t *place, void *out, int64_t sos,
+                          void *stream);
+int pcamd_expert_combine(const void *rows, int dtype, int64_t tokens,
+                         int64_t choices, int64_t width, int64_t srs,
+                         const int32_t *place, const void *weights, int w_dtype,
+                         void *out, int64_t sot, void *stream);
+int pcamd_expert_combine_backward(const void *grad, const void *rows, int dtype,
+                                  int64_t tokens, int64_t choices,
+                                  int64_t width, int64_t sgt, int64_t srs,
+                                  const int32_t *place, const void *weights,
+                                  int w_dtype, void *grad_rows, int64_t sos,
+                                  float *grad_weights, void *stream);
+
+/*
+ * The int8 product grouped by expert: rows starts[e] .. starts[e + 1] - 1 of
+ * c[pairs, n] are rows of a times b[e] (b[experts, n, k]; 2 n rows each with
+ * PCAMD_ACT_SWIGLU), with sa[row of a], sb[e, column] and bias[e, column].
+ * Row s of c takes row s of a, or where order is given row order[s] / choices
+ * (a then holds pairs / choices tokens). Rows behind starts[experts] are
+ * written as zeros.
+ */
+int pcamd_expert_bmm_int8(const void *a, int64_t a_rows, const void *b,
+                          int64_t experts, int64_t n, int64_t k, int64_t sam,
+                          int64_t sbe, int64_t sbn, void *c, int c_dtype,
+                          int64_t scm, const void *bias, int bias_dtype,
+                          int64_t sbiase, int64_t sbiasn, const float *sa,
+                          int64_t ssam, const float *sb, int64_t ssbe,
+                          int64_t ssbn, const int32_t *starts,
+                          const int32_t *order, int64_t pairs, int64_t choices,
+                          int activation, void *stream);
 
 #ifdef __cplusplus
 }

@@ -9,6 +9,9 @@ Public API (drop-in for xuOAO/practice_cuda's fp8_training/fp8_bench):
 * latent attention in 8 bits (serving): rms_norm_quant, LatentCache,
   latent_append, latent_decode, latent_prefill; latent_layer.LatentAttention
   runs them as one layer
+* products of int8 codes: int8_quant, int8_bmm
+* experts: expert_sort (an ExpertPlan), expert_dispatch and expert_combine (with
+  gradients), expert_bmm; expert_layer has them as layers
 
 The kernels live in the in-tree HIP library built by
 ``python -m practice_cuda_amd.build``; every entry point raises if it is
@@ -43,6 +46,13 @@ def __getattr__(name):
         "latent_append": ("hip_latent", "hip_latent_append"),
         "latent_decode": ("hip_latent", "hip_latent_decode"),
         "latent_prefill": ("hip_latent", "hip_latent_prefill"),
+        "int8_quant": ("hip_int8", "hip_int8_quant"),
+        "int8_bmm": ("hip_int8", "hip_int8_bmm"),
+        "ExpertPlan": ("hip_expert", "ExpertPlan"),
+        "expert_sort": ("hip_expert", "hip_expert_sort"),
+        "expert_dispatch": ("hip_expert", "hip_expert_dispatch"),
+        "expert_combine": ("hip_expert", "hip_expert_combine"),
+        "expert_bmm": ("hip_expert", "hip_expert_bmm"),
     }
     if name in aliases:
         import importlib

@@ -22,7 +22,7 @@ F32, BF16, F16, E4M3FN, E5M2 = 0, 1, 2, 3, 4
 F64 = 5  # scale arithmetic of pcamd_quant_tensor only (torchao's tensorwise form)
 QUANT_CACHED_OUTPUT = 1  # quantizer flag: outputs with cache-allocating stores
 SCALE_BLOCK, SCALE_CHANNEL, SCALE_TENSOR = 0, 1, 2
-ACT_NONE, ACT_GELU = 0, 1
+ACT_NONE, ACT_GELU, ACT_SWIGLU = 0, 1, 2
 # status codes (include/pcamd_fp8.h)
 OK, ERR_INVALID, ERR_UNSUPPORTED, ERR_LAUNCH = 0, -1, -2, -3
 
@@ -55,6 +55,14 @@ EXPORTED_SYMBOLS = (
     "pcamd_latent_decode_workspace",
     "pcamd_latent_decode",
     "pcamd_latent_prefill",
+    "pcamd_quant_int8",
+    "pcamd_bmm_int8",
+    "pcamd_expert_sort_workspace",
+    "pcamd_expert_sort",
+    "pcamd_expert_dispatch",
+    "pcamd_expert_combine",
+    "pcamd_expert_combine_backward",
+    "pcamd_expert_bmm_int8",
 )
 # test-only entry points (include/pcamd_fp8_selftest.h), exported by the same library
 TEST_SYMBOLS = ("pcamd_selftest_fp8_convert", "pcamd_selftest_copy16", "pcamd_selftest_narrow16")
@@ -131,6 +139,27 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.pcamd_latent_prefill.restype = _int
     lib.pcamd_latent_prefill.argtypes = (
         [_ptr] * 4 + [_int] + [_i64] * 13 + [_ptr, _ptr, _i64] + [_ptr, _i64, _i64] * 2 + [_flt, _int, _ptr])
+    lib.pcamd_quant_int8.restype = _int
+    lib.pcamd_quant_int8.argtypes = ([_ptr, _int] + [_i64] * 5 + [_ptr, _i64, _i64] * 2 + [_flt, _ptr])
+    lib.pcamd_bmm_int8.restype = _int
+    lib.pcamd_bmm_int8.argtypes = (
+        [_ptr, _ptr] + [_i64] * 8 + [_ptr, _int, _i64, _i64] + [_ptr, _int] + [_i64] * 3 + [_ptr, _i64, _i64] * 2
+        + [_int, _ptr])
+    lib.pcamd_expert_sort_workspace.restype = _i64
+    lib.pcamd_expert_sort_workspace.argtypes = [_i64, _i64]
+    lib.pcamd_expert_sort.restype = _int
+    lib.pcamd_expert_sort.argtypes = [_ptr, _int, _i64, _i64, _ptr, _ptr, _ptr, _ptr, _i64, _ptr]
+    lib.pcamd_expert_dispatch.restype = _int
+    lib.pcamd_expert_dispatch.argtypes = [_ptr, _int] + [_i64] * 4 + [_ptr, _ptr, _i64, _ptr]
+    lib.pcamd_expert_combine.restype = _int
+    lib.pcamd_expert_combine.argtypes = [_ptr, _int] + [_i64] * 4 + [_ptr, _ptr, _int, _ptr, _i64, _ptr]
+    lib.pcamd_expert_combine_backward.restype = _int
+    lib.pcamd_expert_combine_backward.argtypes = (
+        [_ptr, _ptr, _int] + [_i64] * 5 + [_ptr, _ptr, _int, _ptr, _i64, _ptr, _ptr])
+    lib.pcamd_expert_bmm_int8.restype = _int
+    lib.pcamd_expert_bmm_int8.argtypes = (
+        [_ptr, _i64, _ptr] + [_i64] * 6 + [_ptr, _int, _i64] + [_ptr, _int, _i64, _i64] + [_ptr, _i64]
+        + [_ptr, _i64, _i64] + [_ptr, _ptr, _i64, _i64] + [_int, _ptr])
     lib.pcamd_selftest_fp8_convert.restype = _int
     lib.pcamd_selftest_fp8_convert.argtypes = [_int, _ptr, _ptr]
     lib.pcamd_selftest_copy16.restype = _int
