@@ -23,7 +23,7 @@ SOURCES = ["abi.hip", "quant.hip", "bmm.hip", "bmm_fast.hip", "bmm_wide.hip", "b
            "bmm_fused_stream.hip", "repack.hip", "rms_norm.hip", "latent_decode.hip",
            "latent_decode_bf16_wide.hip", "latent_decode_bf16_narrow.hip", "latent_decode_f16_wide.hip",
            "latent_decode_f16_narrow.hip", "latent_prefill.hip", "int8_quant.hip", "int8_bmm.hip", "int8_bmm_rows.hip",
-           "expert_route.hip"]
+           "int8_bmm_tiles.hip", "expert_route.hip"]
 
 ARCH = os.environ.get("PCAMD_OFFLOAD_ARCH", "gfx950")
 

@@ -114,9 +114,21 @@ PCAMD_DEV float activate(float x, int act) {
   return act == PCAMD_ACT_GELU ? 0.5f * x * (1.0f + erff(x * 0.7071067811865475f)) : x;
 }
 
+// Four values in the 16-bit type dt
+PCAMD_DEV uint2 pack4(int dt, const float (&v)[4]) {
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  if (dt == kBF16) {
+    typedef __bf16 b16x2 __attribute__((ext_vector_type(2)));
+    return make_uint2(__builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{v[0], v[1]}, b16x2)),
+                      __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{v[2], v[3]}, b16x2)));
+  }
+  typedef _Float16 h16x2 __attribute__((ext_vector_type(2)));
+  return make_uint2(__builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{v[0], v[1]}, h16x2)),
+                    __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{v[2], v[3]}, h16x2)));
+}
+
 // Up to four neighbouring columns of a row of C, rounded once
 PCAMD_DEV void store4(void* c, int dt, int64_t off, int valid, const float (&v)[4]) {
-  typedef float f32x2 __attribute__((ext_vector_type(2)));
   if (dt == kF32) {
     float* p = static_cast<float*>(c) + off;
     if (valid >= 4 && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
@@ -128,24 +140,30 @@ PCAMD_DEV void store4(void* c, int dt, int64_t off, int valid, const float (&v)[
     }
     return;
   }
-  uint32_t w[2];
-  if (dt == kBF16) {
-    typedef __bf16 b16x2 __attribute__((ext_vector_type(2)));
-    w[0] = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{v[0], v[1]}, b16x2));
-    w[1] = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{v[2], v[3]}, b16x2));
-  } else {
-    typedef _Float16 h16x2 __attribute__((ext_vector_type(2)));
-    w[0] = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{v[0], v[1]}, h16x2));
-    w[1] = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{v[2], v[3]}, h16x2));
-  }
+  const uint2 w = pack4(dt, v);
   uint16_t* p = static_cast<uint16_t*>(c) + off;
   if (valid >= 4 && (reinterpret_cast<uintptr_t>(p) & 7) == 0) {
-    *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+    *reinterpret_cast<uint2*>(p) = w;
   } else {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      if (i < valid) p[i] = static_cast<uint16_t>(w[i >> 1] >> (16 * (i & 1)));
+      if (i < valid) p[i] = static_cast<uint16_t>((i < 2 ? w.x : w.y) >> (16 * (i & 1)));
   }
+}
+
+// The same of up to eight
+PCAMD_DEV void store8(void* c, int dt, int64_t off, int valid, const float (&v)[8]) {
+  const float lo[4] = {v[0], v[1], v[2], v[3]}, hi[4] = {v[4], v[5], v[6], v[7]};
+  if (dt != kF32) {
+    uint16_t* p = static_cast<uint16_t*>(c) + off;
+    if (valid >= 8 && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
+      const uint2 a = pack4(dt, lo), b = pack4(dt, hi);
+      *reinterpret_cast<uint4*>(p) = make_uint4(a.x, a.y, b.x, b.y);
+      return;
+    }
+  }
+  store4(c, dt, off, valid, lo);
+  if (valid > 4) store4(c, dt, off + 4, valid - 4, hi);
 }
 
 // 16 bytes of a row from k0 on; those at or past k become zeros
@@ -158,7 +176,11 @@ PCAMD_DEV v4i mask_tail(v4i v, int k0, int k) {
   return v;
 }
 
-int launch_rows(const Args& a, bool grouped, hipStream_t st);  // int8_bmm_rows.hip
+// tiles of 16 rt x 16 ct (int8_bmm_rows.hip)
+int launch_rows(const Args& a, bool grouped, int rt, int ct, hipStream_t st);
+// tiles of 256 x 256 or 128 x 128 (int8_bmm_tiles.hip), where tiles_ok
+bool tiles_ok(const Args& a, bool grouped);
+int launch_tiles(const Args& a, bool grouped, bool wide, hipStream_t st);
 
 }  // namespace int8
 }  // namespace pcamd

@@ -1,4 +1,9 @@
 // int8_bmm.hip - C entries of the int8 products (int8_bmm.h) and the choice of kernel.
+
+
+#include <algorithm>
+#include <cmath>
+
 #include "int8_bmm.h"
 
 namespace pcamd {
@@ -27,6 +32,61 @@ int check_operand(const char* name, const void* p, int64_t rows, int64_t stride,
   if (k && (!aligned16(p) || (rows > 1 && (stride % 16 || stride < k))))
     return set_error(PCAMD_ERR_INVALID, "rows of %s must be 16-byte aligned and not overlap", name);
   return PCAMD_OK;
+}
+
+// What a form of tiles would take, in us for k = 4096 without the launch, from the tile counts. The constants are
+// fitted to timings on MI355X (rotating inputs), us as modelled / measured:
+//   rows 16 rt x 16 ct: a tile costs more with rt + ct, as its waves load that many operands;
+//     24 x 14336 x 4096: 2 x 4 15 / 14, 2 x 2 16 / 17, 4 x 4 19 / 16; 64 x 4096 x 4096: 2 x 2 11 / 10, 4 x 4 19 / 19;
+//     192 rows by 64 experts of 4096 x 7168: 1 x 2 200 / 233, 2 x 4 276 / 241
+//   128 x 128: two workgroups a CU; 512 x 14336 x 4096 42 / 42, 2048 x 4096 x 4096 48 / 45, 1024 x 4096 x 4096 30 / 30
+//   256 x 256: 2048 x 4096 x 4096 53 / 48, 4096 x 4096 x 4096 61 / 61, 8192 x 14336 x 4096 379 / 428
+struct Form {
+  int rows, cols;  // of C, before a gated activation halves the columns
+  int rt, ct;      // of the rows kernel; 0: the tiled one
+};
+constexpr Form kForms[] = {{16, 16, 1, 1}, {16, 32, 1, 2}, {16, 64, 1, 4}, {32, 16, 2, 1}, {32, 32, 2, 2},
+                           {32, 64, 2, 4}, {64, 64, 4, 4}, {128, 128, 0, 0}, {256, 256, 0, 0}};
+
+double cost(const Form& f, double tiles, double cus, double k) {
+  k /= 4096.0;
+  const double rounds = tiles / cus;
+  if (f.rt) {
+    const double s = f.rt + f.ct, each = 1.1 * s + 0.08 * s * s;
+    // many small tiles share a CU and cover each other's start and end
+    return 5.0 + k * each * (rounds >= 4.0 ? (s <= 3.0 ? 0.85 * rounds : rounds) : std::ceil(rounds));
+  }
+  if (f.rows == 128) {
+    const double pairs = std::floor(rounds / 2.0), rest = rounds - 2.0 * pairs;
+    return 6.0 + k * (42.0 * pairs + (rest == 0.0 ? 0.0 : rest <= 1.0 ? 21.0 + 3.0 * rest : 6.0 + 18.0 * rest));
+  }
+  return 8.0 + k * std::ceil(rounds) * (37.0 + 16.0 * std::min(1.0, rounds));
+}
+
+// The cheapest form. Of grouped rows the host knows no more than their number: groups of one size are assumed, each
+// with half a tile more than it fills.
+int launch(const Args& a, bool grouped, hipStream_t st) {
+  const bool gated = a.act == PCAMD_ACT_SWIGLU, tiled = tiles_ok(a, grouped);
+  const int found = device_cu_count(st);
+  const double cus = found > 0 ? found : 256.0;
+  const Form* best = nullptr;
+  double least = 0.0;
+  for (const Form& f : kForms) {
+    if ((!f.rt && !tiled) || (gated && f.ct == 1)) continue;
+    const double n = std::ceil(double(a.n) * (gated ? 2 : 1) / f.cols);
+    double m = std::ceil(double(a.m) / f.rows) * a.batch;
+    if (grouped) {
+      const double used = std::max(1, std::min(a.batch, a.pairs));
+      m = used * std::max(1.0, a.pairs / used / f.rows + 0.5);
+    }
+    const double c = cost(f, m * n, cus, a.k);
+    if (!best || c < least) {
+      best = &f;
+      least = c;
+    }
+  }
+  if (best->rt) return launch_rows(a, grouped, best->rt, best->ct, st);
+  return launch_tiles(a, grouped, best->rows == 256, st);
 }
 
 }  // namespace
@@ -59,7 +119,7 @@ extern "C" int pcamd_bmm_int8(const void* a, const void* b, int64_t batch, int64
   x.m = static_cast<int32_t>(m); x.n = static_cast<int32_t>(n); x.k = static_cast<int32_t>(k);
   x.batch = static_cast<int32_t>(batch < INT32_MAX ? batch : INT32_MAX);
   x.c_dtype = c_dtype; x.bias_dtype = bias_dtype; x.act = activation;
-  return int8::launch_rows(x, false, static_cast<hipStream_t>(stream));
+  return int8::launch(x, false, static_cast<hipStream_t>(stream));
 }
 
 extern "C" int pcamd_expert_bmm_int8(const void* a, int64_t a_rows, const void* b, int64_t experts, int64_t n, int64_t k,
@@ -93,5 +153,5 @@ extern "C" int pcamd_expert_bmm_int8(const void* a, int64_t a_rows, const void* 
   x.c_dtype = c_dtype; x.bias_dtype = bias_dtype; x.act = activation;
   x.starts = starts; x.order = order; x.pairs = static_cast<int32_t>(pairs);
   x.choices = static_cast<int32_t>(choices); x.a_rows = static_cast<int32_t>(a_rows);
-  return int8::launch_rows(x, true, static_cast<hipStream_t>(stream));
+  return int8::launch(x, true, static_cast<hipStream_t>(stream));
 }
