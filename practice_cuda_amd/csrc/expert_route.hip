@@ -98,27 +98,45 @@ __global__ __launch_bounds__(kSortThreads) void place_kernel(SortArgs a) {
   extern __shared__ int32_t shared[];
   const int keys = a.experts + 1, bits = 32 - __clz(a.experts);
   int32_t* counts = shared;                       // [waves][keys]: then the next place of each wave and key
-  int32_t* base = shared + kSortWaves * keys;     // [keys]: this chunk's first place of each key
-  int32_t* sums = base + keys;                    // [waves]
+  int32_t* base = shared + kSortWaves * keys;     // [2 keys]: sums over the chunks, then this one's first places
+  int32_t* sums = base + 2 * keys;                // [waves]
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t first = int64_t(blockIdx.x) * a.chunk;
   count_waves<BYTES>(a, first, counts, bits);
-  // all pairs of each key, and those of earlier chunks; keys are spread over the threads, one each and then the next
-  // 1024 (there are at most kMaxExperts + 1)
-  int32_t before[2] = {0, 0}, total[2] = {0, 0};
+  // All pairs of each key, and those of earlier chunks. Several threads share a key where there are few: each sums every
+  // parts-th chunk (131288 pairs of 128 experts, 65 chunks: 22 us with one thread a key).
+  int32_t before[2] = {0, 0}, total[2] = {0, 0};  // of keys threadIdx.x and threadIdx.x + 1024
+  if (a.chunks == 1) {
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    const int e = threadIdx.x + k * kSortThreads;
-    if (e >= keys) continue;
-    if (a.chunks == 1) {
-      for (int w = 0; w < kSortWaves; ++w) total[k] += counts[w * keys + e];
-    } else {
-      for (int c = 0; c < a.chunks; ++c) {
-        const int n = a.counts[int64_t(c) * keys + e];
-        total[k] += n;
-        before[k] += c < static_cast<int>(blockIdx.x) ? n : 0;
-      }
+    for (int k = 0; k < 2; ++k) {
+      const int e = threadIdx.x + k * kSortThreads;
+      for (int w = 0; e < keys && w < kSortWaves; ++w) total[k] += counts[w * keys + e];
     }
+  } else {
+    for (int i = threadIdx.x; i < 2 * keys; i += kSortThreads) base[i] = 0;
+    __syncthreads();
+    const int parts = keys < kSortThreads ? kSortThreads / keys : 1;
+    for (int i = threadIdx.x; i < keys * parts; i += kSortThreads) {
+      const int e = i % keys, part = i / keys;
+      int32_t all = 0, ahead = 0;
+#pragma unroll 8
+      for (int c = part; c < a.chunks; c += parts) {
+        const int n = a.counts[int64_t(c) * keys + e];
+        all += n;
+        ahead += c < static_cast<int>(blockIdx.x) ? n : 0;
+      }
+      atomicAdd(&base[e], all);  // whole numbers: any order
+      atomicAdd(&base[keys + e], ahead);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int e = threadIdx.x + k * kSortThreads;
+      if (e >= keys) continue;
+      total[k] = base[e];
+      before[k] = base[keys + e];
+    }
+    __syncthreads();
   }
   // exclusive sums over the keys
   int32_t start = 0;
@@ -189,7 +207,7 @@ SortPlan sort_plan(int64_t pairs) {
 
 template <int BYTES>
 int sort(SortArgs a, hipStream_t st) {
-  const int lds = (kSortWaves * (a.experts + 1) + (a.experts + 1) + kSortWaves) * 4;
+  const int lds = (kSortWaves * (a.experts + 1) + 2 * (a.experts + 1) + kSortWaves) * 4;
   if (a.chunks > 1) {
     static std::atomic<uint64_t> done{0};
     int rc = ensure_dynamic_lds(reinterpret_cast<const void*>(count_kernel<BYTES>), 80 * 1024, st, done);
@@ -243,7 +261,7 @@ PCAMD_DEV uint32_t pair16(float lo, float hi) {
   }
 }
 
-template <int DT, int V>
+template <int DT, int V, bool NT = false>
 PCAMD_DEV void store_v(void* p, const float (&v)[V]) {
   if constexpr (V == 1) {
     if constexpr (DT == kF32) *static_cast<float*>(p) = v[0];
@@ -258,7 +276,8 @@ PCAMD_DEV void store_v(void* p, const float (&v)[V]) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) w[i] = pair16<DT>(v[2 * i], v[2 * i + 1]);
     }
-    *static_cast<u32x4_t*>(p) = w;
+    if constexpr (NT) __builtin_nontemporal_store(w, static_cast<u32x4_t*>(p));
+    else *static_cast<u32x4_t*>(p) = w;
   }
 }
 
@@ -298,7 +317,7 @@ PCAMD_DEV Place place_at(const RowArgs& a, int64_t t, int j) {
 PCAMD_DEV int64_t token_of() { return int64_t(blockIdx.y) * gridDim.x + blockIdx.x; }
 
 // Rows are moved as words, whatever they hold.
-template <typename W>
+template <typename W, bool NT>
 __global__ __launch_bounds__(kRowThreads) void dispatch_kernel(RowArgs a, int words) {
   const int64_t t = token_of();
   if (t >= a.tokens) return;
@@ -309,7 +328,10 @@ __global__ __launch_bounds__(kRowThreads) void dispatch_kernel(RowArgs a, int wo
       const Place p = place_at(a, t, j);
       W o = v;
       if (!p.used) o = W{};
-      if (p.in) static_cast<W*>(a.out)[p.row * a.so + at] = o;
+      if (!p.in) continue;
+      W* to = static_cast<W*>(a.out) + p.row * a.so + at;
+      if constexpr (NT) __builtin_nontemporal_store(o, to);
+      else *to = o;
     }
   }
 }
@@ -342,7 +364,7 @@ PCAMD_DEV float wave_sum(float v) {
 }
 
 // out: the rows' gradient, or null; the weights' products are summed in a fixed order
-template <int DT, int V>
+template <int DT, int V, bool NT>
 __global__ __launch_bounds__(kRowThreads) void combine_back_kernel(RowArgs a) {
   extern __shared__ float dots[];  // [choices][waves]
   constexpr int kWaves = kRowThreads / 64;
@@ -369,7 +391,7 @@ __global__ __launch_bounds__(kRowThreads) void combine_back_kernel(RowArgs a) {
         float v[V];
 #pragma unroll
         for (int i = 0; i < V; ++i) v[i] = p.used ? w * g[i] : 0.0f;
-        store_v<DT, V>(static_cast<uint8_t*>(a.out) + (p.row * a.so + at) * elem_bytes<DT>(), v);
+        store_v<DT, V, NT>(static_cast<uint8_t*>(a.out) + (p.row * a.so + at) * elem_bytes<DT>(), v);
       }
       if (a.grad_weights && p.used) {
         float dot = 0.0f;
@@ -393,6 +415,12 @@ __global__ __launch_bounds__(kRowThreads) void combine_back_kernel(RowArgs a) {
     }
   }
 }
+
+// Rows that the 256 MB cache behind the L2 cannot hold for their reader go past it.
+constexpr int64_t kStream = 128 << 20;
+bool streams(int64_t bytes) { return bytes > kStream; }
+template <int DT>
+constexpr int64_t elem_size() { return DT == kF32 ? 4 : 2; }
 
 // One workgroup a token, cut along the row where tokens are few.
 dim3 row_grid(int64_t tokens, int64_t pieces, bool cut) {
@@ -437,8 +465,9 @@ int combine_back(const RowArgs& a, bool wide, hipStream_t st) {
   constexpr int V = DT == kF32 ? 4 : 8;
   const int lds = a.choices * (kRowThreads / 64) * 4;
   const dim3 grid = row_grid(a.tokens, 1, false);
-  if (wide) combine_back_kernel<DT, V><<<grid, kRowThreads, lds, st>>>(a);
-  else combine_back_kernel<DT, 1><<<grid, kRowThreads, lds, st>>>(a);
+  if (!wide) combine_back_kernel<DT, 1, false><<<grid, kRowThreads, lds, st>>>(a);
+  else if (streams(a.pairs * a.width * elem_size<DT>())) combine_back_kernel<DT, V, true><<<grid, kRowThreads, lds, st>>>(a);
+  else combine_back_kernel<DT, V, false><<<grid, kRowThreads, lds, st>>>(a);
   return check_launch("combine_back_kernel");
 }
 
@@ -492,9 +521,11 @@ extern "C" int pcamd_expert_dispatch(const void* x, int dtype, int64_t tokens, i
   a.sx = sxt * size / bytes;
   a.so = sos * size / bytes;
   const dim3 grid = route::row_grid(tokens, (words + route::kRowThreads - 1) / route::kRowThreads, true);
-  if (wide) route::dispatch_kernel<u32x4_t><<<grid, route::kRowThreads, 0, st>>>(a, words);
-  else if (size == 4) route::dispatch_kernel<uint32_t><<<grid, route::kRowThreads, 0, st>>>(a, words);
-  else route::dispatch_kernel<uint16_t><<<grid, route::kRowThreads, 0, st>>>(a, words);
+  if (wide && route::streams(a.pairs * width * size))
+    route::dispatch_kernel<u32x4_t, true><<<grid, route::kRowThreads, 0, st>>>(a, words);
+  else if (wide) route::dispatch_kernel<u32x4_t, false><<<grid, route::kRowThreads, 0, st>>>(a, words);
+  else if (size == 4) route::dispatch_kernel<uint32_t, false><<<grid, route::kRowThreads, 0, st>>>(a, words);
+  else route::dispatch_kernel<uint16_t, false><<<grid, route::kRowThreads, 0, st>>>(a, words);
   return check_launch("dispatch_kernel");
 }
 

@@ -1,6 +1,4 @@
 // int8_bmm.hip - C entries of the int8 products (int8_bmm.h) and the choice of kernel.
-
-
 #include <algorithm>
 #include <cmath>
 
