@@ -174,3 +174,11 @@ def test_entry_refusals():
     says(grouped(starts=None), -1, b"null")
     says(grouped(sam=24), -1, b"rows of a")
     assert grouped(a_rows=0, pairs=0) == 0
+
+
+def test_row_entries_refuse_the_widest_rows():
+    """A thread steps on past the row's end by up to 64 * 256 columns, which has to fit 32 bits."""
+    L = _lib.lib()
+    for width, rc in ((2**31 - 65537, -1), (2**31 - 65536, -2), (2**31 - 8192, -2)):  # -1: null pointers, seen later
+        assert L.pcamd_expert_dispatch(None, _lib.BF16, 1, 1, width, width, FAKE, None, width, None) == rc
+        assert L.pcamd_expert_combine(None, _lib.BF16, 1, 1, width, width, FAKE, FAKE, 0, None, width, None) == rc
