@@ -415,9 +415,10 @@ int pcamd_latent_prefill(const void *q, const void *k_nope, const void *k_rope,
  * scale[b, i] = top / 127 (fp32 division), y = rint(127 x / top) of the real
  * quotient, ties to even. A row with a NaN or an infinity gets the scale NaN
  * and codes of zero. Rows of y are 16-byte aligned and written up to the next
- * multiple of 16 bytes, with zeros behind n. Available from PCAMD_ABI_VERSION
- * 7, as the functions below. No counterpart in the reference, whose quantizers
- * are fp8 (fp8_training/fp8_bench/impls/triton_per_channel.py:90-219).
+ * multiple of 16 bytes, with zeros behind n. n is at most 2^31 - 16385.
+ * Available from PCAMD_ABI_VERSION 7, as the functions below. No counterpart in
+ * the reference, whose quantizers are fp8
+ * (fp8_training/fp8_bench/impls/triton_per_channel.py:90-219).
  */
 int pcamd_quant_int8(const void *x, int x_dtype, int64_t batch, int64_t m,
                      int64_t n, int64_t sxb, int64_t sxm, void *y, int64_t syb,

@@ -232,8 +232,9 @@ extern "C" int pcamd_quant_int8(const void* x, int x_dtype, int64_t batch, int64
   if (reinterpret_cast<uintptr_t>(x) % size) return set_error(PCAMD_ERR_INVALID, "x is not aligned to its elements");
   if ((reinterpret_cast<uintptr_t>(y) & 15) || (m > 1 && sym % 16) || (batch > 1 && syb % 16))
     return set_error(PCAMD_ERR_INVALID, "rows of codes must be 16-byte aligned");
-  if (m > INT32_MAX || n > INT32_MAX - 16 || batch > INT32_MAX / m)
-    return set_error(PCAMD_ERR_UNSUPPORTED, "int8 quant: more than 2^31 - 1 rows or columns");
+  // a thread's place in a long row steps on by 1024 * 8 values, past the row's end, in 32 bits
+  if (m > INT32_MAX || n > INT32_MAX - 16384 || batch > INT32_MAX / m)
+    return set_error(PCAMD_ERR_UNSUPPORTED, "int8 quant: more than 2^31 - 1 rows or 2^31 - 16385 columns");
   int8q::Args a{x, static_cast<int8_t*>(y), scale, sxb, sxm, syb, sym, ssb, ssm, batch * m, static_cast<int32_t>(m),
                 static_cast<int32_t>(n), eps};
   hipStream_t st = static_cast<hipStream_t>(stream);

@@ -33,7 +33,7 @@ def hip_int8_quant(x: torch.Tensor, *, channel_axis: int = -2, eps: float = 1e-1
     channel_axis=-2: one scale per row, x contiguous along N (a product's left
     operand); -1: one per column, x contiguous along M (its right operand: a
     weight [.., N, K] passed as ``w.transpose(-1, -2)``). Rows (columns) may
-    have any strides and length. The codes lie as x does, each row (column) at
+    have any strides, and up to 2^31 - 16385 values. The codes lie as x does, each row (column) at
     a multiple of 16 bytes, so the result may be a view of padded memory; eps is
     the floor of a row's maximum. A row with a NaN or an infinity gets codes of
     zero and a scale of NaN, which makes its products NaN. There is no gradient:
