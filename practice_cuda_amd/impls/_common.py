@@ -10,6 +10,7 @@ from __future__ import annotations
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from .. import _lib
 from ..registry import QuantResult
@@ -17,6 +18,13 @@ from ..registry import QuantResult
 _INPUT_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 _FP8_DTYPES = (torch.float8_e4m3fn, torch.float8_e5m2)
 _OUT_DTYPES = (torch.bfloat16, torch.float16, torch.float32, torch.float8_e4m3fn, torch.float8_e5m2)
+
+
+def has_tangent(*tensors: Optional[torch.Tensor]) -> bool:
+    """Whether one of the tensors carries a forward-mode tangent. Its requires_grad need not say so, and the kernels
+    read its values alone. Outside of any dual level this is one comparison."""
+    return forward_ad._current_level >= 0 and any(
+        t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 class _Inference(torch.autograd.Function):

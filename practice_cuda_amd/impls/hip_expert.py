@@ -127,29 +127,64 @@ def _rows_major(grad: torch.Tensor) -> torch.Tensor:
     return grad if grad.stride(1) == 1 or grad.shape[1] <= 1 else grad.contiguous()
 
 
+def _tangent(t: torch.Tensor, like: torch.Tensor) -> torch.Tensor:
+    """A tangent as a tensor that a kernel can read: of its input's type, rows contiguous, no lazy zeros or signs."""
+    if t._is_zerotensor():
+        return torch.zeros(like.shape, dtype=like.dtype, device=like.device)
+    return _rows_major(t.resolve_neg().to(like.dtype))
+
+
+def _refuse_tangents(what: str, *tensors: Optional[torch.Tensor]) -> None:
+    if C.has_tangent(*tensors):
+        raise RuntimeError(f"the gradient of {what} has no forward-mode derivative")
+
+
 class _Dispatch(torch.autograd.Function):
+    """Linear, so a tangent is dispatched like its tokens; and with the forward-mode inputs off in jvp, the calls
+    made there can be differentiated backward."""
+
     @staticmethod
     def forward(ctx, x, place):
+        ctx.set_materialize_grads(False)
         ctx.save_for_backward(place)
+        ctx.save_for_forward(place)
         return _dispatch(x, place)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
+        if grad is None:
+            return None, None
+        _refuse_tangents("expert_dispatch", grad)
         place, = ctx.saved_tensors
         return _combine(_rows_major(grad), place, None), None
 
+    @staticmethod
+    def jvp(ctx, x_t, _):
+        place, = ctx.saved_tensors
+        return _Dispatch.apply(_tangent(x_t, x_t), place)
+
 
 class _Combine(torch.autograd.Function):
+    """Linear in rows and in weights: the tangent is combine of the rows' with the weights, plus combine of the rows
+    with the weights'. Each is rounded to the rows' type before they are added (and the sum once more): two calls of
+    the one kernel, at up to three half steps."""
+
     @staticmethod
     def forward(ctx, rows, weights, place):
+        ctx.set_materialize_grads(False)
         ctx.save_for_backward(rows, weights, place)
+        ctx.save_for_forward(rows, weights, place)
         return _combine(rows, place, weights)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
+        if grad is None:
+            return None, None, None
         rows, weights, place = ctx.saved_tensors
+        _refuse_tangents("expert_combine", grad, weights if ctx.needs_input_grad[0] else None,
+                         rows if ctx.needs_input_grad[1] else None)
         grad = _rows_major(grad)
         tokens, choices = place.shape
         width = rows.shape[1]
@@ -169,18 +204,29 @@ class _Combine(torch.autograd.Function):
             to_weights = to_weights.to(weights.dtype)
         return to_rows, to_weights, None
 
+    @staticmethod
+    def jvp(ctx, rows_t, weights_t, _):
+        rows, weights, place = ctx.saved_tensors
+        parts = []
+        if rows_t is not None:
+            parts.append(_Combine.apply(_tangent(rows_t, rows), weights, place))
+        if weights_t is not None:
+            parts.append(_Combine.apply(rows, _tangent(weights_t, weights).contiguous(), place))
+        return parts[0] if len(parts) == 1 else parts[0] + parts[1]
+
 
 def hip_expert_dispatch(x: torch.Tensor, plan: ExpertPlan) -> torch.Tensor:
     """The rows of x [T, H] in the plan's order: [T * k, H], row s that of pair order[s].
 
     float32, bfloat16 or float16, contiguous along H, any row stride; places of
     pairs without an expert get zeros. The gradient of a token is the sum over
-    its choices, in fp32, rounded once."""
+    its choices, in fp32, rounded once. A forward-mode tangent is dispatched as x
+    is; the gradient itself has none."""
     _check_rows(x, "x", plan.place.shape[0])
     _check_place(plan, x.device)
     if not x.is_cuda:
         _lib.require_gpu_tensor(x, "x")
-    if x.requires_grad and torch.is_grad_enabled():
+    if x.requires_grad and torch.is_grad_enabled() or C.has_tangent(x):
         return _Dispatch.apply(x, plan.place)
     return _dispatch(x, plan.place)
 
@@ -193,7 +239,8 @@ def hip_expert_combine(rows: torch.Tensor, plan: ExpertPlan, weights: torch.Tens
     contiguous. Sums are fp32, over the choices in their order, rounded once to
     the rows' type; pairs without an expert are left out. Gradients: of rows
     (zeros at places of pairs without an expert) and of weights (summed in fp32
-    in a fixed order)."""
+    in a fixed order). Forward-mode tangents of both go through; the gradients
+    themselves have none."""
     pairs, device = plan.place.numel(), rows.device
     _check_rows(rows, "rows", pairs)
     _check_place(plan, device)
@@ -203,7 +250,7 @@ def hip_expert_combine(rows: torch.Tensor, plan: ExpertPlan, weights: torch.Tens
                          f"{device}, got {weights.dtype}, {tuple(weights.shape)} on {weights.device}")
     if not rows.is_cuda:
         _lib.require_gpu_tensor(rows, "rows")
-    if (rows.requires_grad or weights.requires_grad) and torch.is_grad_enabled():
+    if (rows.requires_grad or weights.requires_grad) and torch.is_grad_enabled() or C.has_tangent(rows, weights):
         return _Combine.apply(rows, weights, plan.place)
     return _combine(rows, plan.place, weights)
 
