@@ -274,7 +274,7 @@ def hip_expert_bmm(
     writing them). Both as hip_int8_quant leaves them; bias: [experts, N], any
     strides; activations as hip_int8_bmm's. Returns [T * k, N] (N / 2 for
     "swiglu"): row s is that of pair order[s], and rows of pairs without an
-    expert are zeros. There is no gradient."""
+    expert are zeros. There is no gradient: going backward is an error."""
     at, bt = a.tensor, b.tensor
     if at.ndim != 2 or bt.ndim != 3:
         raise ValueError(f"A must be [rows, K] and B [experts, K, N], got {tuple(at.shape)} and {tuple(bt.shape)}")
@@ -298,7 +298,9 @@ def hip_expert_bmm(
                              or bias.device != device):
         raise ValueError(f"bias must be float32, bfloat16 or float16 {(experts, cols)} on {device}, got {bias.dtype}, "
                          f"{tuple(bias.shape)} on {bias.device}")
-    record = bias is not None and bias.requires_grad and torch.is_grad_enabled()
+    sa, sb = a.dequant_scale, b.dequant_scale
+    record = ((sa.requires_grad or sb.requires_grad or bias is not None and bias.requires_grad)
+              and torch.is_grad_enabled())
     if out is not None:
         if out.shape != (pairs, n) or out.dtype != out_dtype or out.device != device:
             raise ValueError(f"out must be {out_dtype} with shape {(pairs, n)} on {device}, got {out.dtype}, "
@@ -310,7 +312,6 @@ def hip_expert_bmm(
     _lib.require_gpu_tensor(at, "A")
     if out is None:
         out = torch.empty((pairs, n), dtype=out_dtype, device=device)
-    sa, sb = a.dequant_scale, b.dequant_scale
     s_b, s_sb = bt.stride(), sb.stride()
     s_bias = (0, 0) if bias is None else bias.stride()
     rc = _lib.launch(
@@ -323,5 +324,5 @@ def hip_expert_bmm(
     if rc != 0:
         _refused(rc, "pcamd_expert_bmm_int8")
     if record:
-        out, = C.without_gradient("expert_bmm", (bias,), out)
+        out, = C.without_gradient("expert_bmm", (sa, sb, bias), out)
     return out

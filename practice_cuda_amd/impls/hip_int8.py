@@ -120,7 +120,8 @@ def hip_int8_bmm(
     bytes, as hip_int8_quant leaves them; K up to 131071, where the sums are
     exact. bias: [B, M, N], any strides. activation: "none", "gelu", or "swiglu",
     which takes the first half of b's columns as gates of the second: silu(gate)
-    * other, [B, M, N / 2] (bias still has N columns). There is no gradient."""
+    * other, [B, M, N / 2] (bias still has N columns). There is no gradient: going
+    backward is an error."""
     at, bt = a.tensor, b.tensor
     if at.ndim != 3 or bt.ndim != 3:
         raise ValueError("BMM expects 3D quantized tensors")
@@ -137,10 +138,12 @@ def hip_int8_bmm(
         out = C.prepare_out(out, out_dtype, batch, m, n, at.device)
     bias, bias_strides, bias_code = C.check_bias(bias, batch, m, cols, at.device, require_n_contiguous=False)
     _lib.require_gpu_tensor(at, "A")
-    record = bias is not None and bias.requires_grad and torch.is_grad_enabled()
+    sa, sb = a.dequant_scale, b.dequant_scale
+    # the scales of a quantized input stand for it: its codes are whole numbers, which require no gradient
+    record = ((sa.requires_grad or sb.requires_grad or bias is not None and bias.requires_grad)
+              and torch.is_grad_enabled())
     if record and given:
         C.refuse_recorded("int8_bmm", "out")
-    sa, sb = a.dequant_scale, b.dequant_scale
     s_a, s_b, s_c, s_sa, s_sb = at.stride(), bt.stride(), out.stride(), sa.stride(), sb.stride()
     rc = _lib.launch(
         _lib.lib().pcamd_bmm_int8, at,
@@ -150,5 +153,5 @@ def hip_int8_bmm(
     if rc != 0:
         _refused(rc, "pcamd_bmm_int8")
     if record:
-        out, = C.without_gradient("int8_bmm", (bias,), out)
+        out, = C.without_gradient("int8_bmm", (sa, sb, bias), out)
     return out
