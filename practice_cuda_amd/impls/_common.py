@@ -48,6 +48,11 @@ def without_gradient(what: str, inputs, *outputs: Optional[torch.Tensor]):
     return tuple(None if t is None else next(new) for t in outputs)
 
 
+def refuse_tangents(what: str, *tensors: Optional[torch.Tensor]) -> None:
+    if has_tangent(*tensors):
+        raise RuntimeError(f"{what} has no forward-mode derivative")
+
+
 def refuse_recorded(what: str, written: str) -> None:
     raise ValueError(f"{what}: an input requires a gradient, which {written} cannot carry; call it under "
                      "torch.no_grad() or with detached inputs")

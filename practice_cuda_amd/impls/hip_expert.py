@@ -134,11 +134,6 @@ def _tangent(t: torch.Tensor, like: torch.Tensor) -> torch.Tensor:
     return _rows_major(t.resolve_neg().to(like.dtype))
 
 
-def _refuse_tangents(what: str, *tensors: Optional[torch.Tensor]) -> None:
-    if C.has_tangent(*tensors):
-        raise RuntimeError(f"the gradient of {what} has no forward-mode derivative")
-
-
 class _Dispatch(torch.autograd.Function):
     """Linear, so a tangent is dispatched like its tokens; and with the forward-mode inputs off in jvp, the calls
     made there can be differentiated backward."""
@@ -155,7 +150,7 @@ class _Dispatch(torch.autograd.Function):
     def backward(ctx, grad):
         if grad is None:
             return None, None
-        _refuse_tangents("expert_dispatch", grad)
+        C.refuse_tangents("expert_dispatch's gradient", grad)
         place, = ctx.saved_tensors
         return _combine(_rows_major(grad), place, None), None
 
@@ -183,8 +178,8 @@ class _Combine(torch.autograd.Function):
         if grad is None:
             return None, None, None
         rows, weights, place = ctx.saved_tensors
-        _refuse_tangents("expert_combine", grad, weights if ctx.needs_input_grad[0] else None,
-                         rows if ctx.needs_input_grad[1] else None)
+        C.refuse_tangents("expert_combine's gradient", grad, weights if ctx.needs_input_grad[0] else None,
+                          rows if ctx.needs_input_grad[1] else None)
         grad = _rows_major(grad)
         tokens, choices = place.shape
         width = rows.shape[1]
@@ -301,6 +296,7 @@ def hip_expert_bmm(
     sa, sb = a.dequant_scale, b.dequant_scale
     record = ((sa.requires_grad or sb.requires_grad or bias is not None and bias.requires_grad)
               and torch.is_grad_enabled())
+    C.refuse_tangents("expert_bmm", sa, sb, bias)
     if out is not None:
         if out.shape != (pairs, n) or out.dtype != out_dtype or out.device != device:
             raise ValueError(f"out must be {out_dtype} with shape {(pairs, n)} on {device}, got {out.dtype}, "

@@ -53,6 +53,7 @@ def hip_int8_quant(x: torch.Tensor, *, channel_axis: int = -2, eps: float = 1e-1
     if strides[-1] != 1 and n > 1:
         raise ValueError(f"x must be contiguous along the dimension that its scales are for all of (channel_axis="
                          f"{channel_axis}); shape={tuple(shape)}, strides={x.stride()}")
+    C.refuse_tangents("int8_quant", x)
     if not x.is_cuda:
         _lib.require_gpu_tensor(x, "x")
     flat = len(shape) == 2
@@ -137,6 +138,7 @@ def hip_int8_bmm(
     if given or at.is_cuda:
         out = C.prepare_out(out, out_dtype, batch, m, n, at.device)
     bias, bias_strides, bias_code = C.check_bias(bias, batch, m, cols, at.device, require_n_contiguous=False)
+    C.refuse_tangents("int8_bmm", a.dequant_scale, b.dequant_scale, bias)
     _lib.require_gpu_tensor(at, "A")
     sa, sb = a.dequant_scale, b.dequant_scale
     # the scales of a quantized input stand for it: its codes are whole numbers, which require no gradient

@@ -150,6 +150,7 @@ def hip_latent_append(
             raise ValueError(f"weight must be on {device}, got {weight.device}")
     if eps < 0 or norm_eps < 0:
         raise ValueError(f"eps and norm_eps must not be negative, got {eps} and {norm_eps}")
+    C.refuse_tangents("latent_append", latent, rope, weight)
     if not latent.is_cuda:
         _lib.require_gpu_tensor(latent, "latent")
     if ((latent.requires_grad or rope.requires_grad or weight is not None and weight.requires_grad)
@@ -242,6 +243,7 @@ def hip_latent_decode(
             or batch > 1 and seq_lens.stride(0) != 1):
         raise ValueError(f"seq_lens must be contiguous int32 with shape ({batch},) on {device}; "
                          f"got {seq_lens.dtype}, {tuple(seq_lens.shape)}, {seq_lens.device}")
+    C.refuse_tangents("latent_decode", q_latent, q_rope)
     record = (q_latent.requires_grad or q_rope.requires_grad) and torch.is_grad_enabled()
     if record and out is not None:
         C.refuse_recorded("latent_decode", "out")
@@ -338,6 +340,7 @@ def hip_latent_prefill(
                 or t.stride(0) != 1):
             raise ValueError(f"cu_q and cu_k must be contiguous int32 [n + 1] on {device}; {name} is {t.dtype}, "
                              f"{tuple(t.shape)}, {t.device}")
+    C.refuse_tangents("latent_prefill", q, k_nope, k_rope, v)
     record = ((q.requires_grad or k_nope.requires_grad or k_rope.requires_grad or v.requires_grad)
               and torch.is_grad_enabled())
     if record and out is not None:

@@ -73,6 +73,7 @@ def hip_rms_norm_quant(
             residual_out = torch.empty(shape, dtype=dtype, device=device)
         residual_args = _like(residual, "residual", shape, dtype, device, flat)
         out_args = _like(residual_out, "residual_out", shape, dtype, device, flat)
+    C.refuse_tangents("rms_norm_quant", x, weight, residual)
     if not x.is_cuda:
         _lib.require_gpu_tensor(x, "x")
     record = ((x.requires_grad or weight.requires_grad or residual is not None and residual.requires_grad)
