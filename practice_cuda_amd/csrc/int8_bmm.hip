@@ -130,6 +130,7 @@ extern "C" int pcamd_expert_bmm_int8(const void* a, int64_t a_rows, const void* 
   int rc = int8::check_common(n, k, c_dtype, bias, bias_dtype, activation);
   if (rc != PCAMD_OK) return rc;
   if (pairs < 0 || experts < 0 || a_rows < 0) return set_error(PCAMD_ERR_INVALID, "negative size");
+  if (pairs == 0 && choices == 0) return PCAMD_OK;  // tokens, if any, without a choice: no rows
   if (order ? choices < 1 || a_rows > pairs || (a_rows && pairs / a_rows < choices) || a_rows * choices != pairs
             : a_rows != pairs)
     return set_error(PCAMD_ERR_INVALID, "a has %lld rows, which do not go with %lld pairs", (long long)a_rows,
