@@ -49,6 +49,37 @@ int pcamd_selftest_copy16(const void *x, void *y, int64_t bytes, void *stream);
  */
 int pcamd_selftest_narrow16(const void *x, void *y, int64_t in_bytes, void *stream);
 
+/*
+ * pcamd_bmm_int8 and pcamd_expert_bmm_int8 (pcamd_fp8.h) in one of the forms
+ * that these choose from by size, so that the tests reach each form at any
+ * size: 0 to 6 the kernel of few rows with tiles of 16 x 16, 16 x 32, 16 x 64,
+ * 32 x 16, 32 x 32, 32 x 64 and 64 x 64, 7 and 8 the kernel of many rows with
+ * 128 x 128 and 256 x 256; -1: as the product entries choose. A form that does
+ * not take the call (the gated activation in forms 0 and 3, no inner size or
+ * operands of 4 GiB in 7 and 8) returns PCAMD_ERR_UNSUPPORTED.
+ */
+int pcamd_selftest_bmm_int8(int form, const void *a, const void *b,
+                            int64_t batch, int64_t m, int64_t n, int64_t k,
+                            int64_t sab, int64_t sam, int64_t sbb, int64_t sbn,
+                            void *c, int c_dtype, int64_t scb, int64_t scm,
+                            const void *bias, int bias_dtype, int64_t sbiasb,
+                            int64_t sbiasm, int64_t sbiasn, const float *sa,
+                            int64_t ssab, int64_t ssam, const float *sb,
+                            int64_t ssbb, int64_t ssbn, int activation,
+                            void *stream);
+int pcamd_selftest_expert_bmm_int8(int form, const void *a, int64_t a_rows,
+                                   const void *b, int64_t experts, int64_t n,
+                                   int64_t k, int64_t sam, int64_t sbe,
+                                   int64_t sbn, void *c, int c_dtype,
+                                   int64_t scm, const void *bias,
+                                   int bias_dtype, int64_t sbiase,
+                                   int64_t sbiasn, const float *sa,
+                                   int64_t ssam, const float *sb, int64_t ssbe,
+                                   int64_t ssbn, const int32_t *starts,
+                                   const int32_t *order, int64_t pairs,
+                                   int64_t choices, int activation,
+                                   void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -65,7 +65,8 @@ EXPORTED_SYMBOLS = (
     "pcamd_expert_bmm_int8",
 )
 # test-only entry points (include/pcamd_fp8_selftest.h), exported by the same library
-TEST_SYMBOLS = ("pcamd_selftest_fp8_convert", "pcamd_selftest_copy16", "pcamd_selftest_narrow16")
+TEST_SYMBOLS = ("pcamd_selftest_fp8_convert", "pcamd_selftest_copy16", "pcamd_selftest_narrow16",
+                "pcamd_selftest_bmm_int8", "pcamd_selftest_expert_bmm_int8")
 
 _i64 = ctypes.c_int64
 _int = ctypes.c_int
@@ -160,6 +161,9 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.pcamd_expert_bmm_int8.argtypes = (
         [_ptr, _i64, _ptr] + [_i64] * 6 + [_ptr, _int, _i64] + [_ptr, _int, _i64, _i64] + [_ptr, _i64]
         + [_ptr, _i64, _i64] + [_ptr, _ptr, _i64, _i64] + [_int, _ptr])
+    for name in ("bmm_int8", "expert_bmm_int8"):
+        product, test = getattr(lib, f"pcamd_{name}"), getattr(lib, f"pcamd_selftest_{name}")
+        test.restype, test.argtypes = _int, [_int, *product.argtypes]
     lib.pcamd_selftest_fp8_convert.restype = _int
     lib.pcamd_selftest_fp8_convert.argtypes = [_int, _ptr, _ptr]
     lib.pcamd_selftest_copy16.restype = _int

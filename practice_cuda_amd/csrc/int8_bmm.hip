@@ -43,6 +43,7 @@ struct Form {
   int rows, cols;  // of C, before a gated activation halves the columns
   int rt, ct;      // of the rows kernel; 0: the tiled one
 };
+// in the order that the test entries count in
 constexpr Form kForms[] = {{16, 16, 1, 1}, {16, 32, 1, 2}, {16, 64, 1, 4}, {32, 16, 2, 1}, {32, 32, 2, 2},
                            {32, 64, 2, 4}, {64, 64, 4, 4}, {128, 128, 0, 0}, {256, 256, 0, 0}};
 
@@ -61,16 +62,16 @@ double cost(const Form& f, double tiles, double cus, double k) {
   return 8.0 + k * std::ceil(rounds) * (37.0 + 16.0 * std::min(1.0, rounds));
 }
 
-// The cheapest form. Of grouped rows the host knows no more than their number: groups of one size are assumed, each
-// with half a tile more than it fills.
-int launch(const Args& a, bool grouped, hipStream_t st) {
+// The cheapest form, or the one with the given place in kForms. Of grouped rows the host knows no more than their
+// number: groups of one size are assumed, each with half a tile more than it fills.
+int launch(const Args& a, bool grouped, int form, hipStream_t st) {
   const bool gated = a.act == PCAMD_ACT_SWIGLU, tiled = tiles_ok(a, grouped);
   const int found = device_cu_count(st);
   const double cus = found > 0 ? found : 256.0;
   const Form* best = nullptr;
   double least = 0.0;
   for (const Form& f : kForms) {
-    if ((!f.rt && !tiled) || (gated && f.ct == 1)) continue;
+    if ((!f.rt && !tiled) || (gated && f.ct == 1) || (form >= 0 && &f - kForms != form)) continue;
     const double n = std::ceil(double(a.n) * (gated ? 2 : 1) / f.cols);
     double m = std::ceil(double(a.m) / f.rows) * a.batch;
     if (grouped) {
@@ -83,33 +84,28 @@ int launch(const Args& a, bool grouped, hipStream_t st) {
       least = c;
     }
   }
+  if (!best) return set_error(PCAMD_ERR_UNSUPPORTED, "int8 product: form %d does not take this call", form);
   if (best->rt) return launch_rows(a, grouped, best->rt, best->ct, st);
   return launch_tiles(a, grouped, best->rows == 256, st);
 }
 
-}  // namespace
-}  // namespace int8
-}  // namespace pcamd
-
-extern "C" int pcamd_bmm_int8(const void* a, const void* b, int64_t batch, int64_t m, int64_t n, int64_t k, int64_t sab,
-                              int64_t sam, int64_t sbb, int64_t sbn, void* c, int c_dtype, int64_t scb, int64_t scm,
-                              const void* bias, int bias_dtype, int64_t sbiasb, int64_t sbiasm, int64_t sbiasn,
-                              const float* sa, int64_t ssab, int64_t ssam, const float* sb, int64_t ssbb, int64_t ssbn,
-                              int activation, void* stream) {
-  using namespace pcamd;
+int bmm(int form, const void* a, const void* b, int64_t batch, int64_t m, int64_t n, int64_t k, int64_t sab,
+        int64_t sam, int64_t sbb, int64_t sbn, void* c, int c_dtype, int64_t scb, int64_t scm, const void* bias,
+        int bias_dtype, int64_t sbiasb, int64_t sbiasm, int64_t sbiasn, const float* sa, int64_t ssab, int64_t ssam,
+        const float* sb, int64_t ssbb, int64_t ssbn, int activation, void* stream) {
   clear_error();
-  int rc = int8::check_common(n, k, c_dtype, bias, bias_dtype, activation);
+  int rc = check_common(n, k, c_dtype, bias, bias_dtype, activation);
   if (rc != PCAMD_OK) return rc;
   if (batch < 0 || m < 0) return set_error(PCAMD_ERR_INVALID, "negative size");
   if (batch == 0 || m == 0 || n == 0) return PCAMD_OK;
   if (!c || !sa || !sb || (k && (!a || !b))) return set_error(PCAMD_ERR_INVALID, "null pointer");
   const int64_t cols = activation == PCAMD_ACT_SWIGLU ? 2 * n : n;
-  if ((rc = int8::check_operand("a", a, m, sam, k)) != PCAMD_OK) return rc;
-  if ((rc = int8::check_operand("b", b, cols, sbn, k)) != PCAMD_OK) return rc;
+  if ((rc = check_operand("a", a, m, sam, k)) != PCAMD_OK) return rc;
+  if ((rc = check_operand("b", b, cols, sbn, k)) != PCAMD_OK) return rc;
   if (k && batch > 1 && (sab % 16 || sbb % 16))
     return set_error(PCAMD_ERR_INVALID, "matrices must start at multiples of 16 bytes");
   if (m > INT32_MAX - 65536) return set_error(PCAMD_ERR_UNSUPPORTED, "int8 product: too many rows");
-  int8::Args x{};
+  Args x{};
   x.a = static_cast<const int8_t*>(a); x.b = static_cast<const int8_t*>(b); x.c = c; x.bias = bias; x.sa = sa; x.sb = sb;
   x.sab = sab; x.lda = m > 1 ? sam : 0; x.sbb = sbb; x.ldb = cols > 1 ? sbn : 0; x.scb = scb; x.scm = scm;
   x.sbiasb = sbiasb; x.sbiasm = sbiasm; x.sbiasn = sbiasn;
@@ -117,17 +113,16 @@ extern "C" int pcamd_bmm_int8(const void* a, const void* b, int64_t batch, int64
   x.m = static_cast<int32_t>(m); x.n = static_cast<int32_t>(n); x.k = static_cast<int32_t>(k);
   x.batch = static_cast<int32_t>(batch < INT32_MAX ? batch : INT32_MAX);
   x.c_dtype = c_dtype; x.bias_dtype = bias_dtype; x.act = activation;
-  return int8::launch(x, false, static_cast<hipStream_t>(stream));
+  return launch(x, false, form, static_cast<hipStream_t>(stream));
 }
 
-extern "C" int pcamd_expert_bmm_int8(const void* a, int64_t a_rows, const void* b, int64_t experts, int64_t n, int64_t k,
-                                     int64_t sam, int64_t sbe, int64_t sbn, void* c, int c_dtype, int64_t scm,
-                                     const void* bias, int bias_dtype, int64_t sbiase, int64_t sbiasn, const float* sa,
-                                     int64_t ssam, const float* sb, int64_t ssbe, int64_t ssbn, const int32_t* starts,
-                                     const int32_t* order, int64_t pairs, int64_t choices, int activation, void* stream) {
-  using namespace pcamd;
+int expert_bmm(int form, const void* a, int64_t a_rows, const void* b, int64_t experts, int64_t n, int64_t k,
+               int64_t sam, int64_t sbe, int64_t sbn, void* c, int c_dtype, int64_t scm, const void* bias,
+               int bias_dtype, int64_t sbiase, int64_t sbiasn, const float* sa, int64_t ssam, const float* sb,
+               int64_t ssbe, int64_t ssbn, const int32_t* starts, const int32_t* order, int64_t pairs,
+               int64_t choices, int activation, void* stream) {
   clear_error();
-  int rc = int8::check_common(n, k, c_dtype, bias, bias_dtype, activation);
+  int rc = check_common(n, k, c_dtype, bias, bias_dtype, activation);
   if (rc != PCAMD_OK) return rc;
   if (pairs < 0 || experts < 0 || a_rows < 0) return set_error(PCAMD_ERR_INVALID, "negative size");
   if (pairs == 0 && choices == 0) return PCAMD_OK;  // tokens, if any, without a choice: no rows
@@ -139,12 +134,12 @@ extern "C" int pcamd_expert_bmm_int8(const void* a, int64_t a_rows, const void* 
   if (!c || !sa || !starts || (experts && (!sb || (k && (!a || !b)))))
     return set_error(PCAMD_ERR_INVALID, "null pointer");
   const int64_t cols = activation == PCAMD_ACT_SWIGLU ? 2 * n : n;
-  if ((rc = int8::check_operand("a", a, a_rows, sam, k)) != PCAMD_OK) return rc;
-  if ((rc = int8::check_operand("b", b, cols, sbn, k)) != PCAMD_OK) return rc;
+  if ((rc = check_operand("a", a, a_rows, sam, k)) != PCAMD_OK) return rc;
+  if ((rc = check_operand("b", b, cols, sbn, k)) != PCAMD_OK) return rc;
   if (k && experts > 1 && sbe % 16) return set_error(PCAMD_ERR_INVALID, "matrices must start at multiples of 16 bytes");
   if (pairs > INT32_MAX - 65536 || experts > 65535)
     return set_error(PCAMD_ERR_UNSUPPORTED, "int8 product: too many pairs or experts");
-  int8::Args x{};
+  Args x{};
   x.a = static_cast<const int8_t*>(a); x.b = static_cast<const int8_t*>(b); x.c = c; x.bias = bias; x.sa = sa; x.sb = sb;
   x.lda = a_rows > 1 ? sam : 0; x.sbb = sbe; x.ldb = cols > 1 ? sbn : 0; x.scm = scm;
   x.sbiasb = sbiase; x.sbiasn = sbiasn; x.ssam = ssam; x.ssbb = ssbe; x.ssbn = ssbn;
@@ -152,5 +147,51 @@ extern "C" int pcamd_expert_bmm_int8(const void* a, int64_t a_rows, const void* 
   x.c_dtype = c_dtype; x.bias_dtype = bias_dtype; x.act = activation;
   x.starts = starts; x.order = order; x.pairs = static_cast<int32_t>(pairs);
   x.choices = static_cast<int32_t>(choices); x.a_rows = static_cast<int32_t>(a_rows);
-  return int8::launch(x, true, static_cast<hipStream_t>(stream));
+  return launch(x, true, form, static_cast<hipStream_t>(stream));
+}
+
+}  // namespace
+}  // namespace int8
+}  // namespace pcamd
+
+extern "C" int pcamd_bmm_int8(const void* a, const void* b, int64_t batch, int64_t m, int64_t n, int64_t k,
+                              int64_t sab, int64_t sam, int64_t sbb, int64_t sbn, void* c, int c_dtype, int64_t scb,
+                              int64_t scm, const void* bias, int bias_dtype, int64_t sbiasb, int64_t sbiasm,
+                              int64_t sbiasn, const float* sa, int64_t ssab, int64_t ssam, const float* sb,
+                              int64_t ssbb, int64_t ssbn, int activation, void* stream) {
+  return pcamd::int8::bmm(-1, a, b, batch, m, n, k, sab, sam, sbb, sbn, c, c_dtype, scb, scm, bias, bias_dtype,
+                          sbiasb, sbiasm, sbiasn, sa, ssab, ssam, sb, ssbb, ssbn, activation, stream);
+}
+
+extern "C" int pcamd_selftest_bmm_int8(int form, const void* a, const void* b, int64_t batch, int64_t m, int64_t n,
+                                       int64_t k, int64_t sab, int64_t sam, int64_t sbb, int64_t sbn, void* c,
+                                       int c_dtype, int64_t scb, int64_t scm, const void* bias, int bias_dtype,
+                                       int64_t sbiasb, int64_t sbiasm, int64_t sbiasn, const float* sa, int64_t ssab,
+                                       int64_t ssam, const float* sb, int64_t ssbb, int64_t ssbn, int activation,
+                                       void* stream) {
+  return pcamd::int8::bmm(form, a, b, batch, m, n, k, sab, sam, sbb, sbn, c, c_dtype, scb, scm, bias, bias_dtype,
+                          sbiasb, sbiasm, sbiasn, sa, ssab, ssam, sb, ssbb, ssbn, activation, stream);
+}
+
+extern "C" int pcamd_expert_bmm_int8(const void* a, int64_t a_rows, const void* b, int64_t experts, int64_t n,
+                                     int64_t k, int64_t sam, int64_t sbe, int64_t sbn, void* c, int c_dtype,
+                                     int64_t scm, const void* bias, int bias_dtype, int64_t sbiase, int64_t sbiasn,
+                                     const float* sa, int64_t ssam, const float* sb, int64_t ssbe, int64_t ssbn,
+                                     const int32_t* starts, const int32_t* order, int64_t pairs, int64_t choices,
+                                     int activation, void* stream) {
+  return pcamd::int8::expert_bmm(-1, a, a_rows, b, experts, n, k, sam, sbe, sbn, c, c_dtype, scm, bias, bias_dtype,
+                                 sbiase, sbiasn, sa, ssam, sb, ssbe, ssbn, starts, order, pairs, choices, activation,
+                                 stream);
+}
+
+extern "C" int pcamd_selftest_expert_bmm_int8(int form, const void* a, int64_t a_rows, const void* b,
+                                              int64_t experts, int64_t n, int64_t k, int64_t sam, int64_t sbe,
+                                              int64_t sbn, void* c, int c_dtype, int64_t scm, const void* bias,
+                                              int bias_dtype, int64_t sbiase, int64_t sbiasn, const float* sa,
+                                              int64_t ssam, const float* sb, int64_t ssbe, int64_t ssbn,
+                                              const int32_t* starts, const int32_t* order, int64_t pairs,
+                                              int64_t choices, int activation, void* stream) {
+  return pcamd::int8::expert_bmm(form, a, a_rows, b, experts, n, k, sam, sbe, sbn, c, c_dtype, scm, bias, bias_dtype,
+                                 sbiase, sbiasn, sa, ssam, sb, ssbe, ssbn, starts, order, pairs, choices, activation,
+                                 stream);
 }
