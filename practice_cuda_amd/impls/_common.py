@@ -23,8 +23,9 @@ _OUT_DTYPES = (torch.bfloat16, torch.float16, torch.float32, torch.float8_e4m3fn
 def has_tangent(*tensors: Optional[torch.Tensor]) -> bool:
     """Whether one of the tensors carries a forward-mode tangent. Its requires_grad need not say so, and the kernels
     read its values alone. Outside of any dual level this is one comparison."""
-    return forward_ad._current_level >= 0 and any(
-        t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+    if forward_ad._current_level < 0:
+        return False
+    return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 class _Inference(torch.autograd.Function):
@@ -49,7 +50,7 @@ def without_gradient(what: str, inputs, *outputs: Optional[torch.Tensor]):
 
 
 def refuse_tangents(what: str, *tensors: Optional[torch.Tensor]) -> None:
-    if has_tangent(*tensors):
+    if forward_ad._current_level >= 0 and has_tangent(*tensors):
         raise RuntimeError(f"{what} has no forward-mode derivative")
 
 
