@@ -65,7 +65,8 @@ def hip_int8_quant(x: torch.Tensor, *, channel_axis: int = -2, eps: float = 1e-1
         _lib.lib().pcamd_quant_int8, x,
         x.data_ptr(), _lib.dtype_code(dtype), batch, m, n, 0 if flat else strides[0], strides[-2],
         codes.data_ptr(), m * pitch, pitch, scale.data_ptr(), m, 1, eps)
-    _refused(rc, "pcamd_quant_int8")
+    if rc != 0:
+        _refused(rc, "pcamd_quant_int8")
     if pitch != n:
         codes = codes[..., :n]
     if channel_axis == -1:
@@ -138,9 +139,9 @@ def hip_int8_bmm(
     if given or at.is_cuda:
         out = C.prepare_out(out, out_dtype, batch, m, n, at.device)
     bias, bias_strides, bias_code = C.check_bias(bias, batch, m, cols, at.device, require_n_contiguous=False)
-    C.refuse_tangents("int8_bmm", a.dequant_scale, b.dequant_scale, bias)
-    _lib.require_gpu_tensor(at, "A")
     sa, sb = a.dequant_scale, b.dequant_scale
+    C.refuse_tangents("int8_bmm", sa, sb, bias)
+    _lib.require_gpu_tensor(at, "A")
     # the scales of a quantized input stand for it: its codes are whole numbers, which require no gradient
     record = ((sa.requires_grad or sb.requires_grad or bias is not None and bias.requires_grad)
               and torch.is_grad_enabled())
