@@ -488,8 +488,8 @@ int pcamd_expert_combine_backward(const void *grad, const void *rows, int dtype,
  * c[pairs, n] are rows of a times b[e] (b[experts, n, k]; 2 n rows each with
  * PCAMD_ACT_SWIGLU), with sa[row of a], sb[e, column] and bias[e, column].
  * Row s of c takes row s of a, or where order is given row order[s] / choices
- * (a then holds pairs / choices tokens). Rows behind starts[experts] are
- * written as zeros.
+ * (a then holds pairs / choices tokens; any number where both are 0). Rows
+ * behind starts[experts] are written as zeros.
  */
 int pcamd_expert_bmm_int8(const void *a, int64_t a_rows, const void *b,
                           int64_t experts, int64_t n, int64_t k, int64_t sam,

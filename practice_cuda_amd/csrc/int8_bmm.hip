@@ -32,13 +32,17 @@ int check_operand(const char* name, const void* p, int64_t rows, int64_t stride,
   return PCAMD_OK;
 }
 
-// What a form of tiles would take, in us for k = 4096 without the launch, from the tile counts. The constants are
-// fitted to timings on MI355X (rotating inputs), us as modelled / measured:
+// What a form of tiles would take, in us, from the tile counts. The constants are fitted to timings on MI355X; us as
+// modelled / measured (rotating inputs, a captured graph of calls):
 //   rows 16 rt x 16 ct: a tile costs more with rt + ct, as its waves load that many operands;
-//     24 x 14336 x 4096: 2 x 4 15 / 14, 2 x 2 16 / 17, 4 x 4 19 / 16; 64 x 4096 x 4096: 2 x 2 11 / 10, 4 x 4 19 / 19;
-//     192 rows by 64 experts of 4096 x 7168: 1 x 2 200 / 233, 2 x 4 276 / 241
-//   128 x 128: two workgroups a CU; 512 x 14336 x 4096 42 / 42, 2048 x 4096 x 4096 48 / 45, 1024 x 4096 x 4096 30 / 30
-//   256 x 256: 2048 x 4096 x 4096 53 / 48, 4096 x 4096 x 4096 61 / 61, 8192 x 14336 x 4096 379 / 428
+//     24 x 14336 x 4096: 2 x 4 14.5 / 16.8, 2 x 2 16.4 / 19.2, 4 x 4 18.9 / 18.9;
+//     64 x 4096 x 4096: 2 x 2 10.7 / 10.5, 4 x 4 18.9 / 19.4;
+//     192 rows by 64 experts of 7168 x 4096: 1 x 2 196 / 220, 2 x 4 270 / 226
+//   128 x 128: two workgroups a CU; 512 x 14336 x 4096 43.5 / 49.3, 2048 x 4096 x 4096 48.0 / 46.4,
+//     1024 x 4096 x 4096 30.0 / 29.4
+//   256 x 256: 2048 x 4096 x 4096 53.0 / 48.6, 4096 x 4096 x 4096 61.0 / 63.4, 8192 x 14336 x 4096 379 / 432
+// Of 24 drawn plain products the chosen form took 1.03 times the fastest on average and 1.30 at worst, of 24 drawn
+// grouped ones 1.04 and 1.19.
 struct Form {
   int rows, cols;  // of C, before a gated activation halves the columns
   int rt, ct;      // of the rows kernel; 0: the tiled one
@@ -52,7 +56,8 @@ double cost(const Form& f, double tiles, double cus, double k) {
   const double rounds = tiles / cus;
   if (f.rt) {
     const double s = f.rt + f.ct, each = 1.1 * s + 0.08 * s * s;
-    // many small tiles share a CU and cover each other's start and end
+    // Many small tiles share a CU and cover each other's start and end: 68 rows by 128 experts of 3344 x 968 take 28 / 24
+    // as 1 x 2, and without the factor would go to 1 x 4, at 31 / 32.
     return 5.0 + k * each * (rounds >= 4.0 ? (s <= 3.0 ? 0.85 * rounds : rounds) : std::ceil(rounds));
   }
   if (f.rows == 128) {

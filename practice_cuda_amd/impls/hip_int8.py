@@ -120,7 +120,7 @@ def hip_int8_bmm(
     a: [B, M, K] with scales per row (channel_axis=-2), b: [B, K, N] with scales
     per column (-1), both contiguous along K, rows (columns) at multiples of 16
     bytes, as hip_int8_quant leaves them; K up to 131071, where the sums are
-    exact. bias: [B, M, N], any strides. activation: "none", "gelu", or "swiglu",
+    exact, and B up to 65535. bias: [B, M, N], any strides. activation: "none", "gelu", or "swiglu",
     which takes the first half of b's columns as gates of the second: silu(gate)
     * other, [B, M, N / 2] (bias still has N columns). There is no gradient: going
     backward is an error."""

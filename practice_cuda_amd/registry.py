@@ -19,7 +19,7 @@ import torch
 
 @dataclass
 class QuantResult:
-    """FP8 tensor plus fp32 *dequant* scale (multiply to recover values).
+    """FP8 (or int8) tensor plus fp32 *dequant* scale (multiply to recover values).
 
     granularity is "tensor", "channel" (meta["channel_axis"] in {-1, -2}) or
     "block" (meta["block_m"], meta["block_n"]); see registry.py:10-70 of the
