@@ -2,14 +2,15 @@
 launches, so what runs here is how tangents and gradients travel through the operators."""
 from __future__ import annotations
 
+import gc
+import weakref
+
 import pytest
 import torch
 from torch.autograd import forward_ad
 
 import practice_cuda_amd as pca
 from practice_cuda_amd.impls import hip_expert
-
-F64 = torch.float64
 
 
 @pytest.fixture
@@ -106,3 +107,15 @@ def test_the_gradients_have_no_tangent(plan):
         out = pca.expert_combine(forward_ad.make_dual(rows, torch.ones(6, 4)), plan, w)
         with pytest.raises(RuntimeError, match="no forward-mode derivative"):
             out.sum().backward()
+
+
+def test_nothing_is_kept_beside_the_saved_tensors(plan):
+    """What a saved-tensor hook replaces is freed with the caller's last reference, the output still there."""
+    x = torch.randn(6, 4, requires_grad=True)
+    rows, w = x * 2.0, torch.rand(3, 2)
+    last = weakref.ref(rows)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.numpy(force=True).copy(), torch.from_numpy):
+        y = pca.expert_combine(rows, plan, w)
+    del rows
+    gc.collect()
+    assert last() is None and y.requires_grad
